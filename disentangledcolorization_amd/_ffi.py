@@ -14,6 +14,8 @@ OK = 0
 ACT_NONE, ACT_RELU, ACT_LRELU, ACT_TANH = 0, 1, 2, 3
 PREC_F16X3, PREC_MX8, PREC_MX8_ALL, PREC_X2Q, PREC_MX6 = 0, 2, 3, 4, 5
 PLANE_LO, PLANE_Q, PLANE_QL, PLANE_Q6 = 1, 2, 4, 8
+F16, BF16, F32 = 0, 1, 2
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_NTK, ROTARY_PARTS = 0, 1, 2, 3
 
 
 class DiscoError(RuntimeError):
@@ -53,6 +55,30 @@ class ConvMxDesc(C.Structure):
                 ("stride", C.c_int32), ("act", C.c_int32), ("slope", C.c_float), ("out_planes", C.c_int32),
                 ("out_sexp", C.c_int32), ("out_f32", C.c_int32), ("res_planes", C.c_int32), ("res_sexp", C.c_int32), ("x2q", C.c_int32),
                 ("q6", C.c_int32), ("d2s", C.c_int32)]
+
+
+class CacheDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("layers", C.c_int32), ("pages", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32),
+                ("dim", C.c_int32), ("rows", C.c_int32), ("table_width", C.c_int32), ("layer_stride", C.c_int64), ("page_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("slot_stride", C.c_int64), ("d_k", C.c_void_p), ("d_v", C.c_void_p)]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("tokens", C.c_int32), ("heads", C.c_int32), ("dim", C.c_int32), ("rotated", C.c_int32),
+                ("interleaved", C.c_int32), ("inverse", C.c_int32), ("wide_positions", C.c_int32), ("x_token", C.c_int64), ("x_head", C.c_int64),
+                ("out_token", C.c_int64), ("out_head", C.c_int64), ("gain", C.c_double)]
+
+
+class AppendDesc(C.Structure):
+    _fields_ = [("tokens", C.c_int32), ("q_heads", C.c_int32), ("rotated", C.c_int32), ("interleaved", C.c_int32), ("wide_positions", C.c_int32),
+                ("q_token", C.c_int64), ("q_head", C.c_int64), ("k_token", C.c_int64), ("k_head", C.c_int64), ("v_token", C.c_int64),
+                ("v_head", C.c_int64), ("out_token", C.c_int64), ("out_head", C.c_int64), ("gain", C.c_double)]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [("tokens", C.c_int32), ("q_heads", C.c_int32), ("causal", C.c_int32), ("window", C.c_int32), ("max_new", C.c_int32),
+                ("max_len", C.c_int32), ("scale", C.c_float), ("q_token", C.c_int64), ("q_head", C.c_int64), ("out_token", C.c_int64),
+                ("out_head", C.c_int64)]
 
 
 # name -> (restype, argtypes); every symbol include/disco_hip.h declares
@@ -124,6 +150,16 @@ SIGNATURES = {
     "disco_op_lab_to_rgb8": (_I, [_P, _P, _I, _I, _I, _I, _I, _P]),
     "disco_op_rgb8_resize_to_lab": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "disco_op_mark_color_hints": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
+    "disco_op_rotary_frequencies": (_I, [_I, _I, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _P]),
+    "disco_op_rotary": (_I, [C.POINTER(RotaryDesc), _P, _P, _P, _P, _P]),
+    "disco_op_cache_append": (_I, [C.POINTER(CacheDesc), C.POINTER(AppendDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "disco_op_cache_attention_workspace_bytes": (_I, [C.POINTER(CacheDesc), C.POINTER(AttentionDesc), C.POINTER(_SZ)]),
+    "disco_op_cache_attention": (_I, [C.POINTER(CacheDesc), C.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "disco_op_cache_reserve": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "disco_op_cache_select": (_I, [C.POINTER(CacheDesc), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "disco_op_cache_compact": (_I, [C.POINTER(CacheDesc), _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "disco_op_cache_pages_workspace_bytes": (_SZ, [_I, _I]),
+    "disco_op_cache_copy_pages": (_I, [C.POINTER(CacheDesc), _P, _P, _I, _P]),
 }
 
 ABI_VERSION = 11      # include/disco_hip.h DISCO_ABI_VERSION this binding matches (struct layouts, entry points)

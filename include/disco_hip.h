@@ -418,6 +418,100 @@ int disco_op_lab_to_rgb8(const float *d_lab, uint8_t *d_rgb8, int n, int hp, int
 int disco_op_mark_color_hints(const float *d_gray, const float *d_target_ab, const float *d_gate, const float *d_base_ab,
                               float *d_out, int n, int h, int w, int kernel_size, void *stream);
 
+/* ---- token sequences served from a paged cache ---------------------------------------------------------------------
+ * The cache of one model: pages of `page_size` tokens, keys and values apart, bf16 or fp16.  Element (layer, page, head, slot, i) of the keys
+ * lies at d_k + layer * layer_stride + page * page_stride + head * head_stride + slot * slot_stride + i (strides in elements, the values with
+ * the same ones).  Row b of the page table (int32, rows x table_width, device) names the pages of sequence b, d_lens[b] says how many tokens
+ * it holds; the new tokens of all sequences lie behind each other and d_cu_new (int32, rows + 1) says where each sequence's begin (equal
+ * neighbours: an idle sequence).  In append and attention d_lens counts the new tokens too: the last one of sequence b has position
+ * d_lens[b] - 1.  Everything on the device is read there, nothing synchronises and nothing allocates: all entry points may be captured into a graph.
+ *
+ * What the device holds is not trusted with addresses: lengths count as 0 .. table_width * page_size, a page number outside the cache is never
+ * followed (append drops the token, attention gives NaN to the queries that see it, the page calls count it in d_info[2]). */
+#define DISCO_F16 0
+#define DISCO_BF16 1
+#define DISCO_F32 2
+
+typedef struct disco_cache_desc {
+    int32_t dtype;                             /* DISCO_F16 / DISCO_BF16 */
+    int32_t layers;                            /* layers that share the page table; append and attention use the first */
+    int32_t pages, kv_heads, page_size, dim;   /* page_size: a power of two; dim: a multiple of 8, 8 .. 256 */
+    int32_t rows, table_width;                 /* of the page table; table_width * page_size <= 2^30 */
+    int64_t layer_stride, page_stride, head_stride, slot_stride;   /* multiples of 8; d_k and d_v aligned to 16 bytes */
+    void *d_k, *d_v;
+} disco_cache_desc;
+
+/* how positions that lie behind the trained length are brought back */
+#define DISCO_ROTARY_PLAIN 0   /* f_i = base^(-2 i / dim) */
+#define DISCO_ROTARY_LINEAR 1  /* f_i / factor */
+#define DISCO_ROTARY_NTK 2     /* base * factor^(dim / (dim - 2)) in base's place: the slowest pair is stretched by factor, the fastest kept */
+#define DISCO_ROTARY_PARTS 3   /* by the turns r_i = original_length f_i / 2 pi that a pair makes over the trained length: kept above `high`,
+                                  f_i / factor below `low`, blended in between */
+/* Host call: h_inv_freq[dim / 2], radians a position. */
+int disco_op_rotary_frequencies(int dim, int scaling, double base, double factor, double original_length, double low, double high,
+                                double *h_inv_freq);
+
+typedef struct disco_rotary_desc {
+    int32_t dtype;                             /* DISCO_F16 / DISCO_BF16 / DISCO_F32 */
+    int32_t tokens, heads, dim, rotated;       /* the first `rotated` (even) of a head's dim elements turn, the others are copied */
+    int32_t interleaved;                       /* pairs (2i, 2i + 1); 0: (i, i + rotated / 2) */
+    int32_t inverse;                           /* turns back (gain still multiplies): what a gradient takes */
+    int32_t wide_positions;                    /* d_positions is int64 (0: int32) */
+    int64_t x_token, x_head, out_token, out_head;   /* strides in elements; a head's elements lie next to each other */
+    double gain;                               /* multiplies the turned elements */
+} disco_rotary_desc;
+/* out = rotation of x by positions; d_out may be d_x (with equal strides).  The angle is computed in 64 bits: positions up to 2^40 keep theirs. */
+int disco_op_rotary(const disco_rotary_desc *d, const void *d_x, const void *d_positions, const double *d_inv_freq, void *d_out, void *stream);
+
+typedef struct disco_append_desc {
+    int32_t tokens;                            /* rows of q, k, v; rows behind d_cu_new[rows] are left alone */
+    int32_t q_heads;                           /* 0: no queries */
+    int32_t rotated, interleaved;              /* as above; rotated = 0: nothing turns */
+    int32_t wide_positions;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+    double gain;
+} disco_append_desc;
+/* Turns q (into d_q_out, which may be d_q) and k by their positions and writes k and v into their pages, one launch.  d_positions: one a token,
+ * or NULL: the token's place in its sequence. */
+int disco_op_cache_append(const disco_cache_desc *c, const disco_append_desc *a, const void *d_q, const void *d_k, const void *d_v,
+                          const int32_t *d_page_table, const int32_t *d_lens, const int32_t *d_cu_new, const void *d_positions,
+                          const double *d_inv_freq, void *d_q_out, void *stream);
+
+typedef struct disco_attention_desc {
+    int32_t tokens, q_heads;                   /* q_heads a multiple of kv_heads: query head h reads key head h / (q_heads / kv_heads) */
+    int32_t causal;                            /* 1: the token at position p sees the keys 0 .. p; 0: all of its sequence */
+    int32_t window;                            /* > 0 (causal only): the keys p - window + 1 .. p */
+    int32_t max_new, max_len;                  /* bounds that the host knows of new tokens and length of one sequence, 0: none.  They choose launch
+                                                  sizes, no result goes wrong where a sequence is longer. */
+    float scale;                               /* of the scores */
+    int64_t q_token, q_head, out_token, out_head;
+} disco_attention_desc;
+/* out = softmax(scale q k^T) v of every new token over its sequence's cache; d_lse (tokens x q_heads fp32, may be NULL): the logarithm of the
+ * softmax's sum.  A token that sees no key gets zeros and -inf; rows behind d_cu_new[rows] are left alone.  Keys that a query does not see cannot
+ * reach it, whatever they hold.  A sequence's result does not depend on the others in the call. */
+int disco_op_cache_attention_workspace_bytes(const disco_cache_desc *c, const disco_attention_desc *a, size_t *bytes);
+int disco_op_cache_attention(const disco_cache_desc *c, const disco_attention_desc *a, const void *d_q, const int32_t *d_page_table,
+                             const int32_t *d_lens, const int32_t *d_cu_new, void *d_out, float *d_lse, void *d_ws, size_t ws_bytes, void *stream);
+
+/* Page calls: from a table, lengths and counts to new ones (other buffers than the old ones); entries behind a row's last page become -1.
+ * d_refs[pages]: how many rows name a page, 0 = free.  d_info[4]: free pages afterwards; pages that were missing (then nothing has changed: the new
+ * state is the old one); entries or lengths out of range; pages copied.  rows <= 16384. */
+/* Pages for the new tokens of every row (d_lens: without them, d_lens_out: with them), the lowest free numbers first, rows ascending. */
+int disco_op_cache_reserve(int rows, int table_width, int pages, int page_size, const int32_t *d_page_table, const int32_t *d_lens,
+                           const int32_t *d_refs, const int32_t *d_cu_new, int32_t *d_page_table_out, int32_t *d_lens_out, int32_t *d_refs_out,
+                           int32_t *d_info, void *stream);
+/* Row r becomes what row d_parents[r] was (-1: empty).  Rows of one parent share its full pages; of a last page that is not full one of them keeps
+ * the original (the parent itself, else the lowest) and the others get a copy of its filled slots, in all layers: new tokens never meet in a page. */
+int disco_op_cache_select(const disco_cache_desc *c, const int32_t *d_page_table, const int32_t *d_lens, const int32_t *d_parents,
+                          int32_t *d_page_table_out, int32_t *d_lens_out, int32_t *d_refs_out, int32_t *d_info, void *d_ws, size_t ws_bytes,
+                          void *stream);
+/* The n pages in use become 0 .. n - 1: the lowest page at or above n moves into the lowest free one, and so on. */
+int disco_op_cache_compact(const disco_cache_desc *c, const int32_t *d_page_table, const int32_t *d_lens, int32_t *d_page_table_out,
+                           int32_t *d_refs_out, int32_t *d_info, void *d_ws, size_t ws_bytes, void *stream);
+size_t disco_op_cache_pages_workspace_bytes(int rows, int pages);   /* of select and compact */
+/* Page d_src[i] is copied to page d_dst[i] in all layers, i < count; no page of d_dst may be among d_src.  Pairs out of range are skipped. */
+int disco_op_cache_copy_pages(const disco_cache_desc *c, const int32_t *d_src, const int32_t *d_dst, int count, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,720 @@
+"""-m gpu: the paged-cache operators (disentangledcolorization_amd/paged.py) against plain 64-bit implementations (tests/paged_reference.py).
+
+Tolerances count roundings, eps / 2 each (eps of the tensors' type):
+  rotary     one rounding of the result, and in fp32 the cosine and sine (3e-8 of the series, 2^-32 of a turn, 2^-24), the gain's rounding and three
+             operations: 8 * 2^-24 of |a| + |b| together; far positions add their angle's 64-bit rounding.
+  attention  one rounding of the result; the probabilities enter the second product rounded to the cache's type, so half a step of the weighted
+             |v|; the scores' fp32 errors (bounded by the reference from |q| |k|) and the exponential's change every weight by a factor, twice (numerator
+             and sum); fp16 probabilities below 2^-14 of the row's largest are off by at most 2^-25 of it each.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import paged_reference as R  # noqa: E402
+from disentangledcolorization_amd import _ffi, paged  # noqa: E402
+
+DEV = "cuda:0"
+BF, HF, FL = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    assert torch.cuda.is_available(), "GPU tests need a HIP device"
+    _ffi.lib()
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+# ---- rotary -----------------------------------------------------------------------------------------------------------------------------
+
+def close_turned(got, x, positions, f, gain, interleaved, inverse=False):
+    want, size = R.turned(x, positions, f, gain, interleaved, inverse)
+    angle = positions.double().abs().max().item() * f.double().max().item()
+    tol = half(x.dtype) * want.abs() + (8 * 2.0 ** -24 + angle * 2.0 ** -51) * size + torch.finfo(x.dtype).smallest_normal
+    off = (got.double().cpu() - want).abs()
+    assert (off <= tol).all(), (off - tol).max().item()
+
+
+ROTARY = [
+    # tokens, heads, dim, rotated
+    (1, 1, 2, 2), (1, 5, 64, 64), (3, 40, 128, 128), (7, 3, 80, 32), (33, 4, 96, 50), (5, 2, 65, 6), (700, 6, 64, 62), (2, 7, 256, 256), (9, 3, 24, 8), (4100, 2, 40, 40),
+    (2, 300, 8, 4), (1, 2, 512, 500),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FL])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("shape", ROTARY)
+def test_rotary(shape, interleaved, dtype):
+    tokens, heads, dim, rotated = shape
+    x = torch.randn(tokens, heads, dim, generator=gen(tokens + dim)).to(dtype).to(DEV)
+    f = paged.rotary_frequencies(rotated)
+    positions = torch.randint(0, 1 << 20, (tokens,), generator=gen(3)).to(DEV)
+    got = paged.rotary(x, positions, f, gain=1.25, interleaved=interleaved)
+    assert got.dtype == dtype and got.is_contiguous()
+    close_turned(got, x, positions, f, 1.25, interleaved)
+    assert torch.equal(got[..., rotated:], x[..., rotated:])
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_places_and_strides(interleaved):
+    """A slice of a joined projection, every alignment of its first element, another order of the axes, in place, int32 positions, negative and far ones."""
+    joined = torch.randn(19, 9, 72, generator=gen(1)).half().to(DEV)
+    f = paged.rotary_frequencies(32)
+    positions = torch.arange(-9, 10, device=DEV)
+    for at in (0, 1, 2, 3, 4, 8):
+        x = joined[:, 2:7, at:at + 64]
+        close_turned(paged.rotary(x, positions, f, interleaved=interleaved), x, positions, f, 1.0, interleaved)
+    x = joined[:, :, :64].transpose(0, 1).contiguous().transpose(0, 1)
+    got = paged.rotary(x, positions.int(), f, interleaved=interleaved)
+    close_turned(got, x, positions, f, 1.0, interleaved)
+    for far in (2 ** 31 - 1, 2 ** 40):
+        p = far - torch.arange(19, device=DEV)
+        close_turned(paged.rotary(x, p, f, interleaved=interleaved), x, p, f, 1.0, interleaved)
+    y, before = joined.clone(), joined[:, 1:4].clone()
+    out = y[:, 1:4, 2:66]
+    assert paged.rotary(out, positions, f, interleaved=interleaved, out=out) is out
+    close_turned(out, before[..., 2:66], positions, f, 1.0, interleaved)
+    y[:, 1:4, 2:66] = joined[:, 1:4, 2:66]
+    assert torch.equal(y, joined)                       # nothing else was touched
+
+
+def test_rotary_there_and_back():
+    """inverse is the transposed rotation: <y, rot(x)> = <rot'(y), x>, and without a gain it undoes the rotation."""
+    x, y = (torch.randn(50, 3, 48, generator=gen(s)).to(DEV) for s in (1, 2))
+    f, p = paged.rotary_frequencies(40, scaling="ntk", factor=4), torch.arange(50, device=DEV) * 1000
+    for inter in (False, True):
+        close_turned(paged.rotary(x, p, f, 0.9, inter, inverse=True), x, p, f, 0.9, inter, True)
+        there = paged.rotary(x, p, f, 0.9, inter).double()
+        back = paged.rotary(y, p, f, 0.9, inter, inverse=True).double()
+        a, b = (there * y).sum(), (back * x).sum()
+        assert abs(a - b) <= 16 * 2.0 ** -24 * (there.abs() * y.abs() + back.abs() * x.abs()).sum()
+        z = paged.rotary(paged.rotary(x, p, f, interleaved=inter), p, f, interleaved=inter, inverse=True)
+        assert (z - x).abs().max() <= 4 * 16 * 2.0 ** -24 * x.abs().max()
+
+
+def test_rotary_of_nothing_and_refusals():
+    f, p = paged.rotary_frequencies(8), torch.zeros(3, dtype=torch.int64, device=DEV)
+    assert paged.rotary(torch.zeros(0, 4, 8, device=DEV), p[:0], f).shape == (0, 4, 8)
+    assert paged.rotary(torch.zeros(3, 0, 8, device=DEV), p, f).shape == (3, 0, 8)
+    x = torch.zeros(3, 2, 8, device=DEV)
+    for bad in (lambda: paged.rotary(x.double(), p, f), lambda: paged.rotary(x[0], p, f), lambda: paged.rotary(x, p[:2], f), lambda: paged.rotary(x, p.float(), f),
+                lambda: paged.rotary(x, p, f.float()), lambda: paged.rotary(x.transpose(1, 2), p, f), lambda: paged.rotary(x, p, f, out=x[:2]),
+                lambda: paged.rotary(x, p, f, out=x.half()), lambda: paged.rotary(x, p.cpu(), f)):
+        with pytest.raises((ValueError, _ffi.DiscoError)):
+            bad()
+    with pytest.raises(_ffi.DiscoError, match="rotated"):
+        paged.rotary(x, p, paged.rotary_frequencies(10))
+    with pytest.raises(NotImplementedError, match="inference only"):
+        paged.rotary(x.requires_grad_(), p, f)
+    with torch.no_grad():
+        paged.rotary(x, p, f)
+
+
+# ---- a cache to work on -----------------------------------------------------------------------------------------------------------------
+
+class Served:
+    """Sequences of given lengths whose pages lie anywhere in the pool; slots that no token uses hold NaN."""
+
+    def __init__(self, lens, new, kv_heads=2, group=2, dim=64, page=16, dtype=BF, seed=0, spare=2, slot_major=False, q_scale=1.0, layers=None):
+        g, rows = gen(seed), len(lens)
+        used = [-(-n // page) for n in lens]
+        pool, width = sum(used) + spare, max(max(used), 1) + 1
+        order = torch.randperm(pool, generator=g).tolist()
+        table, at = torch.full((rows, width), -1, dtype=torch.int32), 0
+        for b, u in enumerate(used):
+            table[b, :u] = torch.tensor(order[at:at + u], dtype=torch.int32)
+            at += u
+        shape = (pool, page, kv_heads, dim) if slot_major else (pool, kv_heads, page, dim)
+        shape = shape if layers is None else (layers, *shape)
+        self.k, self.v = (torch.randn(shape, generator=g).to(dtype) for _ in range(2))
+        if slot_major:
+            self.k, self.v = self.k.transpose(-3, -2), self.v.transpose(-3, -2)
+        filled = torch.zeros(pool, page, dtype=torch.bool)
+        for b, n in enumerate(lens):
+            for i in range(used[b]):
+                filled[table[b, i], :max(0, min(page, n - i * page))] = True
+        for c in (self.k, self.v):
+            c.transpose(-3, -2)[..., ~filled, :, :] = math.nan
+        self.q = (torch.randn(sum(new), kv_heads * group, dim, generator=g) * q_scale).to(dtype)
+        self.lens, self.cu = torch.tensor(lens, dtype=torch.int32), torch.tensor([sum(new[:i]) for i in range(rows + 1)], dtype=torch.int32)
+        self.table, self.page, self.dtype, self.used, self.pool = table, page, dtype, used, pool
+        for n in ("k", "v", "q", "lens", "cu", "table"):
+            t = getattr(self, n)
+            setattr(self, n, t.to(DEV) if t.dim() < 4 or not slot_major else t.transpose(-3, -2).to(DEV).transpose(-3, -2))
+
+    def args(self):
+        return self.k, self.v, self.table, self.lens, self.cu
+
+    def refs(self):
+        refs = torch.zeros(self.pool, dtype=torch.int32)
+        for b, u in enumerate(self.used):
+            for p in self.table[b, :u].tolist():
+                refs[p] += 1
+        return refs.to(DEV)
+
+
+def close_attended(got, lse, q, k, v, table, lens, cu, **kw):
+    want, size, want_lse, off = R.attended(q, k, v, table, lens, cu, **kw)
+    n, dtype = want.shape[0], q.dtype
+    got, lse = got[:n].double().cpu(), lse[:n].double().cpu()
+    factor = 2 * off[..., None] + 2.0 ** -20
+    tiny = int(lens.max()) * 2.0 ** -25 * v.double().nan_to_num(0, 0, 0).abs().max().item() if dtype == HF else 0.0
+    tol = half(dtype) * want.abs() + (half(dtype) + factor) * size + tiny + torch.finfo(dtype).smallest_normal
+    same = (got == want) | (got.isnan() & want.isnan())
+    assert (same | ((got - want).abs() <= tol)).all(), ((got - want).abs() - tol).nan_to_num(0).max().item()
+    same = (lse == want_lse) | (lse.isnan() & want_lse.isnan())
+    assert (same | ((lse - want_lse).abs() <= off + 2.0 ** -22 * (1 + want_lse.abs()))).all()
+
+
+def check(s, **kw):
+    call = {n: kw[n] for n in ("causal", "window", "scale") if n in kw}
+    got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True, **kw)
+    torch.cuda.synchronize()
+    close_attended(got, lse, s.q, *s.args(), **call)
+    return got, lse
+
+
+# ---- attention ----------------------------------------------------------------------------------------------------------------------------
+
+ATTENTION = [
+    # lens, new, kv heads, group, dim, page
+    ([1], [1], 1, 1, 8, 16),
+    ([1], [1], 1, 1, 64, 1),
+    ([17], [1], 2, 4, 64, 16),
+    ([256], [1], 8, 1, 64, 16),
+    ([1537], [1], 2, 8, 128, 16),
+    ([700, 33, 0, 5, 512], [1, 1, 0, 1, 1], 2, 4, 128, 32),
+    ([31, 32, 33, 64, 65, 1], [5, 1, 33, 2, 65, 1], 2, 3, 64, 8),
+    ([40], [40], 1, 2, 80, 16),
+    ([300], [130], 2, 2, 128, 64),
+    ([129], [100], 1, 4, 256, 16),
+    ([333, 20], [77, 20], 1, 1, 192, 4),
+    ([200, 90], [64, 3], 2, 1, 96, 128),
+    ([500], [3], 1, 16, 32, 16),
+    ([90, 0, 0, 200, 7], [2, 0, 0, 9, 7], 3, 5, 40, 2),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("case", ATTENTION)
+def test_attention(case, dtype):
+    lens, new, kv_heads, group, dim, page = case
+    check(Served(lens, new, kv_heads, group, dim, page, dtype, seed=len(lens) + dim))
+
+
+@pytest.mark.parametrize("case", ATTENTION[2:10])
+@pytest.mark.parametrize("kw", [dict(causal=False), dict(window=1), dict(window=37), dict(window=1000), dict(scale=0.7), dict(scale=0.0), dict(scale=-0.2)])
+def test_attention_masks_and_scales(case, kw):
+    lens, new, kv_heads, group, dim, page = case
+    check(Served(lens, new, kv_heads, group, dim, page, BF, seed=5), **kw)
+
+
+@pytest.mark.parametrize("new", [1, 3, 9, 70, 300])
+def test_attention_of_a_long_history(new):
+    """Lengths at which the keys are split over workgroups; peaked and flat rows."""
+    for length, scale in ((2049, 1.0), (5000, 3.0), (12345, 0.0)):
+        s = Served([length, 100], [min(new, 20) if length > 5000 else new, 1], 1, 4, 64, 16, HF, seed=new, q_scale=scale)
+        check(s)
+
+
+def test_attention_of_a_very_long_history():
+    check(Served([70001], [1], 1, 2, 64, 16, BF, seed=3))
+
+
+@pytest.mark.parametrize("new", [1, 50])
+def test_attention_where_the_maximum_grows_late(new):
+    """Scores that rise by hundreds along the keys: what was summed first has to vanish without a trace."""
+    s = Served([900], [new], 1, 2, 64, 16, BF, seed=2)
+    s.k.mul_(0.05)
+    at = torch.arange(900, device=DEV)
+    s.k[s.table[0].long()[at // 16], 0, at % 16] += (at[:, None] / 900 * 4).to(BF)
+    s.q.copy_(s.q.abs() * 4)
+    check(s)
+    check(s, scale=-0.3)
+
+
+@pytest.mark.parametrize("slot_major", [False, True])
+def test_attention_strides(slot_major):
+    """Pages laid out slot by slot, keys and values in one pool, queries as a slice of a joined projection, a given output."""
+    s = Served([100, 37, 64], [3, 37, 1], 2, 2, 64, 16, HF, seed=1, slot_major=slot_major)
+    check(s)
+    both = torch.stack((s.k, s.v), 1)
+    assert both[:, 0].stride()[0] == 2 * both[:, 0][0].numel()
+    joined = torch.randn(41, 8, 72, generator=gen(9)).half().to(DEV)
+    joined[:, 2:6, 8:] = s.q
+    q = joined[:, 2:6, 8:]
+    room = torch.full((41, 4, 128), 7.0, dtype=HF, device=DEV)
+    got = paged.cache_attention(q, both[:, 0], both[:, 1], s.table, s.lens, s.cu, out=room[..., 64:])
+    assert got.data_ptr() == room[..., 64:].data_ptr()
+    assert torch.equal(got, paged.cache_attention(s.q, *s.args())) and (room[..., :64] == 7).all()
+
+
+def test_attention_bounds_do_not_change_results():
+    s = Served([700, 40, 0, 3000], [40, 1, 0, 2], 2, 4, 64, 16, BF, seed=8)
+    want = paged.cache_attention(s.q, *s.args())
+    for kw in (dict(max_new=40, max_len=3000), dict(max_len=3000), dict(max_new=40), dict(max_new=1, max_len=1), dict(max_new=4, max_len=100)):
+        got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True, **kw)
+        close_attended(got, lse, s.q, *s.args())
+        if kw.get("max_new") == 40 or "max_new" not in kw:
+            if kw.get("max_len", 3000) == 3000:
+                assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("new", [1, 6, 90])
+def test_a_sequence_does_not_depend_on_its_batch(new):
+    lens, news = [777, 2100, 64, 5000], [new, 1, min(new, 64), new]
+    s = Served(lens, news, 2, 4, 128, 16, BF, seed=4)
+    together = paged.cache_attention(s.q, *s.args())
+    for b in range(4):
+        a, e = int(s.cu[b]), int(s.cu[b + 1])
+        alone = paged.cache_attention(s.q[a:e], s.k, s.v, s.table[b:b + 1].contiguous(), s.lens[b:b + 1].contiguous(), ints([0, e - a]))
+        assert torch.equal(alone, together[a:e])
+
+
+def test_rows_behind_the_last_sequence_stay():
+    s = Served([50, 20], [4, 1], 2, 2, 64, 16, BF)
+    q = torch.cat((s.q, torch.full((7, 4, 64), math.nan, dtype=BF, device=DEV)))
+    out = torch.full((12, 4, 64), 3.0, dtype=BF, device=DEV)
+    paged.cache_attention(q, *s.args(), out=out)
+    assert (out[5:] == 3).all() and torch.equal(out[:5], paged.cache_attention(s.q, *s.args()))
+
+
+def test_attention_of_nothing():
+    s = Served([50, 0, 20], [0, 0, 0], 2, 2, 64, 16, BF)
+    assert paged.cache_attention(s.q, *s.args()).shape == (0, 4, 64)
+    s = Served([0, 20], [0, 1], 2, 2, 64, 16, BF)
+    check(s)
+    # more new tokens than the length holds: those before the sequence's start see nothing
+    s = Served([3, 20], [3, 1], 1, 2, 64, 16, BF)
+    q = torch.randn(6, 2, 64, generator=gen(1)).to(BF).to(DEV)
+    for cu in (ints([0, 5, 6]),):
+        got, lse = paged.cache_attention(q, s.k, s.v, s.table, s.lens, cu, return_lse=True)
+        assert (got[:2] == 0).all() and (lse[:2] == -math.inf).all()
+        close_attended(got, lse, q, s.k, s.v, s.table, s.lens, cu)
+    zero = ints([0, 0])                                  # lengths of zero with new tokens
+    got, lse = paged.cache_attention(q, s.k, s.v, s.table, zero, ints([0, 5, 6]), return_lse=True)
+    assert (got == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("new", [4, 9, 80])
+def test_what_a_query_does_not_see_cannot_reach_it(new, value):
+    """A key and value in the middle of the new tokens, or before the window, that are not finite: only the queries that see them notice."""
+    for kw, hit in ((dict(), 150 - new // 2), (dict(window=20), 150 - new - 5), (dict(window=20), 150 - new // 2)):
+        s = Served([150], [new], 1, 2, 64, 16, BF, seed=6)
+        page, slot = int(s.table[0, hit // 16]), hit % 16
+        for which in ("k", "v"):
+            clean = paged.cache_attention(s.q, *s.args(), **kw)
+            keep = getattr(s, which)[page, 0, slot].clone()
+            getattr(s, which)[page, 0, slot, 3:11] = value
+            got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True, **kw)
+            pos = torch.arange(150 - new, 150, device=DEV)
+            sees = (pos >= hit) & (pos < hit + kw.get("window", 1 << 20))
+            assert sees.any() or hit < 150 - new
+            assert torch.equal(got[~sees], clean[~sees])
+            if which == "v":
+                want = R.attended(s.q, *s.args(), **kw)[0]
+                for i in sees.nonzero()[:, 0].tolist():
+                    assert torch.equal(got[i].double().cpu().isfinite(), want[i].isfinite())
+                    assert torch.equal(got[i].isnan().cpu(), want[i].isnan())
+            elif math.isnan(value):
+                assert got[sees].isnan().all()
+            getattr(s, which)[page, 0, slot] = keep
+
+
+def test_scores_that_overflow():
+    """A row whose scores are all -inf has no softmax: NaN, unlike a row without keys.  One +inf: NaN too, as exp(inf - inf)."""
+    s = Served([40], [2], 1, 1, 64, 16, BF)
+    q = torch.zeros(2, 1, 64, dtype=BF, device=DEV)
+    s.k.nan_to_num_(0)
+    s.k[:] = 3e38
+    q[0], q[1] = -3e38, 1e-30
+    got, lse = paged.cache_attention(q, *s.args(), return_lse=True)
+    assert got[0].isnan().all() and got[1].isfinite().all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_outside_the_cache_are_not_read(new):
+    """A page number out of range gives NaN to the queries that see it and to no others, and no address is formed from it."""
+    for number in (-1, -2 ** 31, 1 << 20, 2 ** 31 - 1):
+        s = Served([120, 90], [new, new], 2, 2, 64, 16, BF, seed=new)
+        clean = paged.cache_attention(s.q, *s.args())
+        s.table[0, 6] = number                           # keys 96 .. 111
+        got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True)
+        pos = torch.arange(120 - new, 120)
+        sees = torch.cat((pos >= 96, torch.zeros(new, dtype=torch.bool))).to(DEV)
+        assert got[sees].isnan().all() and lse[sees].isnan().all()
+        assert torch.equal(got[~sees], clean[~sees])
+
+
+def test_lengths_out_of_range_are_cut():
+    s = Served([64], [1], 1, 1, 64, 16, BF, spare=0)
+    s.table = torch.cat((s.table[:, :4], s.table[:, :4]), 1).contiguous()      # capacity 128 tokens
+    want = paged.cache_attention(s.q, s.k, s.v, s.table, ints([128]), s.cu)
+    got = paged.cache_attention(s.q, s.k, s.v, s.table, ints([2 ** 31 - 1]), s.cu)
+    assert torch.equal(got, want)
+    got = paged.cache_attention(s.q, s.k, s.v, s.table, ints([-5]), s.cu)
+    assert (got == 0).all()
+
+
+def test_attention_refusals():
+    s = Served([50, 20], [4, 1], 2, 2, 64, 16, BF)
+    bad = [
+        lambda: paged.cache_attention(s.q.half(), *s.args()), lambda: paged.cache_attention(s.q[..., :32], *s.args()),
+        lambda: paged.cache_attention(s.q, s.k, s.v[:-1], s.table, s.lens, s.cu), lambda: paged.cache_attention(s.q, s.k.float(), s.v.float(), s.table, s.lens, s.cu),
+        lambda: paged.cache_attention(s.q, s.k, s.v.half(), s.table, s.lens, s.cu), lambda: paged.cache_attention(s.q, s.k, s.v, s.table.long(), s.lens, s.cu),
+        lambda: paged.cache_attention(s.q, s.k, s.v, s.table[:, ::2], s.lens, s.cu), lambda: paged.cache_attention(s.q, s.k, s.v, s.table, s.lens[:1], s.cu),
+        lambda: paged.cache_attention(s.q, s.k, s.v, s.table, s.lens, s.cu[:2]), lambda: paged.cache_attention(s.q, *s.args(), out=s.q[:2]),
+        lambda: paged.cache_attention(s.q.transpose(1, 2), *s.args()), lambda: paged.cache_attention(s.q[:, :3].contiguous(), *s.args()),
+        lambda: paged.cache_attention(s.q, *s.args(), window=-1), lambda: paged.cache_attention(s.q, *s.args(), causal=False, window=3),
+        lambda: paged.cache_attention(s.q, *s.args(), scale=math.inf), lambda: paged.cache_attention(s.q, s.k.cpu(), s.v, s.table, s.lens, s.cu),
+        lambda: paged.cache_attention(torch.zeros(5, 4, 65, dtype=BF, device=DEV)[..., 1:], *s.args())]
+    for call in bad:
+        with pytest.raises((ValueError, _ffi.DiscoError)):
+            call()
+    with pytest.raises(NotImplementedError):
+        paged.cache_attention(s.q.clone().requires_grad_(), *s.args())
+
+
+# ---- append -------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("case", [
+    # lens, new, q heads, kv heads, dim, rotated, page, interleaved
+    ([1], [1], 1, 1, 8, 8, 1, False), ([300, 0, 7, 40], [1, 0, 7, 13], 8, 2, 64, 64, 16, False), ([33, 1000], [20, 1], 5, 1, 80, 32, 32, True),
+    ([64, 65], [64, 1], 4, 4, 128, 50, 8, False), ([200, 5], [90, 2], 2, 2, 256, 256, 128, True), ([70], [9], 0, 3, 96, 0, 16, False), ([700], [600], 6, 2, 40, 6, 16, True)])
+def test_append(case, dtype):
+    lens, new, q_heads, kv_heads, dim, rotated, page, inter = case
+    s = Served(lens, new, kv_heads, 1, dim, page, dtype, seed=dim)
+    total = sum(new)
+    qkv = torch.randn(total + 2, q_heads + 2 * kv_heads, dim, generator=gen(3)).to(dtype).to(DEV)       # two rows behind the last sequence
+    q, k, v = qkv.split([q_heads, kv_heads, kv_heads], 1)
+    f = paged.rotary_frequencies(rotated) if rotated else None
+    kc, vc = s.k.clone(), s.v.clone()
+    out = torch.full((total + 2, q_heads, dim), 5.0, dtype=dtype, device=DEV) if q_heads else None
+    got = paged.cache_append(q if q_heads else None, k, v, kc, vc, s.table, s.lens, s.cu, inv_freq=f, gain=1.1, interleaved=inter, q_out=out)
+    pos = torch.cat([torch.arange(n - m, n) for n, m in zip(lens, new)]).to(DEV)
+    if q_heads:
+        assert (got[total:] == 5).all()
+        if rotated:
+            close_turned(got[:total], q[:total], pos, f, 1.1, inter)
+        else:
+            assert torch.equal(got[:total], q[:total])
+    want_k, want_v, at = s.k.clone(), s.v.clone(), 0
+    there = torch.zeros(s.pool, page, dtype=torch.bool, device=DEV)
+    for b, (n, m) in enumerate(zip(lens, new)):
+        for p in range(n - m, n):
+            pg, slot = int(s.table[b, p // page]), p % page
+            there[pg, slot] = True
+            if rotated:
+                close_turned(kc[pg, :, slot][None], k[at:at + 1], pos[at:at + 1], f, 1.1, inter)
+            else:
+                assert torch.equal(kc[pg, :, slot], k[at])
+            assert torch.equal(vc[pg, :, slot], v[at])
+            at += 1
+    for a, b in ((kc, s.k), (vc, s.v)):                   # the other slots are as they were
+        assert torch.equal(a.transpose(1, 2)[~there].nan_to_num(9), b.transpose(1, 2)[~there].nan_to_num(9))
+
+
+def test_append_positions_place_and_bad_pages():
+    """Given positions; in place; tokens whose page is out of range, or whose place lies before the sequence, are not written anywhere."""
+    s = Served([60, 30], [10, 3], 2, 1, 64, 16, BF, seed=2)
+    qkv = torch.randn(13, 6, 64, generator=gen(3)).to(BF).to(DEV)
+    q, k, v = qkv.clone().split([2, 2, 2], 1)
+    f, pos = paged.rotary_frequencies(64), torch.randint(0, 99999, (13,), generator=gen(4)).to(DEV)
+    for p in (pos, pos.int()):
+        kc, vc, qq = s.k.clone(), s.v.clone(), q.clone()
+        assert paged.cache_append(qq, k, v, kc, vc, s.table, s.lens, s.cu, inv_freq=f, positions=p, q_out=qq) is qq
+        close_turned(qq, q, pos, f, 1.0, False)
+        close_turned(kc[int(s.table[1, 1]), :, 11:14].transpose(0, 1), k[10:], pos[10:], f, 1.0, False)
+    s.table[0, 3] = 1 << 30                                # places 48 .. of the first sequence
+    kc, vc = s.k.clone(), s.v.clone()
+    paged.cache_append(q, k, v, kc, vc, s.table, ints([60, 2]), s.cu, inv_freq=f)       # and the second has one place before its start
+    same = (kc == s.k) | (kc.isnan() & s.k.isnan())
+    changed = (~same).any(-1).any(1).nonzero().tolist()   # (page, slot)
+    assert sorted(map(tuple, changed)) == sorted([(int(s.table[1, 0]), 0), (int(s.table[1, 0]), 1)])
+    paged.cache_append(None, k[:0], v[:0], kc, vc, s.table, s.lens, ints([0, 0, 0]), inv_freq=f)
+
+
+# ---- pages --------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,pages,page,width", [(1, 3, 16, 4), (5, 40, 8, 9), (70, 3000, 1, 64), (1100, 9000, 16, 16), (3, 70000, 4, 1000), (9, 64, 16, 8), (16384, 20000, 16, 2)])
+def test_reserve(rows, pages, page, width):
+    g = gen(rows)
+    budget = torch.randint(0, width * page + 1, (rows,), generator=g)
+    lens = (budget * torch.rand(rows, generator=g)).int().tolist()
+    order, table, at = torch.randperm(pages, generator=g).tolist(), [[-7] * width for _ in range(rows)], 0
+    for b in range(rows):
+        u = -(-lens[b] // page)
+        if at + u > pages * 2 // 3:
+            lens[b], u = 0, 0
+        table[b][:u] = order[at:at + u]
+        at += u
+    refs = [0] * pages
+    for p in order[:at]:
+        refs[p] = 1
+    new = [int(min(max(0, n - m), torch.randint(0, 3 * page + 1, (1,), generator=g))) if b % 7 else 0 for b, (n, m) in enumerate(zip(budget.tolist(), lens))]
+    for scale in (0, 1, 1000):                            # no new tokens, as drawn, far too many
+        n = [x * scale for x in new]
+        cu = [0]
+        for x in n:
+            cu.append(cu[-1] + x)
+        want = R.reserved(table, lens, refs, cu, page)
+        got = paged.cache_reserve(ints(table), ints(lens), ints(refs), ints(cu), page)
+        assert got[0].tolist() == want[0] and got[1].tolist() == want[1] and got[2].tolist() == want[2]
+        assert got[3].tolist() == [*want[3], 0, 0]
+
+
+def test_reserve_counts_what_is_out_of_range():
+    got = paged.cache_reserve(ints([[0, -1], [-1, -1]]), ints([99, -4]), ints([1, 0, 0, 0]), ints([0, 0, 3]), 16)
+    assert got[1].tolist() == [32, 3] and got[3].tolist() == [2, 0, 2, 0] and got[0].tolist() == [[0, -1], [1, -1]]
+
+
+def fork_state(rows, page, seed, full=False):
+    """Rows of which some share their first pages."""
+    g = gen(seed)
+    lens, table, count = [], [], 0
+    for r in range(rows):
+        if r and float(torch.rand(1, generator=g)) < 0.5:
+            o = int(torch.randint(0, r, (1,), generator=g))
+            n = lens[o] if full else max(lens[o] // page * page, lens[o] - int(torch.randint(0, 2 * page, (1,), generator=g)))
+            shared = n // page if n < lens[o] or True else 0
+            mine = list(range(count, count + -(-n // page) - shared))
+            table.append(table[o][:shared] + mine)
+        else:
+            n = int(torch.randint(0, 9 * page, (1,), generator=g))
+            mine = list(range(count, count + -(-n // page)))
+            table.append(mine)
+        count += len(mine)
+        lens.append(n)
+    return lens, table, count
+
+
+@pytest.mark.parametrize("rows,page,layers,kv_heads,dim", [(1, 16, 1, 1, 8), (6, 8, 3, 2, 64), (40, 16, 2, 1, 80), (1200, 4, 1, 1, 16)])
+@pytest.mark.parametrize("spare", [0, 3, 2000])
+def test_select(rows, page, layers, kv_heads, dim, spare):
+    g = gen(rows + spare)
+    lens, table, count = fork_state(rows, page, rows)
+    pages, width = count + spare + 1, max(max(map(len, table)), 1) + 1
+    place = torch.randperm(pages, generator=g).tolist()
+    table = [[place[p] for p in row] + [-5] * (width - len(row)) for row in table]
+    k, v = (torch.randn(layers, pages, kv_heads, page, dim, generator=g).half().to(DEV) for _ in range(2))
+    identity = list(range(rows))
+    for parents in (identity, [-1] * rows, [0] * rows, [int(x) for x in torch.randint(-1, rows, (rows,), generator=g)], identity[::-1],
+                    [p if i % 3 else max(0, i - 1) for i, p in enumerate(identity)]):
+        want = R.selected([row[:] for row in table], lens, parents, page, pages)
+        kk, vv = k.clone(), v.clone()
+        got = paged.cache_select(ints(table), ints(lens), ints(parents), kk, vv)
+        assert got[0].tolist() == want[0] and got[1].tolist() == want[1] and got[2].tolist() == want[2]
+        free, missing, copied = want[3]
+        assert got[3].tolist() == [free, missing, 0, copied]
+        for src, dst, slots in want[4]:
+            for new, old in ((kk, k), (vv, v)):
+                assert torch.equal(new[:, dst, :, :slots], old[:, src, :, :slots])
+        for new, old in ((kk, k), (vv, v)):               # nothing else
+            for src, dst, slots in want[4]:
+                new[:, dst, :, :slots] = old[:, dst, :, :slots]
+            assert torch.equal(new, old)
+
+
+def test_select_counts_what_is_out_of_range():
+    """Parents that are no rows are empty rows; page numbers outside the cache are passed on, never followed; lengths are cut."""
+    k = torch.zeros(4, 1, 16, 8, dtype=BF, device=DEV)
+    got = paged.cache_select(ints([[2, 99], [1, -3], [0, 3]]), ints([20, 20, 1000]), ints([0, 0, 7]), k, k.clone())
+    # (both rows share page 2; row 0 keeps its last "page" 99, row 1 gets the lowest free page, 0, as its copy of 99: nothing is copied)
+    assert got[0].tolist() == [[2, 99], [2, 0], [-1, -1]] and got[1].tolist() == [20, 20, 0] and got[2].tolist() == [1, 0, 2, 0]
+    assert got[3].tolist()[2] == 3 and (k == 0).all()
+    got = paged.cache_select(ints([[2, 99], [1, -3], [0, 3]]), ints([20, 20, 1000]), ints([2, -1, -1]), k, k.clone())
+    assert got[1].tolist() == [32, 0, 0] and got[0].tolist() == [[0, 3], [-1, -1], [-1, -1]] and got[3].tolist() == [2, 0, 1, 0]
+
+
+@pytest.mark.parametrize("rows,page,layers,kv_heads,dim,spare", [(1, 16, 1, 1, 8, 0), (6, 8, 3, 2, 64, 30), (40, 16, 2, 1, 80, 200), (1, 1, 1, 1, 16, 5000), (300, 4, 1, 1, 16, 9000)])
+@pytest.mark.parametrize("slot_major", [False, True])
+def test_compact(rows, page, layers, kv_heads, dim, spare, slot_major):
+    g = gen(rows + spare)
+    lens, table, count = fork_state(rows, page, rows)
+    pages, width = count + spare + 1, max(max(map(len, table)), 1) + 2
+    place = torch.randperm(pages, generator=g).tolist()
+    table = [[place[p] for p in row] + [77] * (width - len(row)) for row in table]
+    shape = (layers, pages, page, kv_heads, dim) if slot_major else (layers, pages, kv_heads, page, dim)
+    k, v = (torch.randn(shape, generator=g).to(BF).to(DEV) for _ in range(2))
+    if slot_major:
+        k, v = k.transpose(2, 3), v.transpose(2, 3)
+    want_table, want_refs, (free, moved), moves = R.compacted(table, lens, page, pages)
+    wk, wv = k.clone(), v.clone()
+    for src, dst in moves:
+        wk[:, dst], wv[:, dst] = k[:, src], v[:, src]
+    got = paged.cache_compact(ints(table), ints(lens), k, v)
+    assert got[0].tolist() == want_table and got[1].tolist() == want_refs and got[2].tolist() == [free, 0, 0, moved]
+    assert torch.equal(k, wk) and torch.equal(v, wv)
+    again = paged.cache_compact(got[0], ints(lens), k, v)
+    assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1]) and again[2].tolist() == [free, 0, 0, 0] and torch.equal(k, wk)
+
+
+def test_copy_pages():
+    k, v = (torch.randn(2, 30, 3, 8, 40, generator=gen(s)).half().to(DEV) for s in (1, 2))
+    src, dst = [0, 5, 5, 29, -1, 30, 7, 8], [1, 2, 3, 4, 9, 10, -1, 1 << 30]       # the last four have a page out of range
+    wk, wv = k.clone(), v.clone()
+    for a, b in zip(src[:4], dst[:4]):
+        wk[:, b], wv[:, b] = k[:, a], v[:, a]
+    paged.cache_copy_pages(k, v, ints(src), ints(dst))
+    paged.cache_copy_pages(k, v, ints([]), ints([]))
+    assert torch.equal(k, wk) and torch.equal(v, wv)
+    paged.cache_copy_pages(k[0], v[0], ints([12]), ints([13]))
+    assert torch.equal(k[0, 13], k[0, 12]) and not torch.equal(k[1, 13], k[1, 12])
+
+
+# ---- all of them together -----------------------------------------------------------------------------------------------------------------
+
+class Model:
+    """Sequences grown step by step on a paged cache, and beside it their keys and values as plain lists."""
+
+    def __init__(self, rows, pages, width, layers=2, kv_heads=2, group=2, dim=64, page=8, dtype=HF):
+        self.table, self.lens, self.refs = ints([[-1] * width] * rows), ints([0] * rows), ints([0] * pages)
+        self.k, self.v = (torch.full((layers, pages, kv_heads, page, dim), math.nan, dtype=dtype, device=DEV) for _ in range(2))
+        self.f = paged.rotary_frequencies(dim)
+        self.plain = [[(torch.zeros(0, kv_heads, dim, dtype=dtype), torch.zeros(0, kv_heads, dim, dtype=dtype)) for _ in range(layers)] for _ in range(rows)]
+        self.rows, self.layers, self.kv_heads, self.heads, self.dim, self.page, self.dtype = rows, layers, kv_heads, group * kv_heads, dim, page, dtype
+
+    def step(self, new, seed):
+        cu = ints([sum(new[:i]) for i in range(len(new) + 1)])
+        self.table, self.lens, self.refs, info = paged.cache_reserve(self.table, self.lens, self.refs, cu, self.page)
+        assert info.tolist()[1:3] == [0, 0]
+        for layer in range(self.layers):
+            qkv = torch.randn(sum(new), self.heads + 2 * self.kv_heads, self.dim, generator=gen(seed * 10 + layer)).to(self.dtype).to(DEV)
+            q, k, v = qkv.split([self.heads, self.kv_heads, self.kv_heads], 1)
+            before = [len(r[layer][0]) for r in self.plain]
+            pos = torch.cat([torch.arange(b, b + n) for b, n in zip(before, new)]).to(DEV)
+            q = paged.cache_append(q, k, v, self.k[layer], self.v[layer], self.table, self.lens, cu, inv_freq=self.f)
+            turned = paged.rotary(k, pos, self.f)
+            at = 0
+            for r, n in enumerate(new):
+                a, b = self.plain[r][layer]
+                self.plain[r][layer] = (torch.cat((a, turned[at:at + n].cpu())), torch.cat((b, v[at:at + n].cpu())))
+                at += n
+            got, lse = paged.cache_attention(q, self.k[layer], self.v[layer], self.table, self.lens, cu, return_lse=True)
+            self.compare(got, lse, q, layer, new)
+
+    def compare(self, got, lse, q, layer, new):
+        at = 0
+        for r, n in enumerate(new):
+            if n:                                         # the row's own keys and values as a cache of one page
+                a, b = (x.transpose(0, 1)[None] for x in self.plain[r][layer])
+                close_attended(got[at:at + n], lse[at:at + n], q[at:at + n], a, b, torch.zeros(1, 1, dtype=torch.int32), torch.tensor([a.shape[2]]), torch.tensor([0, n]))
+            at += n
+
+    def select(self, parents):
+        self.table, self.lens, self.refs, info = paged.cache_select(self.table, self.lens, ints(parents), self.k, self.v)
+        assert info.tolist()[1:3] == [0, 0]
+        layers = range(self.layers)
+        empty = [tuple(x[:0] for x in self.plain[0][layer]) for layer in layers]
+        self.plain = [[self.plain[p][layer] if p >= 0 else empty[layer] for layer in layers] for p in parents]
+
+
+def test_a_run_of_all_operators():
+    """Prompts, steps, forks, an ended sequence whose row is used again, a compaction, steps: at every step attention sees what each sequence has been told."""
+    m = Model(5, 60, 12)
+    m.step([13, 0, 30, 1, 8], 1)
+    m.step([1, 0, 1, 1, 1], 2)
+    m.select([0, 0, 2, 2, 0])
+    m.step([1, 1, 1, 1, 1], 3)
+    m.select([3, 1, -1, 3, 1])
+    m.step([2, 1, 19, 5, 1], 4)
+    live = int((m.refs > 0).sum())
+    m.table, m.refs, info = paged.cache_compact(m.table, m.lens, m.k, m.v)
+    assert info.tolist()[:3] == [60 - live, 0, 0] and (m.refs[:live] > 0).all() and (m.refs[live:] == 0).all()
+    m.step([1, 1, 1, 1, 1], 5)
+    m.select([4, 3, 2, 1, 0])
+    m.step([1, 7, 0, 1, 1], 6)
+    for _ in range(3):
+        m.step([1] * 5, 7 + _)
+
+
+def test_a_captured_step():
+    """reserve, append, attention and select in one graph, replayed with other inputs in the same places, with eager work in between: every replay equals the eager result."""
+    lens, new, page = [700, 33, 0, 64, 90], [1, 3, 0, 1, 20], 16
+    s = Served(lens, [0] * 5, 2, 4, 64, page, BF, seed=1, spare=20)
+    s.table = torch.cat((s.table, torch.full((5, 3), -1, dtype=torch.int32, device=DEV)), 1).contiguous()
+    cu, refs, f = ints([0, 1, 4, 4, 5, 25]), s.refs(), paged.rotary_frequencies(64)
+    parents = ints([0, 0, 3, 3, 4])
+    qkv = torch.randn(25, 12, 64, generator=gen(2)).to(BF).to(DEV)
+    k0, v0 = s.k.clone(), s.v.clone()
+
+    def step():
+        q, k, v = qkv.split([8, 2, 2], 1)
+        table, lens, r, info = paged.cache_reserve(s.table, s.lens, refs, cu, page)
+        q = paged.cache_append(q, k, v, s.k, s.v, table, lens, cu, inv_freq=f)
+        out = paged.cache_attention(q, s.k, s.v, table, lens, cu)
+        return (out, *paged.cache_select(table, lens, parents, s.k, s.v), info)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(4):
+        qkv.copy_(torch.randn(25, 12, 64, generator=gen(10 + i)).to(BF))
+        s.k.copy_(k0)
+        s.v.copy_(v0)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in outs] + [s.k.clone(), s.v.clone()]
+        s.k.copy_(k0)
+        s.v.copy_(v0)
+        want = [*step(), s.k, s.v]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a.nan_to_num(7) if a.is_floating_point() else a, b.nan_to_num(7) if b.is_floating_point() else b)
+
+
+def test_other_streams_and_calls_at_once():
+    """Each call runs on the current stream; calls on several streams at once have workspaces of their own."""
+    s = [Served([3000 + 7 * i, 40], [1, 30], 2, 4, 64, 16, BF, seed=i) for i in range(4)]
+    want = [paged.cache_attention(x.q, *x.args()) for x in s]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in s], [None] * 4
+    for _ in range(3):
+        for i, (x, st) in enumerate(zip(s, streams)):
+            with torch.cuda.stream(st):
+                got[i] = paged.cache_attention(x.q, *x.args())
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def test_offsets_beyond_32_bits():
+    """A pool of more than 4 GiB a side: the last pages are read, written and copied where they are."""
+    page, kv_heads, dim = 128, 8, 256
+    pages = (1 << 32) // (page * kv_heads * dim * 2) + 9
+    k, v = (torch.empty(pages, kv_heads, page, dim, dtype=HF, device=DEV) for _ in range(2))
+    for c, seed in ((k, 1), (v, 2)):
+        c[-3:].copy_(torch.randn(3, kv_heads, page, dim, generator=gen(seed)).half())
+        c[:3].zero_()
+    table, lens, cu = ints([[pages - 1, pages - 3]]), ints([200]), ints([0, 2])
+    q = torch.randn(2, kv_heads, dim, generator=gen(3)).half().to(DEV)
+    got, lse = paged.cache_attention(q, k, v, table, lens, cu, return_lse=True)
+    small = torch.stack((k[-1], k[-3])), torch.stack((v[-1], v[-3]))
+    close_attended(got, lse, q, *small, torch.tensor([[0, 1]]), lens, cu)
+    new_k, new_v = (torch.randn(2, kv_heads, dim, generator=gen(s)).half().to(DEV) for s in (4, 5))
+    paged.cache_append(None, new_k, new_v, k, v, table, lens, cu)
+    assert torch.equal(k[-3, :, 70], new_k[0]) and torch.equal(v[-3, :, 71], new_v[1])
+    t, r, info = paged.cache_compact(table, lens, k, v)
+    assert t.tolist() == [[1, 0]] and torch.equal(k[1], k[-1]) and torch.equal(v[0], v[-3])
