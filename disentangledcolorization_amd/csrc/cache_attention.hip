@@ -1,81 +1,769 @@
 // cache_attention.hip - attention of new tokens over a paged cache.
+//
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(c q.k_j - m),   c = scale log2 e,   m: a maximum of the row so far
+//
+// One pass over the keys.  The rows that share a key head - the queries of its group, for all new tokens of a sequence - form the rows of one
+// matrix (row = token * group + head in group), so that keys and values are read once for all of them.  Both products run on the matrix cores
+// in transposed form: S^T = K Q^T puts one row's scores into one lane's registers, where maximum, exponential and sum need no exchange
+// but that between the lanes of a column, and the registers that hold the probabilities are in place the operand of O^T = V^T P^T (their key order
+// is the accumulator's; V^T is read in the same order by the transposing LDS read).
+//
+// Two forms, chosen by a sequence's own rows (new tokens * group), so that its result does not depend on what else is in the call:
+//   few rows   (cache_attention_few_kernel)   16 rows a workgroup, its four waves deal 32-key tiles: bound by reading the cache
+//   many rows  (cache_attention_many_kernel)  128 rows a workgroup, 32 a wave, keys and values staged in LDS for all four: bound by the matrix
+//                                             cores, the exponentials and LDS together
+// Where a sequence alone does not fill the GPU its keys are split; the parts (m, sum, o in fp32) are joined by cache_attention_join_kernel.
+//
+// A tile that some row sees only in part, or that has a page outside the cache, takes the masked path: scores of unseen keys are replaced (never
+// added to), and values that are not finite are kept out of the product and given to the rows that see them.
+#include <type_traits>
 #include "paged.h"
 
 namespace disco {
 
 namespace {
 
+typedef __bf16 bf16;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Mat;
+template <> struct Mat<f16> {
+    typedef f16x8 x8;
+    static constexpr uint32_t INF = 0x7c00, ONE = 0x3c00;
+    // probabilities below 2^-14 lose bits in fp16, so all of a row are 2^6 larger (at most 2^14: see the rescale)
+    static constexpr float BIAS = 6.f;
+    static __device__ __forceinline__ f32x16 mul(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<bf16> {
+    typedef bf16 x8 __attribute__((ext_vector_type(8)));
+    static constexpr uint32_t INF = 0x7f80, ONE = 0x3f80;
+    static constexpr float BIAS = 0.f;
+    static __device__ __forceinline__ f32x16 mul(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
 struct AttnArgs {
     const char *q, *k, *v; char* out; float* lse;
+    float *part_o; float2* part_ml;                                // of a row (token * q_heads + head) and a split
     const int *table, *lens, *cu_new;
     long q_token, q_head, out_token, out_head, page_stride, head_stride, slot_stride;    // bytes
     int tokens, q_heads, kv_heads, group, dim, rows, width, pages, page_shift, causal, window;
-    float scale;
+    int splits;                                                    // parts of a row that the workspace has room for
+    int few;                                                       // sequences of at most so many rows take the few-rows form
+    float c;                                                       // |scale| log2 e, not 0
+    int negate;                                                    // scale < 0: the queries change sign instead
 };
 
-// One wave an output row, 64 keys at a time: lane = key for the scores, lane = elements for the sums
-template <typename T>
-__global__ __launch_bounds__(64) void cache_attention_kernel(AttnArgs a) {
-    const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-    const int b = seq_of_token(a.cu_new, a.rows, token);
-    if (b >= a.rows) return;
-    const int first = a.cu_new[b], n = a.cu_new[b + 1] - first;
-    const int len = clamp_len(a.lens[b], a.width << a.page_shift), p = len - n + (token - first);
-    const int end = a.causal ? min(len, p + 1) : len, begin = a.window > 0 ? max(0, p - a.window + 1) : 0;
-    const T* q = (const T*)(a.q + token * a.q_token + head * a.q_head);
-    const long at_head = (head / a.group) * a.head_stride;
-    float m = -INFINITY, l = 0, o[4] = {0, 0, 0, 0};
-    for (int k0 = begin; k0 < end; k0 += 64) {
-        const int key = k0 + lane;
-        float s = -INFINITY;
-        long at = 0;
-        bool bad = false;
-        if (key < end) {
-            const int page = a.table[(long)b * a.width + (key >> a.page_shift)];
-            bad = page < 0 || page >= a.pages;
-            at = (bad ? 0 : page * a.page_stride) + (key & ((1 << a.page_shift) - 1)) * a.slot_stride + at_head;
-            const T* kr = (const T*)(a.k + at);
-            float d = 0;
-            for (int i = 0; i < a.dim; ++i) d = fmaf((float)q[i], (float)kr[i], d);
-            s = bad ? NAN : d * a.scale;
+constexpr int FEW_ROWS = 16, MANY_ROWS = 128;
+constexpr float LN2 = 0.6931471805599453f;
+
+// ---- how a sequence is cut ------------------------------------------------------------------------------------------------------------
+struct Cut { int tiles, splits, begin, chunk; };
+
+// parts of a sequence's keys; grows with them
+// few rows: a workgroup's waves take 128 keys a round, and up to 512 keys (4 us) one workgroup is done sooner than two and a join; 64 parts of 8 key
+//           heads are two workgroups a CU
+// many rows: as many parts as make 256 workgroups of the sequence, of at least 512 keys (a part costs a write and a read of its rows in fp32)
+__host__ __device__ __forceinline__ int splits_of(bool few, int tiles, int keys, int kv_heads) {
+    if (few) return keys <= 512 ? 1 : (keys > 64 * 256 ? 64 : (keys + 255) / 256);
+    const int units = tiles * kv_heads;
+    int s = units >= 256 ? 1 : 256 / units;
+    if (s > 8) s = 8;
+    const int by_keys = keys <= 512 ? 1 : (keys + 511) / 512;
+    return s < by_keys ? s : by_keys;
+}
+
+// keys that some new token of the sequence sees: begin (a multiple of 64) .. len; every part takes `chunk` of them, a multiple of 128
+__host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv_heads, int window, int few, int most) {
+    Cut u;
+    const int rows = n * group;
+    const bool is_few = rows <= few;
+    u.begin = window > 0 && len - n - window + 1 > 0 ? (len - n - window + 1) & ~63 : 0;
+    const int keys = len - u.begin;
+    u.tiles = is_few ? (rows + FEW_ROWS - 1) / FEW_ROWS : (rows + MANY_ROWS - 1) / MANY_ROWS;
+    int s = splits_of(is_few, u.tiles, keys, kv_heads);
+    if (s > most) s = most;
+    u.chunk = ((keys + s - 1) / s + 127) & ~127;
+    if (u.chunk < 128) u.chunk = 128;
+    u.splits = (keys + u.chunk - 1) / u.chunk;
+    if (u.splits < 1) u.splits = 1;
+    return u;
+}
+
+struct Unit { int b, n, len, first, tile, split, head; Cut cut; };
+
+// unit number `want` of the form FEW over all sequences (key head fastest, then split, then tile - the last, longest tiles first); false behind the last.
+// Every lane of the wave calls it and gets the same.
+template <bool FEW>
+__device__ __forceinline__ bool find_unit(const AttnArgs& a, int want, Unit& u) {
+    const int lane = threadIdx.x & 63, capacity = a.width << a.page_shift;
+    int left = want;
+    for (int b0 = 0; b0 < a.rows; b0 += 64) {
+        const int b = b0 + lane;
+        int n = 0, len = 0, first = 0, units = 0;
+        Cut cut{};
+        if (b < a.rows) {
+            first = a.cu_new[b];
+            n = a.cu_new[b + 1] - first;
+            len = clamp_len(a.lens[b], capacity);
+            if (first < 0 || n < 0 || n > a.tokens || first > a.tokens - n) n = 0;       // (not offsets)
+            if (n > 0 && (n * (long)a.group <= a.few) == FEW) {
+                cut = cut_of(n, len, a.group, a.kv_heads, a.window, a.few, a.splits);
+                units = cut.tiles * cut.splits * a.kv_heads;
+            }
         }
-        float top = s;
-        for (int i = 32; i; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
-        const float now = fmaxf(m, top), back = now == -INFINITY ? 1.f : expf(m - now), pr = key < end ? expf(s - now) : 0.f;
-        float sum = pr;
-        for (int i = 32; i; i >>= 1) sum += __shfl_xor(sum, i);
-        l = l * back + sum;
+        int upto = units;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int x = __shfl_up(upto, d);
+            if (lane >= d) upto += x;
+        }
+        const unsigned long long here = __ballot(upto > left);
+        if (here) {
+            const int at = __ffsll((long long)here) - 1;
+            u.b = b0 + at;
+            u.n = __builtin_amdgcn_readlane(n, at);
+            u.len = __builtin_amdgcn_readlane(len, at);
+            u.first = __builtin_amdgcn_readlane(first, at);
+            u.cut.tiles = __builtin_amdgcn_readlane(cut.tiles, at);
+            u.cut.splits = __builtin_amdgcn_readlane(cut.splits, at);
+            u.cut.begin = __builtin_amdgcn_readlane(cut.begin, at);
+            u.cut.chunk = __builtin_amdgcn_readlane(cut.chunk, at);
+            int x = left - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(units, at));
+            u.head = x % a.kv_heads; x /= a.kv_heads;
+            u.split = x % u.cut.splits;
+            u.tile = u.cut.tiles - 1 - x / u.cut.splits;
+            return true;
+        }
+        left -= __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
+// ---- pieces of both forms -----------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// 4 x 16 elements of LDS, transposed on the way: in each group of 16 lanes, lane i names the four elements at row i / 4, columns 4 (i % 4) .. + 3
+// of the group's block and receives rows 0 .. 3 of column i
+__device__ __forceinline__ s16x4 read_transposed(const char* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
+template <typename T>
+__device__ __forceinline__ typename Mat<T>::x8 join(s16x4 a, s16x4 b) {
+    const s16x8 x = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(typename Mat<T>::x8, x);
+}
+
+// Halves of a word, both at once: 0x8000 where the magnitude is above `most`
+__device__ __forceinline__ uint32_t above(uint32_t w, uint32_t most) { return ((w & 0x7fff7fffu) + (0x7fffu - most) * 0x10001u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t word(uint4 w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
+
+// not 0 where one of the lane's eight values is infinite or NaN
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(typename Mat<T>::x8 x) {
+    const uint4 w = __builtin_bit_cast(uint4, x);
+    return above(w.x, Mat<T>::INF - 1) | above(w.y, Mat<T>::INF - 1) | above(w.z, Mat<T>::INF - 1) | above(w.w, Mat<T>::INF - 1);
+}
+
+// Values that are not finite, in a tile that not every row sees whole: 0 * inf would give NaN to rows that do not see them.  The finite ones are multiplied;
+// then, for each of NaN, inf and -inf, a product of indicators (which elements of V are it, which keys the row sees) counts what a row sees.
+template <typename T, typename Acc>
+__device__ __forceinline__ Acc multiply_seen(typename Mat<T>::x8 v, typename Mat<T>::x8 p, uint32_t seen, Acc o) {
+    typedef typename Mat<T>::x8 x8;
+    const uint4 w = __builtin_bit_cast(uint4, v);
+    uint32_t clean[4], rows[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t y = word(w, i);
+        clean[i] = y & ~((above(y, Mat<T>::INF - 1) >> 15) * 0xffffu);
+        rows[i] = ((seen >> (2 * i) & 1) | (seen >> (2 * i + 1) & 1) << 16) * Mat<T>::ONE;
+    }
+    o = Mat<T>::mul(__builtin_bit_cast(x8, uint4{clean[0], clean[1], clean[2], clean[3]}), p, o);
+    const x8 who = __builtin_bit_cast(x8, uint4{rows[0], rows[1], rows[2], rows[3]});
+#pragma unroll 1
+    for (int kind = 0; kind < 3; ++kind) {
+        uint32_t is[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t y = word(w, i), nan = above(y, Mat<T>::INF), inf = above(y, Mat<T>::INF - 1) & ~nan;
+            is[i] = ((kind == 0 ? nan : (kind == 1 ? inf & ~y : inf & y)) >> 15) * Mat<T>::ONE;
+        }
+        Acc count;
+#pragma unroll
+        for (int r = 0; r < (int)(sizeof(Acc) / 4); ++r) count[r] = 0;
+        count = Mat<T>::mul(__builtin_bit_cast(x8, uint4{is[0], is[1], is[2], is[3]}), who, count);
+        const float add = kind == 0 ? __builtin_nanf("") : (kind == 1 ? INFINITY : -INFINITY);
+#pragma unroll
+        for (int r = 0; r < (int)(sizeof(Acc) / 4); ++r) if (count[r] > 0) o[r] += add;
+    }
+    __builtin_amdgcn_sched_barrier(0);                             // (one at a time: this path is rare, its registers are not)
+    return o;
+}
+
+// What a wave keeps of its rows while it walks along the keys (a lane: of its own row): the maximum in use, in log2 units, and the sum of the keys that
+// this lane saw.
+struct Run {
+    float m = -INFINITY, l = 0.f;
+    // A tile's largest score `top` (log2 units, the same in all lanes of the row).  The accumulators are rescaled only where the maximum in use is
+    // more than 2^8 too small, which after a few tiles hardly happens; returns whether some lane asks for it, and the factor.
+    __device__ __forceinline__ bool rises(float top, float& back) {
+        const bool up = top > m + 8.f;
+        if (!__any(up)) return false;
+        const float now = fmaxf(m, top);
+        back = now == -INFINITY ? 1.f : exp2_of(m - now);
         m = now;
+        l *= back;
+        return true;
+    }
+    template <typename T> __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m - Mat<T>::BIAS; }
+};
+
+template <typename T> struct Quad { T e[4]; };
+
+// ---- few rows -------------------------------------------------------------------------------------------------------------------------------
+// A wave takes every fourth 32-key tile of the workgroup's range.  Keys go from memory straight into the operand (lane: key lane % 16, 8 elements at
+// 32 ks + 8 (lane / 16)); values go through registers into the wave's own piece of LDS, from where they are read transposed.  The next tile's
+// loads are in flight under the current tile.  No barrier but for the join of the four waves at the end.
+template <typename T, int DP> struct Few {
+    static constexpr int VROW = DP * 2 + 32;                       // (rows 32 bytes apart in bank phase)
+    static constexpr int OROW = DP + 4;                            // floats of a row that is joined
+    static constexpr int WAVE = 32 * VROW > 16 * OROW * 4 ? 32 * VROW : 16 * OROW * 4;
+};
+
+// One unit.  ODD: the form that keeps values which are not finite, and pages outside the cache, from the rows that do not see them; without it returns whether
+// there were any (then the unit is done again with it).  Both add the same products in the same order.
+template <typename T, int DP, bool ODD>
+__device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, char* lds, float (&part_m)[4][16], float (&part_l)[4][16]) {
+    typedef typename Mat<T>::x8 x8;
+    constexpr int KS = DP / 32, DB = DP / 16, NV = DP / 16, VROW = Few<T, DP>::VROW, OROW = Few<T, DP>::OROW, WAVE = Few<T, DP>::WAVE;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
+    char* mine = lds + wave * WAVE;
+    const int head_bytes = a.dim * 2;
+    const int rows = u.n * a.group;
+    // this lane's row: its token, its head, its position
+    const int row = u.tile * FEW_ROWS + col, row_in = row < rows ? row : rows - 1;
+    const int token = row_in / a.group, head = u.head * a.group + (row_in - token * a.group);
+    const int pos = a.causal ? u.len - u.n + token : u.len - 1;
+    const int last_token = (min(u.tile * FEW_ROWS + FEW_ROWS, rows) - 1) / a.group, first_token = u.tile * FEW_ROWS / a.group;
+    const int high = a.causal ? u.len - u.n + last_token : u.len - 1, low = a.causal ? u.len - u.n + first_token : u.len - 1;
+    const int begin = u.cut.begin + u.split * u.cut.chunk, end = min(min(begin + u.cut.chunk, u.len), high + 1);
+    x8 q[KS];
+    {
+        const char* p = a.q + (u.first + token) * a.q_token + head * a.q_head;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= back;
-        const int there = min(64, end - k0);
-        for (int j = 0; j < there; ++j) {
-            const float w = __shfl(pr, j);
-            const T* vr = (const T*)(a.v + __shfl(at, j));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) if (lane + 64 * i < a.dim) o[i] = fmaf(w, (float)vr[lane + 64 * i], o[i]);
+        for (int ks = 0; ks < KS; ++ks) {
+            uint4 w = uint4{0, 0, 0, 0};
+            if ((32 * ks + 8 * g) * 2 < head_bytes) w = *(const uint4*)(p + (32 * ks + 8 * g) * 2);
+            if (a.negate) { w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u; }
+            q[ks] = __builtin_bit_cast(x8, w);
         }
     }
-    T* out = (T*)(a.out + token * a.out_token + head * a.out_head);
+    f32x4 o[DB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) if (lane + 64 * i < a.dim) out[lane + 64 * i] = (T)(end > begin ? o[i] / l : 0.f);
-    if (a.lse && lane == 0) a.lse[(long)token * a.q_heads + head] = end > begin ? m + logf(l) : -INFINITY;
+    for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
+    Run run;
+    uint32_t odd = 0;
+    const int* table = a.table + (long)u.b * a.width;
+    const long head_at = u.head * a.head_stride;
+    const int slots = (1 << a.page_shift) - 1;
+    // pages of the 32 keys of a tile, one a lane (twice)
+    auto pages_at = [&](int k0) { return table[min(k0 + (lane & 31), end - 1) >> a.page_shift]; };
+    auto at = [&](int page, int key) {
+        const int p = (unsigned)page < (unsigned)a.pages ? page : 0;
+        return p * a.page_stride + (min(key, end - 1) & slots) * a.slot_stride + head_at;
+    };
+    uint4 kf[2][KS], vf[NV];
+    auto fetch_k = [&](int k0, int pg) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const char* p = a.k + at(__shfl(pg, 16 * t + col), k0 + 16 * t + col);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int byte = (32 * ks + 8 * g) * 2;
+                kf[t][ks] = byte < head_bytes ? *(const uint4*)(p + byte) : uint4{0, 0, 0, 0};
+            }
+        }
+    };
+    auto fetch_v = [&](int k0, int pg) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int piece = i * 64 + lane, r = piece / (DP / 8), byte = (piece - r * (DP / 8)) * 16;
+            const long p = at(__shfl(pg, r), k0 + r);
+            vf[i] = byte < head_bytes ? *(const uint4*)(a.v + p + byte) : uint4{0, 0, 0, 0};
+        }
+    };
+    int k0 = begin + 32 * wave, pg = 0, pg_next = 0;
+    if (k0 < end) {
+        pg = pages_at(k0);
+        pg_next = pages_at(k0 + 128);
+        fetch_k(k0, pg);
+        fetch_v(k0, pg);
+    }
+    for (; k0 < end; k0 += 128) {
+        const uint32_t bad = (uint32_t)__ballot((unsigned)pg >= (unsigned)a.pages);
+        const bool whole = k0 + 32 <= end && k0 + 31 <= low && (a.window == 0 || k0 > high - a.window) && (!ODD || bad == 0);
+        if (!ODD) odd |= bad;
+        f32x4 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            s[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s[t] = Mat<T>::mul(__builtin_bit_cast(x8, kf[t][ks]), q[ks], s[t]);
+        }
+        const bool more = k0 + 128 < end;
+        if (more) fetch_k(k0 + 128, pg_next);
+        uint32_t seen = 0xff;                                  // of this lane's eight keys
+        if (!whole) {
+            seen = 0;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int in_tile = 16 * t + 4 * g + r, key = k0 + in_tile;
+                    const bool sees = key < end && key <= pos && (a.window == 0 || key > pos - a.window);
+                    if (ODD && sees) seen |= 1u << (4 * t + r);
+                    s[t][r] = !sees ? -INFINITY : (ODD && (bad >> in_tile & 1) ? __builtin_nanf("") : s[t][r]);
+                }
+        }
+        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        float back;
+        if (run.rises(top * a.c, back)) {
+#pragma unroll
+            for (int i = 0; i < DB; ++i) o[i] *= back;
+        }
+        const float base = run.base<T>();
+        x8 p;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = exp2_of(fmaf(s[t][r], a.c, -base));
+                run.l += e;
+                p[4 * t + r] = (T)e;
+            }
+        // the tile's values into LDS; a wave's LDS operations take place in order
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int piece = i * 64 + lane, r = piece / (DP / 8), byte = (piece - r * (DP / 8)) * 16;
+            *(uint4*)(mine + r * VROW + byte) = vf[i];
+        }
+        if (more) {
+            fetch_v(k0 + 128, pg_next);
+            pg = pg_next;
+            pg_next = pages_at(k0 + 256);
+        }
+        __builtin_amdgcn_wave_barrier();
+        const char* vt = mine + (4 * g + (col >> 2)) * VROW + (col & 3) * 8;
+        auto value = [&](int i) { return join<T>(read_transposed(vt + i * 32), read_transposed(vt + 16 * VROW + i * 32)); };
+        if (!ODD || whole) {
+#pragma unroll
+            for (int i = 0; i < DB; ++i) {
+                const x8 v = value(i);
+                if (!ODD && !whole) odd |= not_finite<T>(v);
+                o[i] = Mat<T>::mul(v, p, o[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < DB; ++i) o[i] = multiply_seen<T>(value(i), p, seen, o[i]);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    run.l += __shfl_xor(run.l, 16);
+    run.l += __shfl_xor(run.l, 32);
+    // the four waves' rows: o to LDS (over the values), then every thread joins four elements of a row at a time
+    float* om = (float*)mine;
+#pragma unroll
+    for (int i = 0; i < DB; ++i) *(f32x4*)(om + col * OROW + 16 * i + 4 * g) = o[i];
+    if (g == 0) { part_m[wave][col] = run.m; part_l[wave][col] = run.l; }
+    __syncthreads();
+    for (int x = threadIdx.x; x < 16 * (DP / 4); x += 256) {
+        const int r = x / (DP / 4), d = (x - r * (DP / 4)) * 4, rr = u.tile * FEW_ROWS + r;
+        if (rr >= rows || d >= a.dim) continue;
+        float m = fmaxf(fmaxf(part_m[0][r], part_m[1][r]), fmaxf(part_m[2][r], part_m[3][r])), l = 0;
+        f32x4 y = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = part_m[w][r] == -INFINITY ? (part_l[w][r] == 0.f ? 0.f : 1.f) : exp2_of(part_m[w][r] - m);
+            if (f != 0.f) {                                    // (a wave that saw nothing of the row; NaN is not 0)
+                l += f * part_l[w][r];
+                y += f * *(const f32x4*)((const float*)(lds + w * WAVE) + r * OROW + d);
+            }
+        }
+        const int tok = rr / a.group, h = u.head * a.group + (rr - tok * a.group);
+        const long t = u.first + tok, at_row = t * a.q_heads + h;
+        if (u.cut.splits > 1) {
+            const long slot = at_row * a.splits + u.split;
+            *(f32x4*)(a.part_o + slot * a.dim + d) = y;
+            if (d == 0) a.part_ml[slot] = float2{m, l};
+        } else {
+            const int p = a.causal ? u.len - u.n + tok : u.len - 1;
+            const bool none = p < 0;
+            const float f = none ? 0.f : 1.f / l;
+            Quad<T> z;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z.e[i] = (T)(none ? 0.f : y[i] * f);
+            *(Quad<T>*)(a.out + t * a.out_token + h * a.out_head + d * 2) = z;
+            if (a.lse && d == 0) a.lse[at_row] = none ? -INFINITY : ((m == -INFINITY ? 0.f : m - Mat<T>::BIAS) + log2f(l)) * LN2;
+        }
+    }
+    return odd;
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_few_kernel(AttnArgs a) {
+    __shared__ __align__(16) char lds[4 * Few<T, DP>::WAVE];
+    __shared__ float part_m[4][16], part_l[4][16];
+    for (int want = blockIdx.x;; want += gridDim.x) {
+        Unit u;
+        if (!find_unit<true>(a, want, u)) break;
+        if (__syncthreads_or(few_unit<T, DP, false>(a, u, lds, part_m, part_l) != 0)) {
+            few_unit<T, DP, true>(a, u, lds, part_m, part_l);
+            __syncthreads();
+        }
+    }
+}
+
+// ---- many rows ------------------------------------------------------------------------------------------------------------------------------
+// 16 bytes a lane from memory to LDS at `to` + 16 * lane (of the whole wave; lanes that are off write nothing), without a register in between.  Nothing but
+// dma_landed() waits for it.
+__device__ __forceinline__ void dma16(const char* from, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(to) : "memory", "m0");
+}
+__device__ __forceinline__ void dma_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Tiles lie in LDS as they come, rows of DP elements without padding (the copy writes 1 KB runs), and which 16-byte piece of a row sits where is
+// exchanged instead: such that 16 rows read at one piece (keys), and 4 rows read at 64 bytes (values, transposed), meet every bank once.
+template <int DP> __device__ __forceinline__ int key_piece(int row, int piece) {
+    return piece ^ (DP % 128 == 0 ? row & 15 : (DP % 64 == 0 ? row >> 1 & 7 : row >> 2 & 3));
+}
+template <int DP> __device__ __forceinline__ int value_piece(int row, int piece) {
+    return piece ^ (DP % 128 == 0 ? (row & 3) << 2 : (DP % 64 == 0 ? (row >> 1 & 1) << 2 : 0));
+}
+
+template <int DP> constexpr int tile_keys() { return DP <= 128 ? 64 : 32; }
+template <int DP> constexpr int many_lds() { return 4 * tile_keys<DP>() * DP * 2; }
+
+template <typename T, int DP, bool ODD>
+__device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, char* lds) {
+    typedef typename Mat<T>::x8 x8;
+    constexpr int KT = tile_keys<DP>(), SUB = KT / 32, KS = DP / 16, DB = DP / 32, ROW = DP * 2, BUF = KT * ROW, NP = BUF / 4096;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
+    const int head_bytes = a.dim * 2;
+    const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;      // keys, keys, values, values
+    const int rows = u.n * a.group, row0 = u.tile * MANY_ROWS + wave * 32;
+    const int row = row0 + col, row_in = row < rows ? row : rows - 1;
+    const int token = row_in / a.group, head = u.head * a.group + (row_in - token * a.group);
+    const int pos = a.causal ? u.len - u.n + token : u.len - 1;
+    const bool any_row = row0 < rows;                          // of this wave
+    auto pos_of = [&](int r) { return a.causal ? u.len - u.n + min(r, rows - 1) / a.group : u.len - 1; };
+    const int low = pos_of(row0), high = pos_of(row0 + 31), tile_low = pos_of(u.tile * MANY_ROWS), tile_high = pos_of(u.tile * MANY_ROWS + MANY_ROWS - 1);
+    const int split_begin = u.cut.begin + u.split * u.cut.chunk, end = min(min(split_begin + u.cut.chunk, u.len), tile_high + 1);
+    int begin = split_begin;                                   // keys before the tile's first window are left out
+    if (a.window > 0 && tile_low - a.window + 1 > begin) begin = (tile_low - a.window + 1) & ~63;
+    x8 q[KS];
+    {
+        const char* p = a.q + (u.first + token) * a.q_token + head * a.q_head;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            uint4 w = uint4{0, 0, 0, 0};
+            if ((16 * ks + 8 * h) * 2 < head_bytes) w = *(const uint4*)(p + (16 * ks + 8 * h) * 2);
+            if (a.negate) { w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u; }
+            q[ks] = __builtin_bit_cast(x8, w);
+        }
+    }
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+    Run run;
+    uint32_t odd = 0;
+    const int* table = a.table + (long)u.b * a.width;
+    const long head_at = u.head * a.head_stride;
+    const int slots = (1 << a.page_shift) - 1;
+    auto pages_at = [&](int k0) { return table[min(k0 + (lane & (KT - 1)), end - 1) >> a.page_shift]; };
+    auto fetch = [&](int k0, int pg, int buf) {                // the wave's share of a tile: NP runs of 1 KB of keys and of values
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int at = (i * 4 + wave) * 1024, x = at + lane * 16, r = x / ROW, piece = (x - r * ROW) / 16;
+            const int page = __shfl(pg, r), p = (unsigned)page < (unsigned)a.pages ? page : 0;
+            const long from = p * a.page_stride + (min(k0 + r, end - 1) & slots) * a.slot_stride + head_at;
+            const int kp = key_piece<DP>(r, piece) * 16, vp = value_piece<DP>(r, piece) * 16;
+            if (kp < head_bytes) dma16(a.k + from + kp, lds_at + buf * BUF + at);
+            if (vp < head_bytes) dma16(a.v + from + vp, lds_at + (2 + buf) * BUF + at);
+        }
+    };
+    int pg = 0, pg_next = 0;
+    if (begin < end) {
+        pg = pages_at(begin);
+        pg_next = pages_at(begin + KT);
+        fetch(begin, pg, 0);
+    }
+    dma_landed();
+    __syncthreads();
+    int buf = 0;
+    for (int k0 = begin; k0 < end; k0 += KT, buf ^= 1) {
+        const unsigned long long bad = __ballot((unsigned)pg >= (unsigned)a.pages);
+        if (k0 + KT < end) {
+            fetch(k0 + KT, pg_next, buf ^ 1);
+            pg = pg_next;
+            pg_next = pages_at(k0 + 2 * KT);
+        }
+        if (any_row && k0 <= high && (a.window == 0 || k0 + KT - 1 > low - a.window)) {
+            const char *kb = lds + buf * BUF, *vb = lds + (2 + buf) * BUF;
+            const bool whole = k0 + KT <= end && k0 + KT - 1 <= low && (a.window == 0 || k0 > high - a.window) && (!ODD || bad == 0);
+            if (!ODD) odd |= bad != 0;
+            f32x16 s[SUB];
+            uint32_t seen[SUB] = {};
+#pragma unroll
+            for (int t = 0; t < SUB; ++t) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const int r = 32 * t + col;
+                    s[t] = Mat<T>::mul(*(const x8*)(kb + r * ROW + key_piece<DP>(r, 2 * ks + h) * 16), q[ks], s[t]);
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int in_tile = 32 * t + (r & 3) + 8 * (r >> 2) + 4 * h, key = k0 + in_tile;
+                        const bool sees = key < end && key <= pos && (a.window == 0 || key > pos - a.window);
+                        if (ODD && sees) seen[t] |= 1u << r;
+                        s[t][r] = !sees ? -INFINITY : (ODD && (bad >> in_tile & 1) ? __builtin_nanf("") : s[t][r]);
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
+            top = fmaxf(top, __shfl_xor(top, 32));
+            float back;
+            if (run.rises(top * a.c, back)) {
+#pragma unroll
+                for (int i = 0; i < DB; ++i) o[i] *= back;
+            }
+            const float base = run.base<T>();
+            // element block i (32 elements: 64 bytes), keys 16 m + 4 h + {0..3} and + 8 of sub-tile t
+            auto value = [&](int t, int m, int i) {
+                const int r = 32 * t + 16 * m + 4 * h + ((lane & 15) >> 2), in_block = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+                return join<T>(read_transposed(vb + r * ROW + value_piece<DP>(r, 4 * i) * 16 + in_block),
+                               read_transposed(vb + (r + 8) * ROW + value_piece<DP>(r + 8, 4 * i) * 16 + in_block));
+            };
+#pragma unroll
+            for (int t = 0; t < SUB; ++t) {
+                x8 p[2];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float e = exp2_of(fmaf(s[t][j], a.c, -base));
+                    run.l += e;
+                    p[j >> 3][j & 7] = (T)e;
+                }
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int i = 0; i < DB; ++i) {
+                        const x8 v = value(t, m, i);
+                        if (ODD && !whole) o[i] = multiply_seen<T>(v, p[m], seen[t] >> (8 * m), o[i]);
+                        else o[i] = Mat<T>::mul(v, p[m], o[i]);
+                    }
+            }
+            if (!ODD && !whole) {
+#pragma unroll
+                for (int x = 0; x < SUB * 2 * DB; ++x) odd |= not_finite<T>(value(x / (2 * DB), x / DB % 2, x % DB));
+            }
+        }
+        dma_landed();
+        __syncthreads();
+    }
+    run.l += __shfl_xor(run.l, 32);
+    if (row < rows) {
+        const long t = u.first + token, at_row = t * a.q_heads + head;
+        if (u.cut.splits > 1) {
+            const long slot = at_row * a.splits + u.split;
+            if (h == 0) a.part_ml[slot] = float2{run.m, run.l};
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const int d = 32 * i + 2 * r + 4 * h;
+                    if (d < a.dim) *(f32x4*)(a.part_o + slot * a.dim + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+                }
+        } else {
+            const bool none = pos < 0;
+            const float f = none ? 0.f : 1.f / run.l;
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const int d = 32 * i + 2 * r + 4 * h;
+                    if (d >= a.dim) continue;
+                    Quad<T> z;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) z.e[j] = (T)(none ? 0.f : o[i][r + j] * f);
+                    *(Quad<T>*)(a.out + t * a.out_token + head * a.out_head + d * 2) = z;
+                }
+            if (a.lse && h == 0) a.lse[at_row] = none ? -INFINITY : (run.base<T>() + log2f(run.l)) * LN2;
+        }
+    }
+    return odd;
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_many_kernel(AttnArgs a) {
+    extern __shared__ __align__(16) char lds[];
+    if (a.dim < DP) {                                              // what lies behind the head's end is never copied: zeros
+        for (int x = threadIdx.x * 16; x < many_lds<DP>(); x += 4096) *(uint4*)(lds + x) = uint4{0, 0, 0, 0};
+        __syncthreads();
+    }
+    for (int want = blockIdx.x;; want += gridDim.x) {
+        Unit u;
+        if (!find_unit<false>(a, want, u)) break;
+        if (__syncthreads_or(many_unit<T, DP, false>(a, u, lds) != 0)) many_unit<T, DP, true>(a, u, lds);
+    }
+}
+
+// ---- the parts of a row whose keys were split -------------------------------------------------------------------------------------------------
+// A wave a row: lane = split for the weights, lane = elements for the sums
+template <typename T>
+__global__ __launch_bounds__(256) void cache_attention_join_kernel(AttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long at_row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (at_row >= (long)a.tokens * a.q_heads) return;
+    const int t = (int)(at_row / a.q_heads), h = (int)(at_row - (long)t * a.q_heads);
+    const int b = seq_of_token(a.cu_new, a.rows, t);
+    if (b >= a.rows) return;
+    const int first = a.cu_new[b], n = a.cu_new[b + 1] - first, len = clamp_len(a.lens[b], a.width << a.page_shift);
+    if (first < 0 || n < 0 || n > a.tokens || first > a.tokens - n || t < first || t >= first + n) return;
+    const Cut cut = cut_of(n, len, a.group, a.kv_heads, a.window, a.few, a.splits);
+    if (cut.splits <= 1) return;
+    const int pos = a.causal ? len - n + (t - first) : len - 1;
+    // the splits that hold keys of this row (the others may not have been written for it)
+    float2 ml = float2{-INFINITY, 0.f};
+    if (lane < cut.splits) ml = a.part_ml[at_row * a.splits + lane];
+    float m = ml.x;
+#pragma unroll
+    for (int i = 32; i; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
+    const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_of(ml.x - m);
+    float l = w == 0.f ? 0.f : w * ml.y;
+#pragma unroll
+    for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
+    const bool none = pos < 0;
+    const float f = none ? 0.f : 1.f / l;
+    const int d = lane * 4;                                        // (dim is at most 256; every lane stays, its weight is asked for)
+    const float* parts = a.part_o + at_row * a.splits * a.dim + (d < a.dim ? d : 0);
+    f32x4 y = f32x4{0, 0, 0, 0};
+#pragma unroll 8
+    for (int s = 0; s < cut.splits; ++s) {
+        const float ws = __shfl(w, s);
+        const f32x4 x = *(const f32x4*)(parts + (long)s * a.dim);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] += ws != 0.f ? ws * x[i] : 0.f;     // (what a split without a key of the row left there is not a number)
+    }
+    if (d < a.dim) {
+        Quad<T> z;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z.e[i] = (T)(none ? 0.f : y[i] * f);
+        *(Quad<T>*)(a.out + t * a.out_token + h * a.out_head + d * 2) = z;
+    }
+    if (a.lse && lane == 0) a.lse[at_row] = none ? -INFINITY : ((m == -INFINITY ? 0.f : m - Mat<T>::BIAS) + log2f(l)) * LN2;
+}
+
+// ---- what the host decides ----------------------------------------------------------------------------------------------------------------------
+// sequences of at most so many rows take the few-rows form
+constexpr int FEW_LIMIT = 32;
+
+struct Plan {
+    bool few, many;      // which forms are launched
+    int few_limit;       // rows (INT_MAX: all)
+    int splits;          // a row's parts, at most
+    long few_units, many_units;
+};
+
+Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
+    Plan p;
+    const long capacity = (long)c.table_width * c.page_size;
+    const int group = d.q_heads / c.kv_heads;
+    const int len = (int)(d.max_len > 0 && d.max_len < capacity ? d.max_len : capacity);
+    const int most_new = d.max_new > 0 && d.max_new < d.tokens ? d.max_new : d.tokens;
+    const bool alone = c.rows == 1;                                // then its new tokens are all of them
+    p.many = (long)(alone ? d.tokens : most_new) * group > FEW_LIMIT;
+    p.few = !(alone && p.many);
+    p.few_limit = p.many ? FEW_LIMIT : 0x7fffffff;
+    p.splits = 1;
+    p.few_units = p.many_units = 0;
+    // (of the longest sequence: a part more or less because of the others in a call would show in the last bit)
+    const long span = (long)d.window + 63 + (p.many ? FEW_LIMIT : most_new);
+    if (p.few) p.splits = splits_of(true, 1, d.window > 0 && span < len ? (int)span : len, c.kv_heads);
+    if (p.many) {
+        const int tiles = (int)(((long)d.tokens * group + MANY_ROWS - 1) / MANY_ROWS);
+        const int s = splits_of(false, alone ? tiles : 1, len, alone ? c.kv_heads : 1);
+        if (s > p.splits) p.splits = s;
+    }
+    const long tiles = c.rows < d.tokens ? c.rows : d.tokens;
+    if (p.few) p.few_units = (tiles + (long)d.tokens * group / FEW_ROWS) * p.splits * c.kv_heads;
+    if (p.many) p.many_units = (tiles + (long)d.tokens * group / MANY_ROWS) * (p.splits < 8 ? p.splits : 8) * c.kv_heads;
+    return p;
+}
+
+unsigned grid_for(long units, long most) { return (unsigned)(units < 1 ? 1 : (units < most ? units : most)); }
+
+template <typename T, int DP>
+int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
+    if (p.many) {
+        constexpr int LDS = many_lds<DP>();
+        static_assert(LDS <= 65536, "more LDS has to be asked for");
+        cache_attention_many_kernel<T, DP><<<grid_for(p.many_units, 512), 256, LDS, s>>>(a);
+        DISCO_LAUNCH_CHECK("cache_attention_many_kernel");
+    }
+    if (p.few) {
+        cache_attention_few_kernel<T, DP><<<grid_for(p.few_units, 1024), 256, 0, s>>>(a);
+        DISCO_LAUNCH_CHECK("cache_attention_few_kernel");
+    }
+    if (p.splits > 1) {
+        cache_attention_join_kernel<T><<<(unsigned)(((long)a.tokens * a.q_heads + 3) / 4), 256, 0, s>>>(a);
+        DISCO_LAUNCH_CHECK("cache_attention_join_kernel");
+    }
+    return DISCO_OK;
+}
+
+template <typename T>
+int run_dims(const AttnArgs& a, const Plan& p, hipStream_t s) {
+    if (a.dim <= 32) return run_forms<T, 32>(a, p, s);
+    if (a.dim <= 64) return run_forms<T, 64>(a, p, s);
+    if (a.dim <= 96) return run_forms<T, 96>(a, p, s);
+    if (a.dim <= 128) return run_forms<T, 128>(a, p, s);
+    if (a.dim <= 192) return run_forms<T, 192>(a, p, s);
+    return run_forms<T, 256>(a, p, s);
 }
 
 }  // namespace
 
-size_t cache_attention_ws_bytes(const disco_cache_desc&, const disco_attention_desc&) { return 0; }
+size_t cache_attention_ws_bytes(const disco_cache_desc& c, const disco_attention_desc& d) {
+    const Plan p = plan_of(c, d);
+    if (p.splits == 1) return 0;
+    const size_t parts = (size_t)d.tokens * d.q_heads * p.splits;
+    return parts * ((size_t)c.dim * 4 + 8);
+}
 
 int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc& d, const void* q, const int* table, const int* lens,
-                           const int* cu_new, void* out, float* lse, void*, hipStream_t s) {
-    AttnArgs a{(const char*)q, (const char*)c.d_k, (const char*)c.d_v, (char*)out, lse, table, lens, cu_new, d.q_token * 2, d.q_head * 2, d.out_token * 2,
-               d.out_head * 2, c.page_stride * 2, c.head_stride * 2, c.slot_stride * 2, d.tokens, d.q_heads, c.kv_heads, d.q_heads / c.kv_heads, c.dim,
-               c.rows, c.table_width, c.pages, __builtin_ctz((unsigned)c.page_size), d.causal, d.window, d.scale};
-    const dim3 grid(d.tokens, d.q_heads);
-    if (c.dtype == DISCO_F16) cache_attention_kernel<f16><<<grid, 64, 0, s>>>(a);
-    else cache_attention_kernel<__bf16><<<grid, 64, 0, s>>>(a);
-    DISCO_LAUNCH_CHECK("cache_attention_kernel");
-    return DISCO_OK;
+                           const int* cu_new, void* out, float* lse, void* ws, hipStream_t s) {
+    const Plan p = plan_of(c, d);
+    const size_t parts = (size_t)d.tokens * d.q_heads * p.splits;
+    AttnArgs a{(const char*)q, (const char*)c.d_k, (const char*)c.d_v, (char*)out, lse, (float*)ws, (float2*)((char*)ws + (p.splits > 1 ? parts * c.dim * 4 : 0)),
+               table, lens, cu_new, d.q_token * 2, d.q_head * 2, d.out_token * 2, d.out_head * 2, c.page_stride * 2, c.head_stride * 2, c.slot_stride * 2,
+               d.tokens, d.q_heads, c.kv_heads, d.q_heads / c.kv_heads, c.dim, c.rows, c.table_width, c.pages, __builtin_ctz((unsigned)c.page_size), d.causal,
+               d.window, p.splits, p.few_limit, fabsf(d.scale) * 1.4426950408889634f, d.scale < 0};
+    if (a.c < 1e-37f) a.c = 1e-37f;                                // 0 * -inf is not the score of a key that is not seen
+    return c.dtype == DISCO_F16 ? run_dims<f16>(a, p, s) : run_dims<bf16>(a, p, s);
 }
 
 }  // namespace disco

@@ -286,6 +286,17 @@ def test_a_sequence_does_not_depend_on_its_batch(new):
         assert torch.equal(alone, together[a:e])
 
 
+def test_a_sequence_does_not_depend_on_a_longer_one():
+    """Lengths around the most parts that a row's keys are cut into: the longer sequence of a call must not change how the shorter one is cut."""
+    s = Served([16384, 16700, 16000], [1, 1, 40], 1, 1, 64, 64, BF, seed=4)
+    together = paged.cache_attention(s.q, *s.args())
+    for b in range(3):
+        a, e = int(s.cu[b]), int(s.cu[b + 1])
+        for kw in (dict(), dict(max_len=int(s.lens[b])), dict(max_len=int(s.lens[b]), max_new=e - a)):
+            alone = paged.cache_attention(s.q[a:e], s.k, s.v, s.table[b:b + 1].contiguous(), s.lens[b:b + 1].contiguous(), ints([0, e - a]), **kw)
+            assert torch.equal(alone, together[a:e])
+
+
 def test_rows_behind_the_last_sequence_stay():
     s = Served([50, 20], [4, 1], 2, 2, 64, 16, BF)
     q = torch.cat((s.q, torch.full((7, 4, 64), math.nan, dtype=BF, device=DEV)))
