@@ -24,6 +24,7 @@ EXTRA_FLAGS = {"pool.hip": ["-fno-slp-vectorize"], "spixel.hip": ["-fno-slp-vect
                "attention_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 # the paged-cache kernels use no packed fp32 instruction of any form (hipcc's host pass says that it does not know the feature: harmless)
 EXTRA_FLAGS.update({f: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for f in ("rotary.hip", "cache_pages.hip", "cache_attention.hip")})
+EXTRA_FLAGS["cache_attention.hip"] += ["-mllvm", "-amdgpu-mfma-vgpr-form"]
 HEADERS = ["common.h", "paged.h", "ctx.h", "plan.h", "conv_mx_kernel.h", os.path.join("..", "..", "include", "disco_hip.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-x", "hip", "-Wno-unused-result"]

@@ -202,20 +202,21 @@ __device__ __forceinline__ Acc multiply_seen(typename Mat<T>::x8 v, typename Mat
     return o;
 }
 
-// What a wave keeps of its rows while it walks along the keys (a lane: of its own row): the maximum in use, in log2 units, and the sum of the keys that
-// this lane saw.
+// What a wave keeps of its rows while it walks along the keys (a lane: of its own row): the maximum in use, in log2 units, and the sum over the keys that
+// this lane saw.  The maximum of a tile is not looked for as long as the sum of its probabilities says that the one in use will do: up to
+// LIMIT, which fp16 holds (and leaves the fp32 sums of bf16 values up to 2^100 finite).
 struct Run {
     float m = -INFINITY, l = 0.f;
-    // A tile's largest score `top` (log2 units, the same in all lanes of the row).  The accumulators are rescaled only where the maximum in use is
-    // more than 2^8 too small, which after a few tiles hardly happens; returns whether some lane asks for it, and the factor.
-    __device__ __forceinline__ bool rises(float top, float& back) {
-        const bool up = top > m + 8.f;
-        if (!__any(up)) return false;
-        const float now = fmaxf(m, top);
-        back = now == -INFINITY ? 1.f : exp2_of(m - now);
+    static constexpr float LIMIT = 32768.f;
+    __device__ __forceinline__ bool asks(float sum) const { return !(sum <= LIMIT) || m == -INFINITY; }
+    // where the row asks for it, takes a new maximum over `top` (log2 units; both the same in all lanes of the row), and returns the factor of what
+    // has been summed.  A row goes by its own scores alone.
+    __device__ __forceinline__ float raise(bool asked, float top) {
+        if (!asked) return 1.f;
+        const float now = fmaxf(m, top), back = now == -INFINITY ? 1.f : exp2_of(m - now);
         m = now;
         l *= back;
-        return true;
+        return back;
     }
     template <typename T> __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m - Mat<T>::BIAS; }
 };
@@ -301,10 +302,10 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
         fetch_k(k0, pg);
         fetch_v(k0, pg);
     }
-    for (; k0 < end; k0 += 128) {
-        const uint32_t bad = (uint32_t)__ballot((unsigned)pg >= (unsigned)a.pages);
-        const bool whole = k0 + 32 <= end && k0 + 31 <= low && (a.window == 0 || k0 > high - a.window) && (!ODD || bad == 0);
-        if (!ODD) odd |= bad;
+    const char* vt = mine + (4 * g + (col >> 2)) * VROW + (col & 3) * 8;
+    auto value = [&](int i) { return join<T>(read_transposed(vt + i * 32), read_transposed(vt + 16 * VROW + i * 32)); };
+    auto tile = [&](auto masked, uint32_t bad) {
+        constexpr bool MASKED = decltype(masked)::value;
         f32x4 s[2];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -314,9 +315,8 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
         }
         const bool more = k0 + 128 < end;
         if (more) fetch_k(k0 + 128, pg_next);
-        uint32_t seen = 0xff;                                  // of this lane's eight keys
-        if (!whole) {
-            seen = 0;
+        uint32_t seen = 0;                                         // of this lane's eight keys
+        if (MASKED) {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -327,24 +327,34 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
                     s[t][r] = !sees ? -INFINITY : (ODD && (bad >> in_tile & 1) ? __builtin_nanf("") : s[t][r]);
                 }
         }
-        float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        float back;
-        if (run.rises(top * a.c, back)) {
+        x8 p;
+        float sum;
+        auto weights = [&] {
+            const float base = run.base<T>();
+            sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float e = exp2_of(fmaf(s[i / 4][i % 4], a.c, -base));
+                sum += e;
+                p[i] = (T)e;
+            }
+        };
+        weights();
+        const bool asks = run.asks(sum);
+        if (__any(asks)) {
+            asm volatile("");                                      // (a branch: not to be computed ahead)
+            int asked = asks;
+            asked |= __shfl_xor(asked, 16);
+            asked |= __shfl_xor(asked, 32);
+            float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float back = run.raise(asked != 0, top * a.c);
 #pragma unroll
             for (int i = 0; i < DB; ++i) o[i] *= back;
+            weights();
         }
-        const float base = run.base<T>();
-        x8 p;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float e = exp2_of(fmaf(s[t][r], a.c, -base));
-                run.l += e;
-                p[4 * t + r] = (T)e;
-            }
+        run.l += sum;
         // the tile's values into LDS; a wave's LDS operations take place in order
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -357,20 +367,28 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
             pg_next = pages_at(k0 + 256);
         }
         __builtin_amdgcn_wave_barrier();
-        const char* vt = mine + (4 * g + (col >> 2)) * VROW + (col & 3) * 8;
-        auto value = [&](int i) { return join<T>(read_transposed(vt + i * 32), read_transposed(vt + 16 * VROW + i * 32)); };
-        if (!ODD || whole) {
 #pragma unroll
-            for (int i = 0; i < DB; ++i) {
-                const x8 v = value(i);
-                if (!ODD && !whole) odd |= not_finite<T>(v);
+        for (int i = 0; i < DB; ++i) {
+            const x8 v = value(i);
+            if (ODD && MASKED) o[i] = multiply_seen<T>(v, p, seen, o[i]);
+            else {
+                if (MASKED) odd |= not_finite<T>(v);
                 o[i] = Mat<T>::mul(v, p, o[i]);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < DB; ++i) o[i] = multiply_seen<T>(value(i), p, seen, o[i]);
         }
         __builtin_amdgcn_wave_barrier();
+    };
+    auto walk = [&](auto masked, int stop) {                       // tiles that begin before `stop`
+        for (; k0 < stop; k0 += 128) {
+            const uint32_t bad = (uint32_t)__ballot((unsigned)pg >= (unsigned)a.pages);
+            if (!ODD) odd |= bad;
+            tile(masked, bad);
+        }
+    };
+    // tiles that some row sees in part lie before and behind those that all rows see whole
+    for (int part = 0; part < 2; ++part) {
+        walk(std::true_type(), part || ODD ? end : (a.window > 0 ? min(end, high - a.window + 1) : begin));
+        if (!ODD && part == 0) walk(std::false_type(), min(end, low + 1) - 31);
     }
     run.l += __shfl_xor(run.l, 16);
     run.l += __shfl_xor(run.l, 32);
@@ -413,6 +431,28 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
     return odd;
 }
 
+// The rare form as a function of its own, apart from the kernel's registers.  The kernel hands over where its arguments lie (only a kernel can ask for
+// that: in a function the builtin is null), and they are read into scalars again.
+__device__ __forceinline__ uint64_t kernel_args_at() { return (uint64_t)__builtin_amdgcn_kernarg_segment_ptr(); }
+__device__ __forceinline__ AttnArgs kernel_args(uint64_t at) {
+    constexpr int WORDS = sizeof(AttnArgs) / 4;
+    const uint32_t* p = (const uint32_t*)at;
+    struct Words { uint32_t w[WORDS]; } words;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) words.w[i] = __builtin_amdgcn_readfirstlane(p[i]);
+    return __builtin_bit_cast(AttnArgs, words);
+}
+__device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
+__device__ __forceinline__ char* lds_pointer(uint32_t offset) { return (char*)(__attribute__((address_space(3))) char*)(uintptr_t)offset; }
+
+template <typename T, int DP>
+__device__ __noinline__ void few_unit_odd(uint64_t args, int want, uint32_t lds, uint32_t m, uint32_t l) {
+    const AttnArgs a = kernel_args(args);
+    Unit u;
+    if (!find_unit<true>(a, __builtin_amdgcn_readfirstlane(want), u)) return;
+    few_unit<T, DP, true>(a, u, lds_pointer(lds), *(float (*)[4][16])lds_pointer(m), *(float (*)[4][16])lds_pointer(l));
+}
+
 template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_few_kernel(AttnArgs a) {
     __shared__ __align__(16) char lds[4 * Few<T, DP>::WAVE];
@@ -421,7 +461,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_few_ke
         Unit u;
         if (!find_unit<true>(a, want, u)) break;
         if (__syncthreads_or(few_unit<T, DP, false>(a, u, lds, part_m, part_l) != 0)) {
-            few_unit<T, DP, true>(a, u, lds, part_m, part_l);
+            few_unit_odd<T, DP>(kernel_args_at(), want, lds_offset(lds), lds_offset(part_m), lds_offset(part_l));
             __syncthreads();
         }
     }
@@ -431,7 +471,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_few_ke
 // 16 bytes a lane from memory to LDS at `to` + 16 * lane (of the whole wave; lanes that are off write nothing), without a register in between.  Nothing but
 // dma_landed() waits for it.
 __device__ __forceinline__ void dma16(const char* from, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(to) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(from), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory", "m0");
 }
 __device__ __forceinline__ void dma_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -497,28 +537,12 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
             if (vp < head_bytes) dma16(a.v + from + vp, lds_at + (2 + buf) * BUF + at);
         }
     };
-    int pg = 0, pg_next = 0;
-    if (begin < end) {
-        pg = pages_at(begin);
-        pg_next = pages_at(begin + KT);
-        fetch(begin, pg, 0);
-    }
-    dma_landed();
-    __syncthreads();
-    int buf = 0;
-    for (int k0 = begin; k0 < end; k0 += KT, buf ^= 1) {
-        const unsigned long long bad = __ballot((unsigned)pg >= (unsigned)a.pages);
-        if (k0 + KT < end) {
-            fetch(k0 + KT, pg_next, buf ^ 1);
-            pg = pg_next;
-            pg_next = pages_at(k0 + 2 * KT);
-        }
-        if (any_row && k0 <= high && (a.window == 0 || k0 + KT - 1 > low - a.window)) {
-            const char *kb = lds + buf * BUF, *vb = lds + (2 + buf) * BUF;
-            const bool whole = k0 + KT <= end && k0 + KT - 1 <= low && (a.window == 0 || k0 > high - a.window) && (!ODD || bad == 0);
-            if (!ODD) odd |= bad != 0;
-            f32x16 s[SUB];
-            uint32_t seen[SUB] = {};
+    auto tile = [&](auto masked, int k0, const char* kb, const char* vb, unsigned long long bad) {
+        constexpr bool MASKED = decltype(masked)::value;
+        f32x16 s[SUB];
+        x8 p[SUB][2];
+        uint32_t seen[SUB] = {};
+        auto scores = [&] {
 #pragma unroll
             for (int t = 0; t < SUB; ++t) {
 #pragma unroll
@@ -528,10 +552,8 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
                     const int r = 32 * t + col;
                     s[t] = Mat<T>::mul(*(const x8*)(kb + r * ROW + key_piece<DP>(r, 2 * ks + h) * 16), q[ks], s[t]);
                 }
-            }
-            if (!whole) {
-#pragma unroll
-                for (int t = 0; t < SUB; ++t)
+                if (MASKED) {
+                    seen[t] = 0;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
                         const int in_tile = 32 * t + (r & 3) + 8 * (r >> 2) + 4 * h, key = k0 + in_tile;
@@ -539,50 +561,90 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
                         if (ODD && sees) seen[t] |= 1u << r;
                         s[t][r] = !sees ? -INFINITY : (ODD && (bad >> in_tile & 1) ? __builtin_nanf("") : s[t][r]);
                     }
+                }
             }
+        };
+        auto weights = [&] {
+            const float base = run.base<T>();
+            float sum = 0.f;
+#pragma unroll
+            for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float e = exp2_of(fmaf(s[t][j], a.c, -base));
+                    sum += e;
+                    p[t][j >> 3][j & 7] = (T)e;
+                }
+            return sum;
+        };
+        scores();
+        float sum = weights();
+        const bool asks = run.asks(sum);
+        if (__any(asks)) {
+            asm volatile("" ::: "memory");                         // (a branch, and the scores once more rather than kept)
+            scores();
             float top = -INFINITY;
 #pragma unroll
             for (int t = 0; t < SUB; ++t)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
             top = fmaxf(top, __shfl_xor(top, 32));
-            float back;
-            if (run.rises(top * a.c, back)) {
+            const float back = run.raise(asks | __shfl_xor((int)asks, 32), top * a.c);
 #pragma unroll
-                for (int i = 0; i < DB; ++i) o[i] *= back;
-            }
-            const float base = run.base<T>();
-            // element block i (32 elements: 64 bytes), keys 16 m + 4 h + {0..3} and + 8 of sub-tile t
-            auto value = [&](int t, int m, int i) {
-                const int r = 32 * t + 16 * m + 4 * h + ((lane & 15) >> 2), in_block = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
-                return join<T>(read_transposed(vb + r * ROW + value_piece<DP>(r, 4 * i) * 16 + in_block),
-                               read_transposed(vb + (r + 8) * ROW + value_piece<DP>(r + 8, 4 * i) * 16 + in_block));
-            };
+            for (int i = 0; i < DB; ++i) o[i] *= back;
+            sum = weights();
+        }
+        run.l += sum;
+        // element block i (32 elements: 64 bytes), keys 16 m + 4 h + {0..3} and + 8 of sub-tile t
+        auto value = [&](int t, int m, int i) {
+            const int r = 32 * t + 16 * m + 4 * h + ((lane & 15) >> 2), in_block = ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+            return join<T>(read_transposed(vb + r * ROW + value_piece<DP>(r, 4 * i) * 16 + in_block),
+                           read_transposed(vb + (r + 8) * ROW + value_piece<DP>(r + 8, 4 * i) * 16 + in_block));
+        };
 #pragma unroll
-            for (int t = 0; t < SUB; ++t) {
-                x8 p[2];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float e = exp2_of(fmaf(s[t][j], a.c, -base));
-                    run.l += e;
-                    p[j >> 3][j & 7] = (T)e;
-                }
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < DB; ++i) {
-                        const x8 v = value(t, m, i);
-                        if (ODD && !whole) o[i] = multiply_seen<T>(v, p[m], seen[t] >> (8 * m), o[i]);
-                        else o[i] = Mat<T>::mul(v, p[m], o[i]);
-                    }
-            }
-            if (!ODD && !whole) {
-#pragma unroll
-                for (int x = 0; x < SUB * 2 * DB; ++x) odd |= not_finite<T>(value(x / (2 * DB), x / DB % 2, x % DB));
+        for (int x = 0; x < SUB * 2 * DB; ++x) {
+            const int t = x / (2 * DB), m = x / DB % 2, i = x % DB;
+            const x8 v = value(t, m, i);
+            if (ODD && MASKED) o[i] = multiply_seen<T>(v, p[t][m], seen[t] >> (8 * m), o[i]);
+            else {
+                if (MASKED) odd |= not_finite<T>(v);
+                o[i] = Mat<T>::mul(v, p[t][m], o[i]);
             }
         }
-        dma_landed();
-        __syncthreads();
+    };
+    int pg = 0, pg_next = 0;
+    if (begin < end) {
+        pg = pages_at(begin);
+        pg_next = pages_at(begin + KT);
+        fetch(begin, pg, 0);
+    }
+    dma_landed();
+    __syncthreads();
+    int buf = 0, k0 = begin;
+    auto walk = [&](auto masked, int stop) {
+        for (; k0 < stop; k0 += KT, buf ^= 1) {
+            const unsigned long long bad = __ballot((unsigned)pg >= (unsigned)a.pages);
+            if (!ODD) odd |= bad != 0;
+            if (k0 + KT < end) {
+                fetch(k0 + KT, pg_next, buf ^ 1);
+                pg = pg_next;
+                pg_next = pages_at(k0 + 2 * KT);
+            }
+            if (any_row && (!decltype(masked)::value || (k0 <= high && (a.window == 0 || k0 + KT - 1 > low - a.window))))
+                tile(masked, k0, lds + buf * BUF, lds + (2 + buf) * BUF, bad);
+            dma_landed();
+            __syncthreads();
+        }
+    };
+    // tiles that some row of the workgroup sees in part lie before and behind those that all rows see whole
+    int whole_from = begin, whole_to = begin;
+    if (!ODD) {
+        if (a.window > 0) whole_from = min(end, begin + max(0, (tile_high - a.window - begin + KT) / KT * KT));
+        whole_to = begin + max(0, min(end, tile_low + 1) - begin) / KT * KT;
+    }
+    for (int part = 0; part < 2; ++part) {
+        walk(std::true_type(), part ? end : whole_from);
+        if (!ODD && part == 0) walk(std::false_type(), whole_to);
     }
     run.l += __shfl_xor(run.l, 32);
     if (row < rows) {
@@ -618,6 +680,14 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
 }
 
 template <typename T, int DP>
+__device__ __noinline__ void many_unit_odd(uint64_t args, int want, uint32_t lds) {
+    const AttnArgs a = kernel_args(args);
+    Unit u;
+    if (!find_unit<false>(a, __builtin_amdgcn_readfirstlane(want), u)) return;
+    many_unit<T, DP, true>(a, u, lds_pointer(lds));
+}
+
+template <typename T, int DP>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_many_kernel(AttnArgs a) {
     extern __shared__ __align__(16) char lds[];
     if (a.dim < DP) {                                              // what lies behind the head's end is never copied: zeros
@@ -627,7 +697,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_many_k
     for (int want = blockIdx.x;; want += gridDim.x) {
         Unit u;
         if (!find_unit<false>(a, want, u)) break;
-        if (__syncthreads_or(many_unit<T, DP, false>(a, u, lds) != 0)) many_unit<T, DP, true>(a, u, lds);
+        if (__syncthreads_or(many_unit<T, DP, false>(a, u, lds) != 0)) many_unit_odd<T, DP>(kernel_args_at(), want, lds_offset(lds));
     }
 }
 
