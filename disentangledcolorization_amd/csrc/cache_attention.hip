@@ -56,6 +56,14 @@ struct AttnArgs {
     int negate;                                                    // scale < 0: the queries change sign instead
 };
 
+// The kernels read their arguments where they lie, piece by piece: held in registers from start to end they would not fit beside the loops.  fresh()
+// makes the compiler forget what it has read.
+typedef const __attribute__((address_space(4))) AttnArgs* ArgsAt;
+__device__ __forceinline__ ArgsAt fresh(ArgsAt p) {
+    asm volatile("" : "+s"(p));
+    return p;
+}
+
 constexpr int FEW_ROWS = 16, MANY_ROWS = 128;
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -97,21 +105,21 @@ struct Unit { int b, n, len, first, tile, split, head; Cut cut; };
 // unit number `want` of the form FEW over all sequences (key head fastest, then split, then tile - the last, longest tiles first); false behind the last.
 // Every lane of the wave calls it and gets the same.
 template <bool FEW>
-__device__ __forceinline__ bool find_unit(const AttnArgs& a, int want, Unit& u) {
-    const int lane = threadIdx.x & 63, capacity = a.width << a.page_shift;
+__device__ __forceinline__ bool find_unit(ArgsAt a, int want, Unit& u) {
+    const int lane = threadIdx.x & 63, capacity = a->width << a->page_shift;
     int left = want;
-    for (int b0 = 0; b0 < a.rows; b0 += 64) {
+    for (int b0 = 0; b0 < a->rows; b0 += 64) {
         const int b = b0 + lane;
         int n = 0, len = 0, first = 0, units = 0;
         Cut cut{};
-        if (b < a.rows) {
-            first = a.cu_new[b];
-            n = a.cu_new[b + 1] - first;
-            len = clamp_len(a.lens[b], capacity);
-            if (first < 0 || n < 0 || n > a.tokens || first > a.tokens - n) n = 0;       // (not offsets)
-            if (n > 0 && (n * (long)a.group <= a.few) == FEW) {
-                cut = cut_of(n, len, a.group, a.kv_heads, a.window, a.few, a.splits);
-                units = cut.tiles * cut.splits * a.kv_heads;
+        if (b < a->rows) {
+            first = a->cu_new[b];
+            n = a->cu_new[b + 1] - first;
+            len = clamp_len(a->lens[b], capacity);
+            if (first < 0 || n < 0 || n > a->tokens || first > a->tokens - n) n = 0;       // (not offsets)
+            if (n > 0 && (n * (long)a->group <= a->few) == FEW) {
+                cut = cut_of(n, len, a->group, a->kv_heads, a->window, a->few, a->splits);
+                units = cut.tiles * cut.splits * a->kv_heads;
             }
         }
         int upto = units;
@@ -132,7 +140,7 @@ __device__ __forceinline__ bool find_unit(const AttnArgs& a, int want, Unit& u) 
             u.cut.begin = __builtin_amdgcn_readlane(cut.begin, at);
             u.cut.chunk = __builtin_amdgcn_readlane(cut.chunk, at);
             int x = left - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(units, at));
-            u.head = x % a.kv_heads; x /= a.kv_heads;
+            u.head = x % a->kv_heads; x /= a->kv_heads;
             u.split = x % u.cut.splits;
             u.tile = u.cut.tiles - 1 - x / u.cut.splits;
             return true;
@@ -236,28 +244,31 @@ template <typename T, int DP> struct Few {
 // One unit.  ODD: the form that keeps values which are not finite, and pages outside the cache, from the rows that do not see them; without it returns whether
 // there were any (then the unit is done again with it).  Both add the same products in the same order.
 template <typename T, int DP, bool ODD>
-__device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, char* lds, float (&part_m)[4][16], float (&part_l)[4][16]) {
+__device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds, float (&part_m)[4][16], float (&part_l)[4][16]) {
     typedef typename Mat<T>::x8 x8;
     constexpr int KS = DP / 32, DB = DP / 16, NV = DP / 16, VROW = Few<T, DP>::VROW, OROW = Few<T, DP>::OROW, WAVE = Few<T, DP>::WAVE;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, col = lane & 15;
     char* mine = lds + wave * WAVE;
-    const int head_bytes = a.dim * 2;
-    const int rows = u.n * a.group;
+    const int head_bytes = a->dim * 2;
+    const int rows = u.n * a->group;
     // this lane's row: its token, its head, its position
     const int row = u.tile * FEW_ROWS + col, row_in = row < rows ? row : rows - 1;
-    const int token = row_in / a.group, head = u.head * a.group + (row_in - token * a.group);
-    const int pos = a.causal ? u.len - u.n + token : u.len - 1;
-    const int last_token = (min(u.tile * FEW_ROWS + FEW_ROWS, rows) - 1) / a.group, first_token = u.tile * FEW_ROWS / a.group;
-    const int high = a.causal ? u.len - u.n + last_token : u.len - 1, low = a.causal ? u.len - u.n + first_token : u.len - 1;
+    const int token = row_in / a->group, head = u.head * a->group + (row_in - token * a->group);
+    const int pos = a->causal ? u.len - u.n + token : u.len - 1;
+    const int last_token = (min(u.tile * FEW_ROWS + FEW_ROWS, rows) - 1) / a->group, first_token = u.tile * FEW_ROWS / a->group;
+    const int high = a->causal ? u.len - u.n + last_token : u.len - 1, low = a->causal ? u.len - u.n + first_token : u.len - 1;
     const int begin = u.cut.begin + u.split * u.cut.chunk, end = min(min(begin + u.cut.chunk, u.len), high + 1);
+    // the keys that this lane's row sees here
+    const int first_seen = a->window > 0 ? pos - a->window + 1 : 0;
+    const uint32_t count_seen = max(0, min(pos + 1, end) - first_seen);
     x8 q[KS];
     {
-        const char* p = a.q + (u.first + token) * a.q_token + head * a.q_head;
+        const char* p = a->q + (u.first + token) * a->q_token + head * a->q_head;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             uint4 w = uint4{0, 0, 0, 0};
             if ((32 * ks + 8 * g) * 2 < head_bytes) w = *(const uint4*)(p + (32 * ks + 8 * g) * 2);
-            if (a.negate) { w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u; }
+            if (a->negate) { w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u; }
             q[ks] = __builtin_bit_cast(x8, w);
         }
     }
@@ -266,20 +277,20 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
     for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
     Run run;
     uint32_t odd = 0;
-    const int* table = a.table + (long)u.b * a.width;
-    const long head_at = u.head * a.head_stride;
-    const int slots = (1 << a.page_shift) - 1;
+    const int* table = a->table + (long)u.b * a->width;
+    const long head_at = u.head * a->head_stride;
+    const int slots = (1 << a->page_shift) - 1;
     // pages of the 32 keys of a tile, one a lane (twice)
-    auto pages_at = [&](int k0) { return table[min(k0 + (lane & 31), end - 1) >> a.page_shift]; };
+    auto pages_at = [&](int k0) { return table[min(k0 + (lane & 31), end - 1) >> a->page_shift]; };
     auto at = [&](int page, int key) {
-        const int p = (unsigned)page < (unsigned)a.pages ? page : 0;
-        return p * a.page_stride + (min(key, end - 1) & slots) * a.slot_stride + head_at;
+        const int p = (unsigned)page < (unsigned)a->pages ? page : 0;
+        return p * a->page_stride + (min(key, end - 1) & slots) * a->slot_stride + head_at;
     };
     uint4 kf[2][KS], vf[NV];
     auto fetch_k = [&](int k0, int pg) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const char* p = a.k + at(__shfl(pg, 16 * t + col), k0 + 16 * t + col);
+            const char* p = a->k + at(__shfl(pg, 16 * t + col), k0 + 16 * t + col);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const int byte = (32 * ks + 8 * g) * 2;
@@ -292,7 +303,7 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
         for (int i = 0; i < NV; ++i) {
             const int piece = i * 64 + lane, r = piece / (DP / 8), byte = (piece - r * (DP / 8)) * 16;
             const long p = at(__shfl(pg, r), k0 + r);
-            vf[i] = byte < head_bytes ? *(const uint4*)(a.v + p + byte) : uint4{0, 0, 0, 0};
+            vf[i] = byte < head_bytes ? *(const uint4*)(a->v + p + byte) : uint4{0, 0, 0, 0};
         }
     };
     int k0 = begin + 32 * wave, pg = 0, pg_next = 0;
@@ -321,8 +332,8 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int in_tile = 16 * t + 4 * g + r, key = k0 + in_tile;
-                    const bool sees = key < end && key <= pos && (a.window == 0 || key > pos - a.window);
+                    const int in_tile = 16 * t + 4 * g + r;
+                    const bool sees = (uint32_t)(k0 + in_tile - first_seen) < count_seen;
                     if (ODD && sees) seen |= 1u << (4 * t + r);
                     s[t][r] = !sees ? -INFINITY : (ODD && (bad >> in_tile & 1) ? __builtin_nanf("") : s[t][r]);
                 }
@@ -334,7 +345,7 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
             sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float e = exp2_of(fmaf(s[i / 4][i % 4], a.c, -base));
+                const float e = exp2_of(fmaf(s[i / 4][i % 4], a->c, -base));
                 sum += e;
                 p[i] = (T)e;
             }
@@ -349,7 +360,7 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
             float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float back = run.raise(asked != 0, top * a.c);
+            const float back = run.raise(asked != 0, top * a->c);
 #pragma unroll
             for (int i = 0; i < DB; ++i) o[i] *= back;
             weights();
@@ -380,18 +391,19 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
     };
     auto walk = [&](auto masked, int stop) {                       // tiles that begin before `stop`
         for (; k0 < stop; k0 += 128) {
-            const uint32_t bad = (uint32_t)__ballot((unsigned)pg >= (unsigned)a.pages);
+            const uint32_t bad = (uint32_t)__ballot((unsigned)pg >= (unsigned)a->pages);
             if (!ODD) odd |= bad;
             tile(masked, bad);
         }
     };
     // tiles that some row sees in part lie before and behind those that all rows see whole
     for (int part = 0; part < 2; ++part) {
-        walk(std::true_type(), part || ODD ? end : (a.window > 0 ? min(end, high - a.window + 1) : begin));
+        walk(std::true_type(), part || ODD ? end : (a->window > 0 ? min(end, high - a->window + 1) : begin));
         if (!ODD && part == 0) walk(std::false_type(), min(end, low + 1) - 31);
     }
     run.l += __shfl_xor(run.l, 16);
     run.l += __shfl_xor(run.l, 32);
+    a = fresh(a);
     // the four waves' rows: o to LDS (over the values), then every thread joins four elements of a row at a time
     float* om = (float*)mine;
 #pragma unroll
@@ -400,7 +412,7 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
     __syncthreads();
     for (int x = threadIdx.x; x < 16 * (DP / 4); x += 256) {
         const int r = x / (DP / 4), d = (x - r * (DP / 4)) * 4, rr = u.tile * FEW_ROWS + r;
-        if (rr >= rows || d >= a.dim) continue;
+        if (rr >= rows || d >= a->dim) continue;
         float m = fmaxf(fmaxf(part_m[0][r], part_m[1][r]), fmaxf(part_m[2][r], part_m[3][r])), l = 0;
         f32x4 y = f32x4{0, 0, 0, 0};
 #pragma unroll
@@ -411,57 +423,54 @@ __device__ __forceinline__ uint32_t few_unit(const AttnArgs& a, const Unit& u, c
                 y += f * *(const f32x4*)((const float*)(lds + w * WAVE) + r * OROW + d);
             }
         }
-        const int tok = rr / a.group, h = u.head * a.group + (rr - tok * a.group);
-        const long t = u.first + tok, at_row = t * a.q_heads + h;
+        const int tok = rr / a->group, h = u.head * a->group + (rr - tok * a->group);
+        const long t = u.first + tok, at_row = t * a->q_heads + h;
         if (u.cut.splits > 1) {
-            const long slot = at_row * a.splits + u.split;
-            *(f32x4*)(a.part_o + slot * a.dim + d) = y;
-            if (d == 0) a.part_ml[slot] = float2{m, l};
+            const long slot = at_row * a->splits + u.split;
+            *(f32x4*)(a->part_o + slot * a->dim + d) = y;
+            if (d == 0) a->part_ml[slot] = float2{m, l};
         } else {
-            const int p = a.causal ? u.len - u.n + tok : u.len - 1;
+            const int p = a->causal ? u.len - u.n + tok : u.len - 1;
             const bool none = p < 0;
             const float f = none ? 0.f : 1.f / l;
             Quad<T> z;
 #pragma unroll
             for (int i = 0; i < 4; ++i) z.e[i] = (T)(none ? 0.f : y[i] * f);
-            *(Quad<T>*)(a.out + t * a.out_token + h * a.out_head + d * 2) = z;
-            if (a.lse && d == 0) a.lse[at_row] = none ? -INFINITY : ((m == -INFINITY ? 0.f : m - Mat<T>::BIAS) + log2f(l)) * LN2;
+            *(Quad<T>*)(a->out + t * a->out_token + h * a->out_head + d * 2) = z;
+            if (a->lse && d == 0) a->lse[at_row] = none ? -INFINITY : ((m == -INFINITY ? 0.f : m - Mat<T>::BIAS) + log2f(l)) * LN2;
         }
     }
     return odd;
 }
 
 // The rare form as a function of its own, apart from the kernel's registers.  The kernel hands over where its arguments lie (only a kernel can ask for
-// that: in a function the builtin is null), and they are read into scalars again.
-__device__ __forceinline__ uint64_t kernel_args_at() { return (uint64_t)__builtin_amdgcn_kernarg_segment_ptr(); }
-__device__ __forceinline__ AttnArgs kernel_args(uint64_t at) {
-    constexpr int WORDS = sizeof(AttnArgs) / 4;
-    const uint32_t* p = (const uint32_t*)at;
-    struct Words { uint32_t w[WORDS]; } words;
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) words.w[i] = __builtin_amdgcn_readfirstlane(p[i]);
-    return __builtin_bit_cast(AttnArgs, words);
+// that: in a function the builtin is null).
+__device__ __forceinline__ uint64_t kernel_args() { return (uint64_t)__builtin_amdgcn_kernarg_segment_ptr(); }
+__device__ __forceinline__ ArgsAt args_at(uint64_t at) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at), hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+    return (ArgsAt)((uint64_t)hi << 32 | lo);
 }
 __device__ __forceinline__ uint32_t lds_offset(const void* p) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p; }
 __device__ __forceinline__ char* lds_pointer(uint32_t offset) { return (char*)(__attribute__((address_space(3))) char*)(uintptr_t)offset; }
 
 template <typename T, int DP>
 __device__ __noinline__ void few_unit_odd(uint64_t args, int want, uint32_t lds, uint32_t m, uint32_t l) {
-    const AttnArgs a = kernel_args(args);
+    const ArgsAt a = args_at(args);
     Unit u;
     if (!find_unit<true>(a, __builtin_amdgcn_readfirstlane(want), u)) return;
     few_unit<T, DP, true>(a, u, lds_pointer(lds), *(float (*)[4][16])lds_pointer(m), *(float (*)[4][16])lds_pointer(l));
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_few_kernel(AttnArgs) {
+    const ArgsAt a = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
     __shared__ __align__(16) char lds[4 * Few<T, DP>::WAVE];
     __shared__ float part_m[4][16], part_l[4][16];
     for (int want = blockIdx.x;; want += gridDim.x) {
         Unit u;
-        if (!find_unit<true>(a, want, u)) break;
-        if (__syncthreads_or(few_unit<T, DP, false>(a, u, lds, part_m, part_l) != 0)) {
-            few_unit_odd<T, DP>(kernel_args_at(), want, lds_offset(lds), lds_offset(part_m), lds_offset(part_l));
+        if (!find_unit<true>(fresh(a), want, u)) break;
+        if (__syncthreads_or(few_unit<T, DP, false>(fresh(a), u, lds, part_m, part_l) != 0)) {
+            few_unit_odd<T, DP>(kernel_args(), want, lds_offset(lds), lds_offset(part_m), lds_offset(part_l));
             __syncthreads();
         }
     }
@@ -488,30 +497,33 @@ template <int DP> constexpr int tile_keys() { return DP <= 128 ? 64 : 32; }
 template <int DP> constexpr int many_lds() { return 4 * tile_keys<DP>() * DP * 2; }
 
 template <typename T, int DP, bool ODD>
-__device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, char* lds) {
+__device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds) {
     typedef typename Mat<T>::x8 x8;
     constexpr int KT = tile_keys<DP>(), SUB = KT / 32, KS = DP / 16, DB = DP / 32, ROW = DP * 2, BUF = KT * ROW, NP = BUF / 4096;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-    const int head_bytes = a.dim * 2;
+    const int head_bytes = a->dim * 2;
     const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;      // keys, keys, values, values
-    const int rows = u.n * a.group, row0 = u.tile * MANY_ROWS + wave * 32;
+    const int rows = u.n * a->group, row0 = u.tile * MANY_ROWS + wave * 32;
     const int row = row0 + col, row_in = row < rows ? row : rows - 1;
-    const int token = row_in / a.group, head = u.head * a.group + (row_in - token * a.group);
-    const int pos = a.causal ? u.len - u.n + token : u.len - 1;
+    const int token = row_in / a->group, head = u.head * a->group + (row_in - token * a->group);
+    const int pos = a->causal ? u.len - u.n + token : u.len - 1;
     const bool any_row = row0 < rows;                          // of this wave
-    auto pos_of = [&](int r) { return a.causal ? u.len - u.n + min(r, rows - 1) / a.group : u.len - 1; };
+    auto pos_of = [&](int r) { return a->causal ? u.len - u.n + min(r, rows - 1) / a->group : u.len - 1; };
     const int low = pos_of(row0), high = pos_of(row0 + 31), tile_low = pos_of(u.tile * MANY_ROWS), tile_high = pos_of(u.tile * MANY_ROWS + MANY_ROWS - 1);
     const int split_begin = u.cut.begin + u.split * u.cut.chunk, end = min(min(split_begin + u.cut.chunk, u.len), tile_high + 1);
     int begin = split_begin;                                   // keys before the tile's first window are left out
-    if (a.window > 0 && tile_low - a.window + 1 > begin) begin = (tile_low - a.window + 1) & ~63;
+    if (a->window > 0 && tile_low - a->window + 1 > begin) begin = (tile_low - a->window + 1) & ~63;
+    // the keys that this lane's row sees here
+    const int first_seen = a->window > 0 ? pos - a->window + 1 : 0;
+    const uint32_t count_seen = max(0, min(pos + 1, end) - first_seen);
     x8 q[KS];
     {
-        const char* p = a.q + (u.first + token) * a.q_token + head * a.q_head;
+        const char* p = a->q + (u.first + token) * a->q_token + head * a->q_head;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             uint4 w = uint4{0, 0, 0, 0};
             if ((16 * ks + 8 * h) * 2 < head_bytes) w = *(const uint4*)(p + (16 * ks + 8 * h) * 2);
-            if (a.negate) { w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u; }
+            if (a->negate) { w.x ^= 0x80008000u; w.y ^= 0x80008000u; w.z ^= 0x80008000u; w.w ^= 0x80008000u; }
             q[ks] = __builtin_bit_cast(x8, w);
         }
     }
@@ -522,19 +534,19 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
         for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
     Run run;
     uint32_t odd = 0;
-    const int* table = a.table + (long)u.b * a.width;
-    const long head_at = u.head * a.head_stride;
-    const int slots = (1 << a.page_shift) - 1;
-    auto pages_at = [&](int k0) { return table[min(k0 + (lane & (KT - 1)), end - 1) >> a.page_shift]; };
+    const int* table = a->table + (long)u.b * a->width;
+    const long head_at = u.head * a->head_stride;
+    const int slots = (1 << a->page_shift) - 1;
+    auto pages_at = [&](int k0) { return table[min(k0 + (lane & (KT - 1)), end - 1) >> a->page_shift]; };
     auto fetch = [&](int k0, int pg, int buf) {                // the wave's share of a tile: NP runs of 1 KB of keys and of values
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int at = (i * 4 + wave) * 1024, x = at + lane * 16, r = x / ROW, piece = (x - r * ROW) / 16;
-            const int page = __shfl(pg, r), p = (unsigned)page < (unsigned)a.pages ? page : 0;
-            const long from = p * a.page_stride + (min(k0 + r, end - 1) & slots) * a.slot_stride + head_at;
+            const int page = __shfl(pg, r), p = (unsigned)page < (unsigned)a->pages ? page : 0;
+            const long from = p * a->page_stride + (min(k0 + r, end - 1) & slots) * a->slot_stride + head_at;
             const int kp = key_piece<DP>(r, piece) * 16, vp = value_piece<DP>(r, piece) * 16;
-            if (kp < head_bytes) dma16(a.k + from + kp, lds_at + buf * BUF + at);
-            if (vp < head_bytes) dma16(a.v + from + vp, lds_at + (2 + buf) * BUF + at);
+            if (kp < head_bytes) dma16(a->k + from + kp, lds_at + buf * BUF + at);
+            if (vp < head_bytes) dma16(a->v + from + vp, lds_at + (2 + buf) * BUF + at);
         }
     };
     auto tile = [&](auto masked, int k0, const char* kb, const char* vb, unsigned long long bad) {
@@ -556,8 +568,8 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
                     seen[t] = 0;
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int in_tile = 32 * t + (r & 3) + 8 * (r >> 2) + 4 * h, key = k0 + in_tile;
-                        const bool sees = key < end && key <= pos && (a.window == 0 || key > pos - a.window);
+                        const int in_tile = 32 * t + (r & 3) + 8 * (r >> 2) + 4 * h;
+                        const bool sees = (uint32_t)(k0 + in_tile - first_seen) < count_seen;
                         if (ODD && sees) seen[t] |= 1u << r;
                         s[t][r] = !sees ? -INFINITY : (ODD && (bad >> in_tile & 1) ? __builtin_nanf("") : s[t][r]);
                     }
@@ -571,7 +583,7 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
             for (int t = 0; t < SUB; ++t)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const float e = exp2_of(fmaf(s[t][j], a.c, -base));
+                    const float e = exp2_of(fmaf(s[t][j], a->c, -base));
                     sum += e;
                     p[t][j >> 3][j & 7] = (T)e;
                 }
@@ -589,7 +601,7 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, s[t][r]);
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float back = run.raise(asks | __shfl_xor((int)asks, 32), top * a.c);
+            const float back = run.raise(asks | __shfl_xor((int)asks, 32), top * a->c);
 #pragma unroll
             for (int i = 0; i < DB; ++i) o[i] *= back;
             sum = weights();
@@ -623,23 +635,24 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
     int buf = 0, k0 = begin;
     auto walk = [&](auto masked, int stop) {
         for (; k0 < stop; k0 += KT, buf ^= 1) {
-            const unsigned long long bad = __ballot((unsigned)pg >= (unsigned)a.pages);
+            const unsigned long long bad = __ballot((unsigned)pg >= (unsigned)a->pages);
             if (!ODD) odd |= bad != 0;
-            if (k0 + KT < end) {
-                fetch(k0 + KT, pg_next, buf ^ 1);
-                pg = pg_next;
-                pg_next = pages_at(k0 + 2 * KT);
-            }
-            if (any_row && (!decltype(masked)::value || (k0 <= high && (a.window == 0 || k0 + KT - 1 > low - a.window))))
+            // (the pages of the tile after the next: asked for ahead of the copies, looked at behind dma_landed() - a look in between would wait for the
+            // copies as well)
+            const int pg_after = pages_at(k0 + 2 * KT);
+            if (k0 + KT < end) fetch(k0 + KT, pg_next, buf ^ 1);
+            if (any_row && (!decltype(masked)::value || (k0 <= high && (a->window == 0 || k0 + KT - 1 > low - a->window))))
                 tile(masked, k0, lds + buf * BUF, lds + (2 + buf) * BUF, bad);
             dma_landed();
+            pg = pg_next;
+            pg_next = pg_after;
             __syncthreads();
         }
     };
     // tiles that some row of the workgroup sees in part lie before and behind those that all rows see whole
     int whole_from = begin, whole_to = begin;
     if (!ODD) {
-        if (a.window > 0) whole_from = min(end, begin + max(0, (tile_high - a.window - begin + KT) / KT * KT));
+        if (a->window > 0) whole_from = min(end, begin + (int)max(0l, ((long)tile_high - a->window - begin + KT) / KT * KT));
         whole_to = begin + max(0, min(end, tile_low + 1) - begin) / KT * KT;
     }
     for (int part = 0; part < 2; ++part) {
@@ -647,17 +660,18 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
         if (!ODD && part == 0) walk(std::false_type(), whole_to);
     }
     run.l += __shfl_xor(run.l, 32);
+    a = fresh(a);
     if (row < rows) {
-        const long t = u.first + token, at_row = t * a.q_heads + head;
+        const long t = u.first + token, at_row = t * a->q_heads + head;
         if (u.cut.splits > 1) {
-            const long slot = at_row * a.splits + u.split;
-            if (h == 0) a.part_ml[slot] = float2{run.m, run.l};
+            const long slot = at_row * a->splits + u.split;
+            if (h == 0) a->part_ml[slot] = float2{run.m, run.l};
 #pragma unroll
             for (int i = 0; i < DB; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
                     const int d = 32 * i + 2 * r + 4 * h;
-                    if (d < a.dim) *(f32x4*)(a.part_o + slot * a.dim + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+                    if (d < a->dim) *(f32x4*)(a->part_o + slot * a->dim + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
                 }
         } else {
             const bool none = pos < 0;
@@ -667,13 +681,13 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
                     const int d = 32 * i + 2 * r + 4 * h;
-                    if (d >= a.dim) continue;
+                    if (d >= a->dim) continue;
                     Quad<T> z;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) z.e[j] = (T)(none ? 0.f : o[i][r + j] * f);
-                    *(Quad<T>*)(a.out + t * a.out_token + head * a.out_head + d * 2) = z;
+                    *(Quad<T>*)(a->out + t * a->out_token + head * a->out_head + d * 2) = z;
                 }
-            if (a.lse && h == 0) a.lse[at_row] = none ? -INFINITY : (run.base<T>() + log2f(run.l)) * LN2;
+            if (a->lse && h == 0) a->lse[at_row] = none ? -INFINITY : (run.base<T>() + log2f(run.l)) * LN2;
         }
     }
     return odd;
@@ -681,70 +695,130 @@ __device__ __forceinline__ uint32_t many_unit(const AttnArgs& a, const Unit& u, 
 
 template <typename T, int DP>
 __device__ __noinline__ void many_unit_odd(uint64_t args, int want, uint32_t lds) {
-    const AttnArgs a = kernel_args(args);
+    const ArgsAt a = args_at(args);
     Unit u;
     if (!find_unit<false>(a, __builtin_amdgcn_readfirstlane(want), u)) return;
     many_unit<T, DP, true>(a, u, lds_pointer(lds));
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_many_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_many_kernel(AttnArgs) {
+    const ArgsAt a = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
     extern __shared__ __align__(16) char lds[];
-    if (a.dim < DP) {                                              // what lies behind the head's end is never copied: zeros
+    if (a->dim < DP) {                                             // what lies behind the head's end is never copied: zeros
         for (int x = threadIdx.x * 16; x < many_lds<DP>(); x += 4096) *(uint4*)(lds + x) = uint4{0, 0, 0, 0};
         __syncthreads();
     }
     for (int want = blockIdx.x;; want += gridDim.x) {
         Unit u;
-        if (!find_unit<false>(a, want, u)) break;
-        if (__syncthreads_or(many_unit<T, DP, false>(a, u, lds) != 0)) many_unit_odd<T, DP>(kernel_args_at(), want, lds_offset(lds));
+        if (!find_unit<false>(fresh(a), want, u)) break;
+        if (__syncthreads_or(many_unit<T, DP, false>(fresh(a), u, lds) != 0)) many_unit_odd<T, DP>(kernel_args(), want, lds_offset(lds));
     }
 }
 
 // ---- the parts of a row whose keys were split -------------------------------------------------------------------------------------------------
-// A wave a row: lane = split for the weights, lane = elements for the sums
-template <typename T>
-__global__ __launch_bounds__(256) void cache_attention_join_kernel(AttnArgs a) {
-    const int lane = threadIdx.x & 63;
-    const long at_row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at_row >= (long)a.tokens * a.q_heads) return;
-    const int t = (int)(at_row / a.q_heads), h = (int)(at_row - (long)t * a.q_heads);
+// Part s counts into sum s % 8, the eight sums are added as ((0 + 1) + (2 + 3)) + ((4 + 5) + (6 + 7)), whichever of the two forms joins a row: how a row is
+// joined does not depend on the parts that other rows have.  Both are bound by latency, the loads of a row's parts all under way at once.
+//   a few rows of many parts   four waves a row, a part a team of dim / 4 lanes (64 rows of 64 parts of 128: 7 us)
+//   many rows                  dim / 4 lanes a row, a wave takes 256 / dim heads of a token
+struct Joined { int n, len, first, splits; };
+
+__device__ __forceinline__ Joined joined_of(const AttnArgs& a, int t) {
+    Joined j{0, 0, 0, 0};
     const int b = seq_of_token(a.cu_new, a.rows, t);
-    if (b >= a.rows) return;
-    const int first = a.cu_new[b], n = a.cu_new[b + 1] - first, len = clamp_len(a.lens[b], a.width << a.page_shift);
-    if (first < 0 || n < 0 || n > a.tokens || first > a.tokens - n || t < first || t >= first + n) return;
-    const Cut cut = cut_of(n, len, a.group, a.kv_heads, a.window, a.few, a.splits);
-    if (cut.splits <= 1) return;
-    const int pos = a.causal ? len - n + (t - first) : len - 1;
-    // the splits that hold keys of this row (the others may not have been written for it)
-    float2 ml = float2{-INFINITY, 0.f};
-    if (lane < cut.splits) ml = a.part_ml[at_row * a.splits + lane];
+    if (b >= a.rows) return j;
+    j.first = a.cu_new[b];
+    j.n = a.cu_new[b + 1] - j.first;
+    j.len = clamp_len(a.lens[b], a.width << a.page_shift);
+    if (j.first < 0 || j.n < 0 || j.n > a.tokens || j.first > a.tokens - j.n || t < j.first || t >= j.first + j.n) j.n = 0;
+    if (j.n > 0) j.splits = cut_of(j.n, j.len, a.group, a.kv_heads, a.window, a.few, a.splits).splits;
+    return j;
+}
+
+// the factor of a part of maximum m and sum l, `top` being the row's maximum; 0: a part that saw no key of the row, and left no numbers
+__device__ __forceinline__ float weight_of(float2 ml, float top) { return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_of(ml.x - top); }
+
+template <typename T>
+__device__ __forceinline__ void put_joined(const AttnArgs& a, const Joined& j, int t, int h, int d, f32x4 y, float m, float l) {
+    const bool none = a.causal ? j.len - j.n + (t - j.first) < 0 : j.len <= 0;
+    const float f = none ? 0.f : 1.f / l;
+    Quad<T> r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.e[i] = (T)(none ? 0.f : y[i] * f);
+    *(Quad<T>*)(a.out + t * a.out_token + h * a.out_head + d * 2) = r;
+    if (a.lse && d == 0) a.lse[(long)t * a.q_heads + h] = none ? -INFINITY : ((m == -INFINITY ? 0.f : m - Mat<T>::BIAS) + log2f(l)) * LN2;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void cache_attention_join_kernel(AttnArgs a, int waves_a_token) {
+    const int lane = threadIdx.x & 63, quads = a.dim / 4, at_once = 64 / quads;
+    const int wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = wave / waves_a_token;
+    if (t >= a.tokens) return;
+    const Joined j = joined_of(a, t);
+    const int h = (wave - t * waves_a_token) * at_once + lane / quads, d = lane % quads * 4;
+    if (j.splits <= 1 || lane / quads >= at_once || h >= a.q_heads) return;
+    const long slot = ((long)t * a.q_heads + h) * a.splits;
+    float m = -INFINITY, l[8];
+    f32x4 y[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) { l[g] = 0.f; y[g] = f32x4{0, 0, 0, 0}; }
+    for (int s0 = 0; s0 < j.splits; s0 += 8)
+#pragma unroll
+        for (int g = 0; g < 8; ++g) if (s0 + g < j.splits) m = fmaxf(m, a.part_ml[slot + s0 + g].x);
+    for (int s0 = 0; s0 < j.splits; s0 += 8) {
+        float w[8];
+        f32x4 x[8];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+            const float2 ml = s0 + g < j.splits ? a.part_ml[slot + s0 + g] : float2{-INFINITY, 0.f};
+            w[g] = weight_of(ml, m);
+            x[g] = s0 + g < j.splits ? *(const f32x4*)(a.part_o + (slot + s0 + g) * a.dim + d) : f32x4{0, 0, 0, 0};
+            l[g] += w[g] != 0.f ? w[g] * ml.y : 0.f;
+        }
+#pragma unroll
+        for (int g = 0; g < 8; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[g][i] += w[g] != 0.f ? w[g] * x[g][i] : 0.f;
+    }
+    put_joined<T>(a, j, t, h, d, ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7])), m,
+                  ((l[0] + l[1]) + (l[2] + l[3])) + ((l[4] + l[5]) + (l[6] + l[7])));
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void cache_attention_join_row_kernel(AttnArgs a) {
+    __shared__ __align__(16) float sums[8][256];
+    const int lane = threadIdx.x & 63, t = blockIdx.x / a.q_heads, h = blockIdx.x - t * a.q_heads;
+    const Joined j = joined_of(a, t);
+    if (j.splits <= 1) return;
+    const long slot = (long)blockIdx.x * a.splits;
+    const float2 ml = lane < j.splits ? a.part_ml[slot + lane] : float2{-INFINITY, 0.f};
     float m = ml.x;
 #pragma unroll
     for (int i = 32; i; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
-    const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_of(ml.x - m);
-    float l = w == 0.f ? 0.f : w * ml.y;
+    const float w = weight_of(ml, m), part_l = w != 0.f ? w * ml.y : 0.f;
+    float l = 0.f;
 #pragma unroll
-    for (int i = 32; i; i >>= 1) l += __shfl_xor(l, i);
-    const bool none = pos < 0;
-    const float f = none ? 0.f : 1.f / l;
-    const int d = lane * 4;                                        // (dim is at most 256; every lane stays, its weight is asked for)
-    const float* parts = a.part_o + at_row * a.splits * a.dim + (d < a.dim ? d : 0);
-    f32x4 y = f32x4{0, 0, 0, 0};
-#pragma unroll 8
-    for (int s = 0; s < cut.splits; ++s) {
-        const float ws = __shfl(w, s);
-        const f32x4 x = *(const f32x4*)(parts + (long)s * a.dim);
+    for (int s0 = 0; s0 < 64; s0 += 8) l += __shfl(part_l, s0 + (lane & 7));
+    l += __shfl_xor(l, 1);
+    l += __shfl_xor(l, 2);
+    l += __shfl_xor(l, 4);
+    const int quads = a.dim / 4, teams = 256 / quads < 8 ? 256 / quads : 8, team = threadIdx.x / quads, d = (threadIdx.x - team * quads) * 4;
+    for (int g0 = 0; g0 < 8; g0 += teams) {                        // (the weights are asked of all lanes: nobody leaves the loop early)
+        const int g = g0 + team;
+        f32x4 sum = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] += ws != 0.f ? ws * x[i] : 0.f;     // (what a split without a key of the row left there is not a number)
+        for (int s0 = 0; s0 < 64; s0 += 8) {
+            const float ws = __shfl(w, (s0 + g) & 63);
+            if (team < teams && g < 8 && s0 + g < j.splits && ws != 0.f) sum += ws * *(const f32x4*)(a.part_o + (slot + s0 + g) * a.dim + d);
+        }
+        if (team < teams && g < 8) *(f32x4*)&sums[g][d] = sum;
     }
-    if (d < a.dim) {
-        Quad<T> z;
+    __syncthreads();
+    if ((int)threadIdx.x >= quads) return;
+    f32x4 y[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z.e[i] = (T)(none ? 0.f : y[i] * f);
-        *(Quad<T>*)(a.out + t * a.out_token + h * a.out_head + d * 2) = z;
-    }
-    if (a.lse && lane == 0) a.lse[at_row] = none ? -INFINITY : ((m == -INFINITY ? 0.f : m - Mat<T>::BIAS) + log2f(l)) * LN2;
+    for (int g = 0; g < 8; ++g) y[g] = *(const f32x4*)&sums[g][threadIdx.x * 4];
+    put_joined<T>(a, j, t, h, threadIdx.x * 4, ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7])), m, l);
 }
 
 // ---- what the host decides ----------------------------------------------------------------------------------------------------------------------
@@ -795,11 +869,16 @@ int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
         DISCO_LAUNCH_CHECK("cache_attention_many_kernel");
     }
     if (p.few) {
-        cache_attention_few_kernel<T, DP><<<grid_for(p.few_units, 1024), 256, 0, s>>>(a);
+        cache_attention_few_kernel<T, DP><<<grid_for(p.few_units, DP <= 128 ? 512 : 256), 256, 0, s>>>(a);
         DISCO_LAUNCH_CHECK("cache_attention_few_kernel");
     }
     if (p.splits > 1) {
-        cache_attention_join_kernel<T><<<(unsigned)(((long)a.tokens * a.q_heads + 3) / 4), 256, 0, s>>>(a);
+        const long rows = (long)a.tokens * a.q_heads;
+        if (p.splits > 8 && rows <= 2048) cache_attention_join_row_kernel<T><<<(unsigned)rows, 256, 0, s>>>(a);
+        else {
+            const int waves_a_token = cdiv(a.q_heads, 256 / a.dim);
+            cache_attention_join_kernel<T><<<(unsigned)(((long)a.tokens * waves_a_token + 3) / 4), 256, 0, s>>>(a, waves_a_token);
+        }
         DISCO_LAUNCH_CHECK("cache_attention_join_kernel");
     }
     return DISCO_OK;
@@ -828,10 +907,11 @@ int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc
                            const int* cu_new, void* out, float* lse, void* ws, hipStream_t s) {
     const Plan p = plan_of(c, d);
     const size_t parts = (size_t)d.tokens * d.q_heads * p.splits;
+    const int window = d.window >= (long)c.table_width * c.page_size ? 0 : d.window;      // (no key is that far back)
     AttnArgs a{(const char*)q, (const char*)c.d_k, (const char*)c.d_v, (char*)out, lse, (float*)ws, (float2*)((char*)ws + (p.splits > 1 ? parts * c.dim * 4 : 0)),
                table, lens, cu_new, d.q_token * 2, d.q_head * 2, d.out_token * 2, d.out_head * 2, c.page_stride * 2, c.head_stride * 2, c.slot_stride * 2,
                d.tokens, d.q_heads, c.kv_heads, d.q_heads / c.kv_heads, c.dim, c.rows, c.table_width, c.pages, __builtin_ctz((unsigned)c.page_size), d.causal,
-               d.window, p.splits, p.few_limit, fabsf(d.scale) * 1.4426950408889634f, d.scale < 0};
+               window, p.splits, p.few_limit, fabsf(d.scale) * 1.4426950408889634f, d.scale < 0};
     if (a.c < 1e-37f) a.c = 1e-37f;                                // 0 * -inf is not the score of a key that is not seen
     return c.dtype == DISCO_F16 ? run_dims<f16>(a, p, s) : run_dims<bf16>(a, p, s);
 }
