@@ -8,10 +8,13 @@
 // but that between the lanes of a column, and the registers that hold the probabilities are in place the operand of O^T = V^T P^T (their key order
 // is the accumulator's; V^T is read in the same order by the transposing LDS read).
 //
-// Two forms, chosen by a sequence's own rows (new tokens * group), so that its result does not depend on what else is in the call:
-//   few rows   (cache_attention_few_kernel)   16 rows a workgroup, its four waves deal 32-key tiles: bound by reading the cache
-//   many rows  (cache_attention_many_kernel)  128 rows a workgroup, 32 a wave, keys and values staged in LDS for all four: bound by the matrix
-//                                             cores, the exponentials and LDS together
+// Three forms, chosen by a sequence's own rows (new tokens * group), so that its result does not depend on what else is in the call:
+//   few (up to 32 rows)    cache_attention_few_kernel: 16 rows a workgroup, its four waves deal 32-key tiles; bound by reading the cache
+//   many (up to 1 024)     cache_attention_many_kernel, 128 rows a workgroup, 32 a wave, keys and values staged in LDS for all of them; two workgroups
+//                          a CU, bound by what L2 delivers into LDS (7 TB/s over the chip) and, at short ranges, by latency
+//   large                  the same with 256 rows, which halves what is delivered; bound by the matrix cores and the exponentials, which overlap in part
+//                          (2 048 tokens of 32 heads of 128 behind 16 384 keys: 128 rows 588 us, 256 rows 530 us; 257 tokens behind 4 111 keys:
+//                          79 and 93 us, a CU then having nothing to do beside one workgroup's start and end).  Heads above 128: 128 rows.
 // Where a sequence alone does not fill the GPU its keys are split; the parts (m, sum, o in fp32) are joined by cache_attention_join_kernel.
 //
 // A tile that some row sees only in part, or that has a page outside the cache, takes the masked path: scores of unseen keys are replaced (never
@@ -51,7 +54,7 @@ struct AttnArgs {
     long q_token, q_head, out_token, out_head, page_stride, head_stride, slot_stride;    // bytes
     int tokens, q_heads, kv_heads, group, dim, rows, width, pages, page_shift, causal, window;
     int splits;                                                    // parts of a row that the workspace has room for
-    int few;                                                       // sequences of at most so many rows take the few-rows form
+    int few, many;                                                 // sequences of at most so many rows take the form of few, of many rows
     float c;                                                       // |scale| log2 e, not 0
     int negate;                                                    // scale < 0: the queries change sign instead
 };
@@ -64,34 +67,37 @@ __device__ __forceinline__ ArgsAt fresh(ArgsAt p) {
     return p;
 }
 
-constexpr int FEW_ROWS = 16, MANY_ROWS = 128;
+// forms, by the rows of a sequence
+enum Form { FEW, MANY, LARGE };
+__host__ __device__ constexpr int rows_of(int form) { return form == FEW ? 16 : (form == MANY ? 128 : 256); }      // of a workgroup
 constexpr float LN2 = 0.6931471805599453f;
 
 // ---- how a sequence is cut ------------------------------------------------------------------------------------------------------------
-struct Cut { int tiles, splits, begin, chunk; };
+struct Cut { int form, tiles, splits, begin, chunk; };
 
 // parts of a sequence's keys; grows with them
 // few rows: a workgroup's waves take 128 keys a round, and up to 512 keys (4 us) one workgroup is done sooner than two and a join; 64 parts of 8 key
 //           heads are two workgroups a CU
-// many rows: as many parts as make 256 workgroups of the sequence, of at least 512 keys (a part costs a write and a read of its rows in fp32)
-__host__ __device__ __forceinline__ int splits_of(bool few, int tiles, int keys, int kv_heads) {
-    if (few) return keys <= 512 ? 1 : (keys > 64 * 256 ? 64 : (keys + 255) / 256);
+// many rows: as many parts as make 256 workgroups of the sequence, of at least 1 024 keys (a part costs a write and a read of its rows in fp32: 24 sequences of up to 257 tokens over
+//           4 111 take 78 us, with parts of 512 keys 93)
+__host__ __device__ __forceinline__ int splits_of(int form, int tiles, int keys, int kv_heads) {
+    if (form == FEW) return keys <= 512 ? 1 : (keys > 64 * 256 ? 64 : (keys + 255) / 256);
     const int units = tiles * kv_heads;
     int s = units >= 256 ? 1 : 256 / units;
     if (s > 8) s = 8;
-    const int by_keys = keys <= 512 ? 1 : (keys + 511) / 512;
+    const int by_keys = keys <= 1024 ? 1 : (keys + 1023) / 1024;
     return s < by_keys ? s : by_keys;
 }
 
 // keys that some new token of the sequence sees: begin (a multiple of 64) .. len; every part takes `chunk` of them, a multiple of 128
-__host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv_heads, int window, int few, int most) {
+__host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv_heads, int window, int few, int many, int most) {
     Cut u;
     const int rows = n * group;
-    const bool is_few = rows <= few;
+    u.form = rows <= few ? FEW : (rows <= many ? MANY : LARGE);
     u.begin = window > 0 && len - n - window + 1 > 0 ? (len - n - window + 1) & ~63 : 0;
-    const int keys = len - u.begin;
-    u.tiles = is_few ? (rows + FEW_ROWS - 1) / FEW_ROWS : (rows + MANY_ROWS - 1) / MANY_ROWS;
-    int s = splits_of(is_few, u.tiles, keys, kv_heads);
+    const int keys = len - u.begin, tile = rows_of(u.form);
+    u.tiles = (rows + tile - 1) / tile;
+    int s = splits_of(u.form, u.tiles, keys, kv_heads);
     if (s > most) s = most;
     u.chunk = ((keys + s - 1) / s + 127) & ~127;
     if (u.chunk < 128) u.chunk = 128;
@@ -102,9 +108,9 @@ __host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv
 
 struct Unit { int b, n, len, first, tile, split, head; Cut cut; };
 
-// unit number `want` of the form FEW over all sequences (key head fastest, then split, then tile - the last, longest tiles first); false behind the last.
+// unit number `want` of a form over all sequences (key head fastest, then split, then tile - the last, longest tiles first); false behind the last.
 // Every lane of the wave calls it and gets the same.
-template <bool FEW>
+template <int FORM>
 __device__ __forceinline__ bool find_unit(ArgsAt a, int want, Unit& u) {
     const int lane = threadIdx.x & 63, capacity = a->width << a->page_shift;
     int left = want;
@@ -117,9 +123,9 @@ __device__ __forceinline__ bool find_unit(ArgsAt a, int want, Unit& u) {
             n = a->cu_new[b + 1] - first;
             len = clamp_len(a->lens[b], capacity);
             if (first < 0 || n < 0 || n > a->tokens || first > a->tokens - n) n = 0;       // (not offsets)
-            if (n > 0 && (n * (long)a->group <= a->few) == FEW) {
-                cut = cut_of(n, len, a->group, a->kv_heads, a->window, a->few, a->splits);
-                units = cut.tiles * cut.splits * a->kv_heads;
+            if (n > 0) {
+                cut = cut_of(n, len, a->group, a->kv_heads, a->window, a->few, a->many, a->splits);
+                if (cut.form == FORM) units = cut.tiles * cut.splits * a->kv_heads;
             }
         }
         int upto = units;
@@ -252,10 +258,10 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
     const int head_bytes = a->dim * 2;
     const int rows = u.n * a->group;
     // this lane's row: its token, its head, its position
-    const int row = u.tile * FEW_ROWS + col, row_in = row < rows ? row : rows - 1;
+    const int row = u.tile * rows_of(FEW) + col, row_in = row < rows ? row : rows - 1;
     const int token = row_in / a->group, head = u.head * a->group + (row_in - token * a->group);
     const int pos = a->causal ? u.len - u.n + token : u.len - 1;
-    const int last_token = (min(u.tile * FEW_ROWS + FEW_ROWS, rows) - 1) / a->group, first_token = u.tile * FEW_ROWS / a->group;
+    const int last_token = (min(u.tile * rows_of(FEW) + rows_of(FEW), rows) - 1) / a->group, first_token = u.tile * rows_of(FEW) / a->group;
     const int high = a->causal ? u.len - u.n + last_token : u.len - 1, low = a->causal ? u.len - u.n + first_token : u.len - 1;
     const int begin = u.cut.begin + u.split * u.cut.chunk, end = min(min(begin + u.cut.chunk, u.len), high + 1);
     // the keys that this lane's row sees here
@@ -411,7 +417,7 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
     if (g == 0) { part_m[wave][col] = run.m; part_l[wave][col] = run.l; }
     __syncthreads();
     for (int x = threadIdx.x; x < 16 * (DP / 4); x += 256) {
-        const int r = x / (DP / 4), d = (x - r * (DP / 4)) * 4, rr = u.tile * FEW_ROWS + r;
+        const int r = x / (DP / 4), d = (x - r * (DP / 4)) * 4, rr = u.tile * rows_of(FEW) + r;
         if (rr >= rows || d >= a->dim) continue;
         float m = fmaxf(fmaxf(part_m[0][r], part_m[1][r]), fmaxf(part_m[2][r], part_m[3][r])), l = 0;
         f32x4 y = f32x4{0, 0, 0, 0};
@@ -457,7 +463,7 @@ template <typename T, int DP>
 __device__ __noinline__ void few_unit_odd(uint64_t args, int want, uint32_t lds, uint32_t m, uint32_t l) {
     const ArgsAt a = args_at(args);
     Unit u;
-    if (!find_unit<true>(a, __builtin_amdgcn_readfirstlane(want), u)) return;
+    if (!find_unit<FEW>(a, __builtin_amdgcn_readfirstlane(want), u)) return;
     few_unit<T, DP, true>(a, u, lds_pointer(lds), *(float (*)[4][16])lds_pointer(m), *(float (*)[4][16])lds_pointer(l));
 }
 
@@ -468,7 +474,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_few_ke
     __shared__ float part_m[4][16], part_l[4][16];
     for (int want = blockIdx.x;; want += gridDim.x) {
         Unit u;
-        if (!find_unit<true>(fresh(a), want, u)) break;
+        if (!find_unit<FEW>(fresh(a), want, u)) break;
         if (__syncthreads_or(few_unit<T, DP, false>(fresh(a), u, lds, part_m, part_l) != 0)) {
             few_unit_odd<T, DP>(kernel_args(), want, lds_offset(lds), lds_offset(part_m), lds_offset(part_l));
             __syncthreads();
@@ -496,20 +502,20 @@ template <int DP> __device__ __forceinline__ int value_piece(int row, int piece)
 template <int DP> constexpr int tile_keys() { return DP <= 128 ? 64 : 32; }
 template <int DP> constexpr int many_lds() { return 4 * tile_keys<DP>() * DP * 2; }
 
-template <typename T, int DP, bool ODD>
+template <typename T, int DP, int FORM, bool ODD>
 __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds) {
     typedef typename Mat<T>::x8 x8;
-    constexpr int KT = tile_keys<DP>(), SUB = KT / 32, KS = DP / 16, DB = DP / 32, ROW = DP * 2, BUF = KT * ROW, NP = BUF / 4096;
+    constexpr int ROWS = rows_of(FORM), KT = tile_keys<DP>(), SUB = KT / 32, KS = DP / 16, DB = DP / 32, ROW = DP * 2, BUF = KT * ROW, STEP = 32 * ROWS, NP = (BUF + STEP - 1) / STEP;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
     const int head_bytes = a->dim * 2;
     const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;      // keys, keys, values, values
-    const int rows = u.n * a->group, row0 = u.tile * MANY_ROWS + wave * 32;
+    const int rows = u.n * a->group, row0 = u.tile * ROWS + wave * 32;
     const int row = row0 + col, row_in = row < rows ? row : rows - 1;
     const int token = row_in / a->group, head = u.head * a->group + (row_in - token * a->group);
     const int pos = a->causal ? u.len - u.n + token : u.len - 1;
     const bool any_row = row0 < rows;                          // of this wave
     auto pos_of = [&](int r) { return a->causal ? u.len - u.n + min(r, rows - 1) / a->group : u.len - 1; };
-    const int low = pos_of(row0), high = pos_of(row0 + 31), tile_low = pos_of(u.tile * MANY_ROWS), tile_high = pos_of(u.tile * MANY_ROWS + MANY_ROWS - 1);
+    const int low = pos_of(row0), high = pos_of(row0 + 31), tile_low = pos_of(u.tile * ROWS), tile_high = pos_of(u.tile * ROWS + ROWS - 1);
     const int split_begin = u.cut.begin + u.split * u.cut.chunk, end = min(min(split_begin + u.cut.chunk, u.len), tile_high + 1);
     int begin = split_begin;                                   // keys before the tile's first window are left out
     if (a->window > 0 && tile_low - a->window + 1 > begin) begin = (tile_low - a->window + 1) & ~63;
@@ -541,7 +547,8 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
     auto fetch = [&](int k0, int pg, int buf) {                // the wave's share of a tile: NP runs of 1 KB of keys and of values
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int at = (i * 4 + wave) * 1024, x = at + lane * 16, r = x / ROW, piece = (x - r * ROW) / 16;
+            const int at = i * STEP + wave * 1024, x = at + lane * 16, r = x / ROW, piece = (x - r * ROW) / 16;
+            if (BUF % STEP && at >= BUF) break;                    // (fewer runs than waves)
             const int page = __shfl(pg, r), p = (unsigned)page < (unsigned)a->pages ? page : 0;
             const long from = p * a->page_stride + (min(k0 + r, end - 1) & slots) * a->slot_stride + head_at;
             const int kp = key_piece<DP>(r, piece) * 16, vp = value_piece<DP>(r, piece) * 16;
@@ -693,26 +700,26 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
     return odd;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int FORM>
 __device__ __noinline__ void many_unit_odd(uint64_t args, int want, uint32_t lds) {
     const ArgsAt a = args_at(args);
     Unit u;
-    if (!find_unit<false>(a, __builtin_amdgcn_readfirstlane(want), u)) return;
-    many_unit<T, DP, true>(a, u, lds_pointer(lds));
+    if (!find_unit<FORM>(a, __builtin_amdgcn_readfirstlane(want), u)) return;
+    many_unit<T, DP, FORM, true>(a, u, lds_pointer(lds));
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_many_kernel(AttnArgs) {
+template <typename T, int DP, int FORM>
+__global__ __launch_bounds__(2 * rows_of(FORM), DP <= 128 ? 2 : 1) void cache_attention_many_kernel(AttnArgs) {
     const ArgsAt a = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
     extern __shared__ __align__(16) char lds[];
     if (a->dim < DP) {                                             // what lies behind the head's end is never copied: zeros
-        for (int x = threadIdx.x * 16; x < many_lds<DP>(); x += 4096) *(uint4*)(lds + x) = uint4{0, 0, 0, 0};
+        for (int x = threadIdx.x * 16; x < many_lds<DP>(); x += 32 * rows_of(FORM)) *(uint4*)(lds + x) = uint4{0, 0, 0, 0};
         __syncthreads();
     }
     for (int want = blockIdx.x;; want += gridDim.x) {
         Unit u;
-        if (!find_unit<false>(fresh(a), want, u)) break;
-        if (__syncthreads_or(many_unit<T, DP, false>(fresh(a), u, lds) != 0)) many_unit_odd<T, DP>(kernel_args(), want, lds_offset(lds));
+        if (!find_unit<FORM>(fresh(a), want, u)) break;
+        if (__syncthreads_or(many_unit<T, DP, FORM, false>(fresh(a), u, lds) != 0)) many_unit_odd<T, DP, FORM>(kernel_args(), want, lds_offset(lds));
     }
 }
 
@@ -731,7 +738,7 @@ __device__ __forceinline__ Joined joined_of(const AttnArgs& a, int t) {
     j.n = a.cu_new[b + 1] - j.first;
     j.len = clamp_len(a.lens[b], a.width << a.page_shift);
     if (j.first < 0 || j.n < 0 || j.n > a.tokens || j.first > a.tokens - j.n || t < j.first || t >= j.first + j.n) j.n = 0;
-    if (j.n > 0) j.splits = cut_of(j.n, j.len, a.group, a.kv_heads, a.window, a.few, a.splits).splits;
+    if (j.n > 0) j.splits = cut_of(j.n, j.len, a.group, a.kv_heads, a.window, a.few, a.many, a.splits).splits;
     return j;
 }
 
@@ -822,14 +829,13 @@ __global__ __launch_bounds__(256) void cache_attention_join_row_kernel(AttnArgs 
 }
 
 // ---- what the host decides ----------------------------------------------------------------------------------------------------------------------
-// sequences of at most so many rows take the few-rows form
-constexpr int FEW_LIMIT = 32;
+constexpr int FEW_LIMIT = 32, MANY_LIMIT = 1024;
 
 struct Plan {
-    bool few, many;      // which forms are launched
-    int few_limit;       // rows (INT_MAX: all)
-    int splits;          // a row's parts, at most
-    long few_units, many_units;
+    bool few, many, large;             // which forms are launched
+    int few_limit, many_limit;         // rows (INT_MAX: all)
+    int splits;                        // a row's parts, at most
+    long few_units, many_units, large_units;
 };
 
 Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
@@ -839,35 +845,46 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     const int len = (int)(d.max_len > 0 && d.max_len < capacity ? d.max_len : capacity);
     const int most_new = d.max_new > 0 && d.max_new < d.tokens ? d.max_new : d.tokens;
     const bool alone = c.rows == 1;                                // then its new tokens are all of them
-    p.many = (long)(alone ? d.tokens : most_new) * group > FEW_LIMIT;
-    p.few = !(alone && p.many);
-    p.few_limit = p.many ? FEW_LIMIT : 0x7fffffff;
+    const long most_rows = (long)(alone ? d.tokens : most_new) * group;
+    const bool wide = c.dim > 128;                                 // (256 rows of them do not fit the registers)
+    p.large = most_rows > MANY_LIMIT && !wide;
+    p.many = most_rows > FEW_LIMIT && !(alone && p.large);
+    p.few = !(alone && most_rows > FEW_LIMIT);
+    p.few_limit = most_rows > FEW_LIMIT ? FEW_LIMIT : 0x7fffffff;
+    p.many_limit = p.large ? MANY_LIMIT : 0x7fffffff;
     p.splits = 1;
-    p.few_units = p.many_units = 0;
     // (of the longest sequence: a part more or less because of the others in a call would show in the last bit)
-    const long span = (long)d.window + 63 + (p.many ? FEW_LIMIT : most_new);
-    if (p.few) p.splits = splits_of(true, 1, d.window > 0 && span < len ? (int)span : len, c.kv_heads);
-    if (p.many) {
-        const int tiles = (int)(((long)d.tokens * group + MANY_ROWS - 1) / MANY_ROWS);
-        const int s = splits_of(false, alone ? tiles : 1, len, alone ? c.kv_heads : 1);
+    const long span = (long)d.window + 63 + (most_rows > FEW_LIMIT ? FEW_LIMIT : most_new);
+    if (p.few) p.splits = splits_of(FEW, 1, d.window > 0 && span < len ? (int)span : len, c.kv_heads);
+    if (p.many || p.large) {
+        const int tile = rows_of(p.large ? LARGE : MANY);
+        const int tiles = (int)(((long)d.tokens * group + tile - 1) / tile);
+        const int s = splits_of(MANY, alone ? tiles : 1, len, alone ? c.kv_heads : 1);
         if (s > p.splits) p.splits = s;
     }
-    const long tiles = c.rows < d.tokens ? c.rows : d.tokens;
-    if (p.few) p.few_units = (tiles + (long)d.tokens * group / FEW_ROWS) * p.splits * c.kv_heads;
-    if (p.many) p.many_units = (tiles + (long)d.tokens * group / MANY_ROWS) * (p.splits < 8 ? p.splits : 8) * c.kv_heads;
+    const long rows = (long)d.tokens * group, some = c.rows < d.tokens ? c.rows : d.tokens, parts = (long)(p.splits < 8 ? p.splits : 8) * c.kv_heads;
+    p.few_units = (some + rows / rows_of(FEW)) * p.splits * c.kv_heads;
+    p.many_units = (some + rows / rows_of(MANY)) * parts;
+    p.large_units = (some + rows / rows_of(LARGE)) * parts;
     return p;
 }
 
 unsigned grid_for(long units, long most) { return (unsigned)(units < 1 ? 1 : (units < most ? units : most)); }
 
+template <typename T, int DP, int FORM>
+int run_many(const AttnArgs& a, long units, long most, hipStream_t s) {
+    static_assert(many_lds<DP>() <= 65536, "more LDS has to be asked for");
+    cache_attention_many_kernel<T, DP, FORM><<<grid_for(units, most), 2 * rows_of(FORM), many_lds<DP>(), s>>>(a);
+    DISCO_LAUNCH_CHECK("cache_attention_many_kernel");
+    return DISCO_OK;
+}
+
 template <typename T, int DP>
 int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
-    if (p.many) {
-        constexpr int LDS = many_lds<DP>();
-        static_assert(LDS <= 65536, "more LDS has to be asked for");
-        cache_attention_many_kernel<T, DP><<<grid_for(p.many_units, 512), 256, LDS, s>>>(a);
-        DISCO_LAUNCH_CHECK("cache_attention_many_kernel");
+    if constexpr (DP <= 128) {
+        if (p.large) if (int rc = run_many<T, DP, LARGE>(a, p.large_units, 256, s)) return rc;
     }
+    if (p.many) if (int rc = run_many<T, DP, MANY>(a, p.many_units, 512, s)) return rc;
     if (p.few) {
         cache_attention_few_kernel<T, DP><<<grid_for(p.few_units, DP <= 128 ? 512 : 256), 256, 0, s>>>(a);
         DISCO_LAUNCH_CHECK("cache_attention_few_kernel");
@@ -911,7 +928,7 @@ int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc
     AttnArgs a{(const char*)q, (const char*)c.d_k, (const char*)c.d_v, (char*)out, lse, (float*)ws, (float2*)((char*)ws + (p.splits > 1 ? parts * c.dim * 4 : 0)),
                table, lens, cu_new, d.q_token * 2, d.q_head * 2, d.out_token * 2, d.out_head * 2, c.page_stride * 2, c.head_stride * 2, c.slot_stride * 2,
                d.tokens, d.q_heads, c.kv_heads, d.q_heads / c.kv_heads, c.dim, c.rows, c.table_width, c.pages, __builtin_ctz((unsigned)c.page_size), d.causal,
-               window, p.splits, p.few_limit, fabsf(d.scale) * 1.4426950408889634f, d.scale < 0};
+               window, p.splits, p.few_limit, p.many_limit, fabsf(d.scale) * 1.4426950408889634f, d.scale < 0};
     if (a.c < 1e-37f) a.c = 1e-37f;                                // 0 * -inf is not the score of a key that is not seen
     return c.dtype == DISCO_F16 ? run_dims<f16>(a, p, s) : run_dims<bf16>(a, p, s);
 }
