@@ -174,13 +174,6 @@ __device__ __forceinline__ typename Mat<T>::x8 join(s16x4 a, s16x4 b) {
 __device__ __forceinline__ uint32_t above(uint32_t w, uint32_t most) { return ((w & 0x7fff7fffu) + (0x7fffu - most) * 0x10001u) & 0x80008000u; }
 __device__ __forceinline__ uint32_t word(uint4 w, int i) { return i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w; }
 
-// not 0 where one of the lane's eight values is infinite or NaN
-template <typename T>
-__device__ __forceinline__ uint32_t not_finite(typename Mat<T>::x8 x) {
-    const uint4 w = __builtin_bit_cast(uint4, x);
-    return above(w.x, Mat<T>::INF - 1) | above(w.y, Mat<T>::INF - 1) | above(w.z, Mat<T>::INF - 1) | above(w.w, Mat<T>::INF - 1);
-}
-
 // Values that are not finite, in a tile that not every row sees whole: 0 * inf would give NaN to rows that do not see them.  The finite ones are multiplied;
 // then, for each of NaN, inf and -inf, a product of indicators (which elements of V are it, which keys the row sees) counts what a row sees.
 template <typename T, typename Acc>
@@ -216,6 +209,17 @@ __device__ __forceinline__ Acc multiply_seen(typename Mat<T>::x8 v, typename Mat
     return o;
 }
 
+// whether a row's sums hold a NaN or an infinity: what a value that is not finite makes of a row that does not see it (0 * inf) is always one
+template <typename Acc, int N>
+__device__ __forceinline__ uint32_t not_numbers(const Acc (&o)[N]) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < (int)(sizeof(Acc) / 4); ++r) x = fmaf(o[i][r], 0.f, x);
+    return x != x;
+}
+
 // What a wave keeps of its rows while it walks along the keys (a lane: of its own row): the maximum in use, in log2 units, and the sum over the keys that
 // this lane saw.  The maximum of a tile is not looked for as long as the sum of its probabilities says that the one in use will do: up to
 // LIMIT, which fp16 holds (and leaves the fp32 sums of bf16 values up to 2^100 finite).
@@ -248,7 +252,7 @@ template <typename T, int DP> struct Few {
 };
 
 // One unit.  ODD: the form that keeps values which are not finite, and pages outside the cache, from the rows that do not see them; without it returns whether
-// there were any (then the unit is done again with it).  Both add the same products in the same order.
+// a row has come out not finite, or a page was outside (then the unit is done again with it).  Both add the same products in the same order.
 template <typename T, int DP, bool ODD>
 __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds, float (&part_m)[4][16], float (&part_l)[4][16]) {
     typedef typename Mat<T>::x8 x8;
@@ -388,10 +392,7 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
         for (int i = 0; i < DB; ++i) {
             const x8 v = value(i);
             if (ODD && MASKED) o[i] = multiply_seen<T>(v, p, seen, o[i]);
-            else {
-                if (MASKED) odd |= not_finite<T>(v);
-                o[i] = Mat<T>::mul(v, p, o[i]);
-            }
+            else o[i] = Mat<T>::mul(v, p, o[i]);
         }
         __builtin_amdgcn_wave_barrier();
     };
@@ -409,6 +410,7 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
     }
     run.l += __shfl_xor(run.l, 16);
     run.l += __shfl_xor(run.l, 32);
+    if (!ODD) odd |= not_numbers(o);
     a = fresh(a);
     // the four waves' rows: o to LDS (over the values), then every thread joins four elements of a row at a time
     float* om = (float*)mine;
@@ -625,10 +627,7 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
             const int t = x / (2 * DB), m = x / DB % 2, i = x % DB;
             const x8 v = value(t, m, i);
             if (ODD && MASKED) o[i] = multiply_seen<T>(v, p[t][m], seen[t] >> (8 * m), o[i]);
-            else {
-                if (MASKED) odd |= not_finite<T>(v);
-                o[i] = Mat<T>::mul(v, p[t][m], o[i]);
-            }
+            else o[i] = Mat<T>::mul(v, p[t][m], o[i]);
         }
     };
     int pg = 0, pg_next = 0;
@@ -667,6 +666,7 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
         if (!ODD && part == 0) walk(std::false_type(), whole_to);
     }
     run.l += __shfl_xor(run.l, 32);
+    if (!ODD) odd |= not_numbers(o);
     a = fresh(a);
     if (row < rows) {
         const long t = u.first + token, at_row = t * a->q_heads + head;
