@@ -70,7 +70,7 @@ int disco_op_rotary(const disco_rotary_desc* d, const void* d_x, const void* d_p
     if (d->dtype < DISCO_F16 || d->dtype > DISCO_F32) return bad_value(op, "fp16, bf16 or fp32");
     if (d->tokens < 0) return bad_shape(op, "negative size");
     if (!positive(op, {d->heads, d->dim})) return DISCO_ESHAPE;
-    if (d->heads > 1 << 16 || d->dim > 1 << 16) return bad_shape(op, "more than 65536 heads or elements a head");
+    if (d->heads > 1 << 16 || d->dim > 1024) return bad_shape(op, "more than 65536 heads, or 1024 elements a head");
     if (d->rotated < 2 || d->rotated % 2 || d->rotated > d->dim) return bad_shape(op, "rotated must be even, 2 .. dim");
     if (!within({d->x_token, d->x_head, d->out_token, d->out_head})) return bad_shape(op, "stride too large");
     if (!d->tokens) return DISCO_OK;

@@ -76,12 +76,13 @@ constexpr float LN2 = 0.6931471805599453f;
 struct Cut { int form, tiles, splits, begin, chunk; };
 
 // parts of a sequence's keys; grows with them
-// few rows: a workgroup's waves take 128 keys a round, and up to 512 keys (4 us) one workgroup is done sooner than two and a join; 64 parts of 8 key
-//           heads are two workgroups a CU
+// few rows: a workgroup's waves take 128 keys a round, and up to 512 keys (4 us) one workgroup is done sooner than two and a join.  Beyond, parts of 256 /
+//           384 / 512 keys take 14.4 / 16.0 / 17.7 us for one sequence of 4 096 and 134 / 129 / 125 us for 64 of up to 4 096 (32 heads of 128 on 8 key
+//           heads); 64 parts of 8 key heads are two workgroups a CU
 // many rows: as many parts as make 256 workgroups of the sequence, of at least 1 024 keys (a part costs a write and a read of its rows in fp32: 24 sequences of up to 257 tokens over
 //           4 111 take 78 us, with parts of 512 keys 93)
 __host__ __device__ __forceinline__ int splits_of(int form, int tiles, int keys, int kv_heads) {
-    if (form == FEW) return keys <= 512 ? 1 : (keys > 64 * 256 ? 64 : (keys + 255) / 256);
+    if (form == FEW) return keys <= 512 ? 1 : (keys > 64 * 384 ? 64 : (keys + 383) / 384);
     const int units = tiles * kv_heads;
     int s = units >= 256 ? 1 : 256 / units;
     if (s > 8) s = 8;

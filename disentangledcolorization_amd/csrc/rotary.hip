@@ -4,8 +4,9 @@
 //
 // Memory-bound: every element is read once and written once.  The angle is what needs care: at position 10^6 an fp32 product is off by
 // 0.06 rad, so t / 2 pi is formed in fp64 and only its fraction is kept, as 32 bits of a turn (6e-10 rad); sine and cosine are then Taylor sums
-// over [-pi/4, pi/4] in fp32 (next term below 3e-8).  That is ~45 instructions a pair, so a lane computes its angles once and
-// uses them for several heads of one token; a wave handles one token (or a slice of its heads where tokens are few).
+// over [-pi/4, pi/4] in fp32 (next term below 3e-8).  That is ~50 instructions a pair, six of them in fp64: a wave handles one token (or a slice of
+// its heads where tokens are few), each pair's angle is computed by one lane, and the heads read it from LDS (16 384 tokens of 32 heads of
+// 128, bf16: 45 us, 5.9 TB/s, what copying the tensor takes).
 #include <type_traits>
 #include "paged.h"
 
@@ -42,47 +43,46 @@ __device__ __forceinline__ uint32_t turns(double position, double inv_freq) {
     return (uint32_t)(unsigned long long)((t - floor(t)) * 4294967296.0);     // 2^32 itself wraps to 0
 }
 
-// A unit is what a lane handles of a head: V pairs (two runs of V elements, or 2 V elements where pairs lie side by side), or behind the
-// rotated part 2 V elements that are copied.  V: the widest for which every run is aligned to its size.
+// What a lane handles of a head, in runs of V elements (the widest that dimensions, strides and addresses allow).  A run a lane, so that a wave reads whole
+// lines: with two runs a lane, half a head or half the rotated part apart, 16 384 tokens of 32 heads of 128 take 54 us, and 78 us where half of each
+// head is rotated; with one 45 us, what copying the tensor takes.
+//   WITHIN    pairs side by side: turned inside the run
+//   EXCHANGE  pairs apart: the other ends of the run's pairs come from the lane that holds them
+//   ACROSS    two runs, both ends of V pairs, or two runs of the part that is copied: what neither of the others can do - runs of one element with pairs
+//             side by side, pairs apart in heads of more than 64 runs
+enum Mode { WITHIN, EXCHANGE, ACROSS };
 template <typename T, int V> struct alignas(sizeof(T) * V) Run { T e[V]; };
 
-template <typename T, int V, bool INTER>
-__device__ __forceinline__ void turn_unit(const T* __restrict__ src, T* __restrict__ dst, int unit, int pair_units, int rotated, int dim, const float (&c)[V],
-                                          const float (&s)[V], bool turn) {
-    typedef Run<T, V> R;
-    int lo, hi;
-    if (unit < pair_units) {
-        lo = INTER ? 2 * V * unit : V * unit;
-        hi = INTER ? lo + V : lo + rotated / 2;
-    } else {
-        lo = rotated + 2 * V * (unit - pair_units);
-        hi = lo + V;
-        turn = false;
-    }
-    const bool two = hi < dim;                                     // an odd number of copied runs ends with one alone
-    const R x = *(const R*)(src + lo), y = two ? *(const R*)(src + hi) : x;
-    R u = x, w = y;
-    if (turn) {
-        if (INTER) {
+// one end of V pairs turned: x c + (the other end) s, the sine's sign being the end's
+template <typename T, int V>
+__device__ __forceinline__ Run<T, V> turn_end(const Run<T, V>& x, const Run<T, V>& other, const float (&c)[V], const float (&s)[V]) {
+    Run<T, V> r;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {                          // pair i: elements 2 i and 2 i + 1 of the 2 V
-                const float a = widen(2 * i < V ? x.e[(2 * i) % V] : y.e[(2 * i) % V]), b = widen(2 * i + 1 < V ? x.e[(2 * i + 1) % V] : y.e[(2 * i + 1) % V]);
-                const T p = narrow<T>(a * c[i] - b * s[i]), q = narrow<T>(a * s[i] + b * c[i]);
-                if (2 * i < V) u.e[(2 * i) % V] = p; else w.e[(2 * i) % V] = p;
-                if (2 * i + 1 < V) u.e[(2 * i + 1) % V] = q; else w.e[(2 * i + 1) % V] = q;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float a = widen(x.e[i]), b = widen(y.e[i]);
-                u.e[i] = narrow<T>(a * c[i] - b * s[i]);
-                w.e[i] = narrow<T>(a * s[i] + b * c[i]);
-            }
-        }
-    }
-    *(R*)(dst + lo) = u;
-    if (two) *(R*)(dst + hi) = w;
+    for (int i = 0; i < V; ++i) r.e[i] = narrow<T>(widen(x.e[i]) * c[i] + widen(other.e[i]) * s[i]);
+    return r;
 }
+// the V / 2 pairs inside a run, `pairs` of them turned
+template <typename T, int V>
+__device__ __forceinline__ void turn_within(Run<T, V>& x, int pairs, const float (&c)[V], const float (&s)[V]) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        const float a = widen(x.e[2 * i]), b = widen(x.e[2 * i + 1]);
+        const T p = narrow<T>(a * c[i] - b * s[i]), q = narrow<T>(a * s[i] + b * c[i]);
+        if (i < pairs) { x.e[2 * i] = p; x.e[2 * i + 1] = q; }
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ Run<T, V> run_of_lane(const Run<T, V>& x, int lane) {
+    constexpr int WORDS = (sizeof(T) * V + 3) / 4;
+    union { Run<T, V> r; int w[WORDS]; } a;
+    a.w[WORDS - 1] = 0;
+    a.r = x;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) a.w[i] = __shfl(a.w[i], lane);
+    return a.r;
+}
+
+constexpr int MOST_PAIRS = 512;
 
 struct RotaryArgs {
     const char *x, *k, *v; char *out;
@@ -99,7 +99,7 @@ struct RotaryArgs {
 };
 
 // APPEND: the wave's heads are the queries' (to out), the keys' and the values' (to their page); else the heads of x
-template <typename T, int V, bool INTER, bool APPEND>
+template <typename T, int V, int MODE, bool INTER, bool APPEND>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
     const int wave = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int token = wave / a.slices, slice = wave - token * a.slices;
@@ -118,37 +118,99 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         }
     }
     if (!APPEND || a.positions) position = a.wide ? ((const long long*)a.positions)[token] : ((const int*)a.positions)[token];
-    const int pair_units = a.rotated / (2 * V), units = pair_units + (a.dim - a.rotated + 2 * V - 1) / (2 * V);
+    const int pair_units = a.rotated / (2 * V), rest_units = ((a.dim - a.rotated) / V + 1) / 2;      // (ACROSS)
+    const int units = MODE == ACROSS ? pair_units + rest_units : a.dim / V;
     const int across = units < 64 ? units : 64;                    // lanes that share a head
     const int lane_head = lane / across, step = 64 / across;       // heads that a wave handles at a time
-    if (lane_head >= step) return;
-    const int heads = APPEND ? a.heads + 2 * a.kv_heads : a.heads;
-    for (int unit = lane - lane_head * across; unit < units; unit += across) {
-        float c[V], s[V];
-        if (unit < pair_units) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                turn_sincos(turns((double)position, a.inv_freq[unit * V + i]), c[i], s[i]);
-                c[i] *= a.gain;
-                s[i] *= a.inverse ? -a.gain : a.gain;
+    const int heads = lane_head < step ? (APPEND ? a.heads + 2 * a.kv_heads : a.heads) : 0, stride = a.slices * step;
+    typedef Run<T, V> R;
+    int unit = lane - lane_head * across, lo, hi;
+    auto place = [&] {
+        lo = V * unit;
+        hi = MODE == ACROSS ? lo + a.rotated / 2 : a.dim;          // (no second run)
+        if (MODE == ACROSS) {
+            if (INTER) { lo = 2 * unit; hi = lo + 1; }             // (V = 1)
+            if (unit >= pair_units) {
+                lo = a.rotated + V * (unit - pair_units);
+                hi = lo + V * rest_units;
             }
         }
-        for (int h = slice * step + lane_head; h < heads; h += a.slices * step) {
-            const char* src; char* dst;
-            bool turn = true;
+    };
+    // four heads at a time, all of their loads ahead of the first store - and the first four's ahead of the angles
+    R x[4], y[4];
+    char* dst[4];
+    auto load = [&](int h0) {
+        const bool two = hi < a.dim;                               // an odd number of copied runs ends with one alone
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int h = h0 + j * stride;
+            dst[j] = nullptr;
+            if (h >= heads) continue;
+            const char* src;
             if (!APPEND || h < a.heads) {
                 src = a.x + token * a.x_token + h * a.x_head;
-                dst = a.out + token * a.out_token + h * a.out_head;
+                dst[j] = a.out + token * a.out_token + h * a.out_head;
             } else {
                 if (page_at < 0) continue;
                 const bool key = h < a.heads + a.kv_heads;
                 const int kh = h - a.heads - (key ? 0 : a.kv_heads);
                 src = key ? a.k + token * a.k_token + kh * a.k_head : a.v + token * a.v_token + kh * a.v_head;
-                dst = (key ? a.ck : a.cv) + page_at + kh * a.head_stride;
-                turn = key;
+                dst[j] = (key ? a.ck : a.cv) + page_at + kh * a.head_stride;
             }
-            turn_unit<T, V, INTER>((const T*)src, (T*)dst, unit, pair_units, a.rotated, a.dim, c, s, turn);
+            x[j] = *(const R*)((const T*)src + lo);
+            y[j] = two ? *(const R*)((const T*)src + hi) : x[j];
         }
+    };
+    const int first = slice * step + lane_head;
+    place();
+    load(first);
+    // the angles, each computed once
+    __shared__ __align__(16) float cosines[4][MOST_PAIRS], sines[4][MOST_PAIRS];
+    float *cw = cosines[threadIdx.x >> 6], *sw = sines[threadIdx.x >> 6];
+    for (int p = lane; p < a.rotated / 2; p += 64) {
+        float c, s;
+        turn_sincos(turns((double)position, a.inv_freq[p]), c, s);
+        cw[p] = c * a.gain;
+        sw[p] = s * (a.inverse ? -a.gain : a.gain);
+    }
+    __builtin_amdgcn_wave_barrier();                               // (a wave's LDS operations take place in order)
+    for (;;) {
+        const bool two = hi < a.dim;
+        const bool turn = MODE == ACROSS ? unit < pair_units : lo < a.rotated, second = lo >= a.rotated / 2;
+        float c[V], s[V];                                          // (WITHIN: of V / 2 pairs)
+#pragma unroll
+        for (int i = 0; i < (MODE == WITHIN ? V / 2 : V); ++i) {
+            int p = MODE == WITHIN ? lo / 2 + i : (MODE == EXCHANGE ? lo + i - (second ? a.rotated / 2 : 0) : unit * V + i);
+            if (p >= a.rotated / 2) p = 0;                         // (not used)
+            c[i] = cw[p];
+            s[i] = MODE == EXCHANGE && !second ? -sw[p] : sw[p];
+        }
+        const int other = lane + (second ? -pair_units : pair_units);
+        for (int h0 = first; h0 < heads; h0 += 4 * stride) {
+            if (h0 != first) load(h0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!dst[j]) continue;
+                if (turn && (!APPEND || h0 + j * stride < a.heads + a.kv_heads)) {
+                    if constexpr (MODE == WITHIN) turn_within<T, V>(x[j], a.rotated / 2 - lo / 2, c, s);
+                    else if constexpr (MODE == EXCHANGE) x[j] = turn_end<T, V>(x[j], run_of_lane<T, V>(x[j], other), c, s);
+                    else {
+                        const R u = x[j];
+                        float minus[V];
+#pragma unroll
+                        for (int i = 0; i < V; ++i) minus[i] = -s[i];
+                        x[j] = turn_end<T, V>(u, y[j], c, minus);
+                        y[j] = turn_end<T, V>(y[j], u, c, s);
+                    }
+                }
+                *(R*)((T*)dst[j] + lo) = x[j];
+                if (two) *(R*)((T*)dst[j] + hi) = y[j];
+            }
+        }
+        unit += across;
+        if (unit >= units) break;
+        place();
+        load(first);
     }
 }
 
@@ -159,25 +221,36 @@ int widest(int most, std::initializer_list<unsigned long long> of) {
     return v;
 }
 
-template <bool APPEND>
-int run_rotary(RotaryArgs& a, int dtype, int v, bool inter, hipStream_t s) {
+template <typename T, int V, bool APPEND>
+int run_rotary(RotaryArgs& a, bool inter, hipStream_t s) {
+    const bool exchange = !inter && a.dim / V <= 64 && a.rotated % (2 * V) == 0;
     const int heads = APPEND ? a.heads + 2 * a.kv_heads : a.heads;
-    const int units = a.rotated / (2 * v) + (a.dim - a.rotated + 2 * v - 1) / (2 * v);
+    const int units = (inter && V > 1) || exchange ? a.dim / V : a.rotated / (2 * V) + ((a.dim - a.rotated) / V + 1) / 2;
     const int passes = cdiv(heads, 64 / (units < 64 ? units : 64));        // of a token's heads, for one wave
-    // tokens alone fill the GPU from about 8 waves a SIMD's worth; below that a token's heads are dealt to several waves, which compute
-    // its angles again
+    // tokens alone fill the GPU from about 4 waves a SIMD; below that a token's heads are dealt to several waves, which compute its angles again
     a.slices = 1;
     while (a.slices * 2 <= passes && (long)a.tokens * a.slices < 4096) a.slices *= 2;
     if (a.tokens < 512) a.slices = passes;
-    const long waves = (long)a.tokens * a.slices;
-    const dim3 grid((unsigned)((waves + 3) / 4));
-#define DISCO_ROTARY(T, V) do { if (inter) rotary_kernel<T, V, true, APPEND><<<grid, 256, 0, s>>>(a); else rotary_kernel<T, V, false, APPEND><<<grid, 256, 0, s>>>(a); } while (0)
-#define DISCO_ROTARY_V(T) do { if (v == 8) DISCO_ROTARY(T, 8); else if (v == 4) DISCO_ROTARY(T, 4); else if (v == 2) DISCO_ROTARY(T, 2); else DISCO_ROTARY(T, 1); } while (0)
-    if (dtype == DISCO_F16) DISCO_ROTARY_V(f16);
-    else if (dtype == DISCO_BF16) DISCO_ROTARY_V(__bf16);
-    else if constexpr (!APPEND) { if (v >= 4) DISCO_ROTARY(float, 4); else if (v == 2) DISCO_ROTARY(float, 2); else DISCO_ROTARY(float, 1); }
+    const dim3 grid((unsigned)(((long)a.tokens * a.slices + 3) / 4));
+    if (inter) rotary_kernel<T, V, (V > 1 ? WITHIN : ACROSS), true, APPEND><<<grid, 256, 0, s>>>(a);
+    else if (exchange) rotary_kernel<T, V, EXCHANGE, false, APPEND><<<grid, 256, 0, s>>>(a);
+    else rotary_kernel<T, V, ACROSS, false, APPEND><<<grid, 256, 0, s>>>(a);
     DISCO_LAUNCH_CHECK("rotary_kernel");
     return DISCO_OK;
+}
+
+template <bool APPEND>
+int run_rotary(RotaryArgs& a, int dtype, int v, bool inter, hipStream_t s) {
+#define DISCO_ROTARY(T) (v == 8 ? run_rotary<T, 8, APPEND>(a, inter, s) : v == 4 ? run_rotary<T, 4, APPEND>(a, inter, s) \
+                         : v == 2 ? run_rotary<T, 2, APPEND>(a, inter, s) : run_rotary<T, 1, APPEND>(a, inter, s))
+    if (dtype == DISCO_F16) return DISCO_ROTARY(f16);
+    if (dtype == DISCO_BF16) return DISCO_ROTARY(__bf16);
+#undef DISCO_ROTARY
+    if constexpr (!APPEND) {
+        if (v >= 4) return run_rotary<float, 4, false>(a, inter, s);
+        return v == 2 ? run_rotary<float, 2, false>(a, inter, s) : run_rotary<float, 1, false>(a, inter, s);
+    }
+    return DISCO_EINVAL;
 }
 
 }  // namespace
@@ -188,7 +261,7 @@ int launch_rotary(const disco_rotary_desc& d, const void* x, const void* positio
     a.x = (const char*)x; a.out = (char*)out; a.positions = positions; a.inv_freq = inv_freq;
     a.x_token = d.x_token * size; a.x_head = d.x_head * size; a.out_token = d.out_token * size; a.out_head = d.out_head * size;
     a.gain = (float)d.gain; a.tokens = d.tokens; a.heads = d.heads; a.dim = d.dim; a.rotated = d.rotated; a.inverse = d.inverse; a.wide = d.wide_positions;
-    const int v = widest(16 / size, {(unsigned long long)d.rotated / 2, (unsigned long long)d.dim, (unsigned long long)d.x_token, (unsigned long long)d.x_head,
+    const int v = widest(16 / size, {d.interleaved ? 0ull : (unsigned long long)d.rotated / 2, (unsigned long long)d.dim, (unsigned long long)d.x_token, (unsigned long long)d.x_head,
                                      (unsigned long long)d.out_token, (unsigned long long)d.out_head, (unsigned long long)(uintptr_t)x / size,
                                      (unsigned long long)(uintptr_t)out / size});
     return run_rotary<false>(a, d.dtype, v, d.interleaved, s);
@@ -207,7 +280,7 @@ int launch_cache_append(const disco_cache_desc& c, const disco_append_desc& d, c
     unsigned long long qs = 0;
     if (d.q_heads) qs = (unsigned long long)(d.q_token | d.q_head | d.out_token | d.out_head | (int64_t)((uintptr_t)q / 2) | (int64_t)((uintptr_t)q_out / 2));
     // the cache's strides are multiples of 8 elements and its pointers of 16 bytes
-    const int w = widest(8, {(unsigned long long)d.rotated / 2, qs, (unsigned long long)d.k_token, (unsigned long long)d.k_head, (unsigned long long)d.v_token,
+    const int w = widest(8, {d.interleaved ? 0ull : (unsigned long long)d.rotated / 2, qs, (unsigned long long)d.k_token, (unsigned long long)d.k_head, (unsigned long long)d.v_token,
                              (unsigned long long)d.v_head, (unsigned long long)(uintptr_t)k / 2, (unsigned long long)(uintptr_t)v / 2});
     return run_rotary<true>(a, c.dtype, w, d.interleaved, s);
 }

@@ -453,7 +453,7 @@ int disco_op_rotary_frequencies(int dim, int scaling, double base, double factor
 
 typedef struct disco_rotary_desc {
     int32_t dtype;                             /* DISCO_F16 / DISCO_BF16 / DISCO_F32 */
-    int32_t tokens, heads, dim, rotated;       /* the first `rotated` (even) of a head's dim elements turn, the others are copied */
+    int32_t tokens, heads, dim, rotated;       /* the first `rotated` (even) of a head's dim (at most 1024) elements turn, the others are copied */
     int32_t interleaved;                       /* pairs (2i, 2i + 1); 0: (i, i + rotated / 2) */
     int32_t inverse;                           /* turns back (gain still multiplies): what a gradient takes */
     int32_t wide_positions;                    /* d_positions is int64 (0: int32) */

@@ -288,9 +288,9 @@ def test_a_sequence_does_not_depend_on_its_batch(new):
 
 def test_a_sequence_does_not_depend_on_a_longer_one():
     """Lengths around the most parts that a row's keys are cut into: the longer sequence of a call must not change how the shorter one is cut."""
-    s = Served([16384, 16700, 16000], [1, 1, 40], 1, 1, 64, 64, BF, seed=4)
+    s = Served([16384, 16700, 16000, 24576, 24900], [1, 1, 40, 1, 1], 1, 1, 64, 64, BF, seed=4)
     together = paged.cache_attention(s.q, *s.args())
-    for b in range(3):
+    for b in range(5):
         a, e = int(s.cu[b]), int(s.cu[b + 1])
         for kw in (dict(), dict(max_len=int(s.lens[b])), dict(max_len=int(s.lens[b]), max_new=e - a)):
             alone = paged.cache_attention(s.q[a:e], s.k, s.v, s.table[b:b + 1].contiguous(), s.lens[b:b + 1].contiguous(), ints([0, e - a]), **kw)

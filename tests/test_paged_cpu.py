@@ -119,7 +119,7 @@ def test_missing_arguments_and_workspaces_are_refused(lib):
     assert lib.disco_op_cache_copy_pages(C.byref(c), p, p, -1, None) == -2
 
 
-@pytest.mark.parametrize("kw", [dict(dtype=9), dict(tokens=-1), dict(heads=0), dict(dim=0), dict(rotated=0), dict(rotated=3), dict(rotated=66), dict(x_token=1 << 60)])
+@pytest.mark.parametrize("kw", [dict(dtype=9), dict(tokens=-1), dict(heads=0), dict(dim=0), dict(rotated=0), dict(rotated=3), dict(rotated=66), dict(dim=1026), dict(heads=1 << 17), dict(x_token=1 << 60)])
 def test_bad_rotations_are_refused(lib, kw):
     d = dict(dtype=_ffi.F32, tokens=4, heads=2, dim=64, rotated=64, interleaved=0, inverse=0, wide_positions=0, x_token=128, x_head=64, out_token=128,
              out_head=64, gain=1.0)
