@@ -44,32 +44,45 @@ __device__ __forceinline__ int pages_of(int len, int shift) { return (len + (1 <
 // counts that this workgroup (or an earlier launch) has changed by atomics: read where the atomics were done
 __device__ __forceinline__ int count_now(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// Calls f(page, rank) for the first `most` pages that `is` holds for, in ascending order, over [0, pages); returns how many there are.  Every wave
-// has a run of pages: counts first, then ranks from ballots.
-template <typename Is, typename F>
-__device__ __forceinline__ int for_ranked(int pages, int most, int* part, Is is, F f) {
+// Looks at every page once, in runs of a wave each: calls look(page) -> bool, then - when all threads know how many pages it holds for - then(total), and then
+// rank(page, it held, how many pages below it held).  Four loads of a lane under way at a time; what look said is kept in a register where a run is
+// no longer than 4096 pages.  Returns the total.
+template <typename Look, typename Then, typename Rank>
+__device__ __forceinline__ int scan_pages(int pages, int* part, Look look, Then then, Rank rank) {
     const int w = threadIdx.x >> 6, run = ((pages + WAVES * 64 - 1) / (WAVES * 64)) * 64;
-    const int from = w * run, to = min(pages, from + run);
+    const int from = min(pages, w * run), to = min(pages, from + run), steps = (to - from + 63) / 64;
+    const bool kept = steps <= 64;
+    unsigned long long bits = 0;
     int mine = 0;
-    for (int p = from; p < to; p += 64) {
-        const int page = p + lane_id();
-        mine += __popcll(__ballot(page < to && is(page)));
+    for (int i = 0; i < steps; i += 4) {
+        bool set[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int page = from + (i + j) * 64 + lane_id();
+            set[j] = page < to && look(page);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            mine += __popcll(__ballot(set[j]));
+            if (kept && set[j]) bits |= 1ull << ((i + j) & 63);
+        }
     }
     __syncthreads();
     if (lane_id() == 0) part[w] = mine;
     __syncthreads();
-    int rank = 0, all = 0;
+    int below = 0, all = 0;
 #pragma unroll
     for (int i = 0; i < WAVES; ++i) {
-        if (i < w) rank += part[i];
+        if (i < w) below += part[i];
         all += part[i];
     }
-    for (int p = from; p < to && rank < most; p += 64) {
-        const int page = p + lane_id();
-        const unsigned long long set = __ballot(page < to && is(page));
-        const int r = rank + __popcll(set & lanes_below());
-        if ((set >> lane_id() & 1) && r < most) f(page, r);
-        rank += __popcll(set);
+    then(all);
+    for (int i = 0; i < steps; ++i) {
+        const int page = from + i * 64 + lane_id();
+        const bool set = page < to && (kept ? bits >> i & 1 : look(page));
+        const unsigned long long here = __ballot(set);
+        if (page < to) rank(page, set, below + __popcll(here & lanes_below()));
+        below += __popcll(here);
     }
     return all;
 }
@@ -121,33 +134,25 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
     }
     __syncthreads();
     const int total = base, too_long = over;
-    // free pages: first how many, then - if they suffice - who gets which
-    const int free_pages = for_ranked(a.pages, 0, part, [&](int p) { return a.refs[p] == 0; }, [](int, int) {});
-    const bool done = total <= free_pages && too_long == 0;
-    for_ranked(a.pages, done ? total : 0, part, [&](int p) { return a.refs[p] == 0; }, [&](int page, int rank) {
-        int lo = 0, hi = a.rows - 1;                               // the first row with upto > rank
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (upto[mid] > rank) hi = mid; else lo = mid + 1;
-        }
-        const int have = pages_of(clamp_len(a.lens[lo], capacity), a.shift);
-        a.table_out[(long)lo * a.width + have + rank - (lo ? upto[lo - 1] : 0)] = page;
-        a.refs_out[page] = 1;
-    });
-    // (a page taken is the only one whose count changes; the others are copied by whoever sees them taken or not)
-    int rank = 0;
-    {
-        const int w = threadIdx.x >> 6, run = ((a.pages + WAVES * 64 - 1) / (WAVES * 64)) * 64, from = w * run, to = min(a.pages, from + run);
-#pragma unroll
-        for (int i = 0; i < WAVES; ++i) if (i < w) rank += part[i];
-        for (int p = from; p < to; p += 64) {
-            const int page = p + lane_id(), refs = page < to ? a.refs[page] : 1;
-            const unsigned long long set = __ballot(refs == 0);
-            const bool taken = done && refs == 0 && rank + __popcll(set & lanes_below()) < total;
-            if (page < to && !taken) a.refs_out[page] = refs;
-            rank += __popcll(set);
-        }
-    }
+    bool done = false;
+    const int free_pages = scan_pages(a.pages, part,
+        [&](int p) {
+            const int refs = a.refs[p];
+            a.refs_out[p] = refs;
+            return refs == 0;
+        },
+        [&](int free) { done = total <= free && too_long == 0; },
+        [&](int page, bool free, int rank) {
+            if (!free || !done || rank >= total) return;
+            int lo = 0, hi = a.rows - 1;                           // the first row with upto > rank
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (upto[mid] > rank) hi = mid; else lo = mid + 1;
+            }
+            const int have = pages_of(clamp_len(a.lens[lo], capacity), a.shift);
+            a.table_out[(long)lo * a.width + have + rank - (lo ? upto[lo - 1] : 0)] = page;
+            a.refs_out[page] = 1;
+        });
     for (int r = threadIdx.x; r < a.rows; r += PLAN) {
         const int len = clamp_len(a.lens[r], capacity);
         a.lens_out[r] = done ? len + reserve_new(a, r) : len;
@@ -172,8 +177,8 @@ __global__ void clear_kernel(int* p, int n, int* q, int m) {
     if (i < m) q[i] = 0;
 }
 
-// a copy of pages: src -> dst, the first `filled` slots
-struct Copy { int src, dst, filled; };
+// a copy of pages: src -> dst, the first `filled` slots; `extra`: the plan's own
+struct Copy { int src, dst, filled, extra; };
 
 struct PlanArgs {
     const int *table, *lens, *parents;                             // parents: select only
@@ -190,143 +195,171 @@ __device__ __forceinline__ int parent_of(const PlanArgs& a, int r) {
     return p >= 0 && p < a.rows ? p : -1;
 }
 
-// select: the rows, gathered; counts of the pages that are full (a last page that is not is counted by the plan)
-// compact: counts of all pages
+// How many rows name each page.  LOCAL: in LDS, for tables and pools that one workgroup looks through while two more launches would only start.
+template <bool LOCAL> struct Counts {
+    int* at;
+    __device__ __forceinline__ int get(int p) const { return LOCAL ? at[p] : count_now(at + p); }
+    __device__ __forceinline__ void add(int p) const { atomicAdd(at + p, 1); }
+    __device__ __forceinline__ void set(int p, int n) const {
+        if (LOCAL) at[p] = n;
+        else __hip_atomic_store(at + p, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+};
+// what one thread of the workgroup wrote is there for the others
+__device__ __forceinline__ void settle() {
+    __threadfence();
+    __syncthreads();
+}
+
+// entry `at` of row r, SELECT: of the gathered rows.  Counts pages (select: those that are full; a last page that is not is counted by the plan), and what
+// is out of range
+template <bool SELECT, bool LOCAL>
+__device__ __forceinline__ void count_entry(const PlanArgs& a, Counts<LOCAL> counts, int* bad, int r, int at) {
+    const int from = SELECT ? parent_of(a, r) : r;
+    const int given = from < 0 ? 0 : a.lens[from], len = clamp_len(given, a.width << a.shift);
+    int page = -1;
+    if (at < pages_of(len, a.shift)) {
+        page = a.table[(long)from * a.width + at];
+        if (page < 0 || page >= a.pages) atomicAdd(bad, 1);
+        else if (!SELECT || (at + 1) << a.shift <= len) counts.add(page);
+    }
+    if (SELECT) a.table_out[(long)r * a.width + at] = page;
+    if (at == 0 && given != len) atomicAdd(bad, 1);
+    if (SELECT && at == 0 && from < 0 && a.parents[r] != -1) atomicAdd(bad, 1);       // a parent that is no row
+}
+
 template <bool SELECT>
 __global__ __launch_bounds__(256) void cache_count_kernel(PlanArgs a) {
-    const int capacity = a.width << a.shift;
     const long total = (long)a.rows * a.width, stride = (long)gridDim.x * 256;
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += stride) {
-        const int r = (int)(i / a.width), at = (int)(i - (long)r * a.width);
-        const int from = SELECT ? parent_of(a, r) : r;
-        const int len = from < 0 ? 0 : clamp_len(a.lens[from], capacity);
-        int page = -1;
-        if (at < pages_of(len, a.shift)) {
-            page = a.table[(long)from * a.width + at];
-            if (page < 0 || page >= a.pages) atomicAdd(a.bad, 1);
-            else if (!SELECT || (at + 1) << a.shift <= len) atomicAdd(&a.refs[page], 1);
-        }
-        if (SELECT) a.table_out[i] = page;
-        if (at == 0 && from >= 0 && len != a.lens[from]) atomicAdd(a.bad, 1);
-        if (SELECT && at == 0 && from != a.parents[r]) {           // a parent that is no row (-1 says none)
-            if (a.parents[r] != -1) atomicAdd(a.bad, 1);
-        }
+        const int r = (int)(i / a.width);
+        count_entry<SELECT, false>(a, Counts<false>{a.refs}, a.bad, r, (int)(i - (long)r * a.width));
     }
 }
 
+// the same by the planning workgroup, a wave a row
+template <bool SELECT>
+__device__ __forceinline__ void count_here(const PlanArgs& a, Counts<true> counts, int* bad) {
+    for (int p = threadIdx.x; p < a.pages; p += PLAN) counts.at[p] = 0;
+    __syncthreads();
+    for (int r = threadIdx.x >> 6; r < a.rows; r += WAVES)
+        for (int at = lane_id(); at < a.width; at += 64) count_entry<SELECT, true>(a, counts, bad, r, at);
+    settle();
+}
+
+template <bool LOCAL>
 __global__ __launch_bounds__(PLAN) void cache_select_plan_kernel(PlanArgs a) {
-    extern __shared__ int keeper[];                                // [rows]: which of a parent's rows keeps its last page
-    __shared__ int part[WAVES];
+    extern __shared__ int keeper[];                                // [rows]: which of a parent's rows keeps its last page; LOCAL: [pages] counts
+    __shared__ int part[WAVES], bad;
     const int capacity = a.width << a.shift, tid = threadIdx.x;
+    const Counts<LOCAL> counts{LOCAL ? keeper + a.rows : a.refs_out};
+    if (tid == 0) bad = LOCAL ? 0 : *a.bad;
     for (int r = tid; r < a.rows; r += PLAN) keeper[r] = 1 << 30;
     __syncthreads();
+    if constexpr (LOCAL) count_here<true>(a, counts, &bad);
     for (int r = tid; r < a.rows; r += PLAN) {
         const int p = parent_of(a, r);
         if (p >= 0) atomicMin(&keeper[p], p == r ? -1 : r);
     }
     __syncthreads();
-    // the kept last pages are in use as well
-    auto tail_of = [&](int r, int& len) {                          // the table index of row r's last page if it is not full, else -1
-        const int p = parent_of(a, r);
-        len = p < 0 ? 0 : clamp_len(a.lens[p], capacity);
-        return len & ((1 << a.shift) - 1) ? (long)r * a.width + (len >> a.shift) : -1l;
-    };
-    auto keeps = [&](int r) { const int p = parent_of(a, r); return keeper[p] == (p == r ? -1 : r); };
-    for (int r = tid; r < a.rows; r += PLAN) {
-        int len;
-        const long t = tail_of(r, len);
-        if (t >= 0 && keeps(r)) {
-            const int page = a.table_out[t];
-            if (page >= 0 && page < a.pages) atomicAdd(&a.refs_out[page], 1);
-        }
-    }
-    __threadfence();
-    __syncthreads();
-    const int free_pages = for_ranked(a.pages, 0, part, [&](int p) { return count_now(&a.refs_out[p]) == 0; }, [](int, int) {});
-    // the rows that need a copy, ascending; their number first
-    int need_total = 0;
+    // last pages that are not full: the keeper's is in use, the others need copies, numbered by row
+    int need = 0;
     for (int r0 = 0; r0 < a.rows; r0 += PLAN) {
-        const int r = r0 + tid;
-        int len, all;
-        const bool need = r < a.rows && tail_of(r, len) >= 0 && !keeps(r);
-        const int rank = need_total + block_scan(need, part, &all) - 1;
-        if (need) {
-            a.copies[rank].src = r;                                // (the row for now)
-            a.copies[rank].filled = len & ((1 << a.shift) - 1);
+        const int r = r0 + tid, p = r < a.rows ? parent_of(a, r) : -1;
+        const int len = p < 0 ? 0 : clamp_len(a.lens[p], capacity), filled = len & ((1 << a.shift) - 1);
+        const bool keeps = p >= 0 && keeper[p] == (p == r ? -1 : r);
+        int page = -1, all;
+        if (filled) {
+            page = a.table_out[(long)r * a.width + (len >> a.shift)];
+            if (keeps && page >= 0 && page < a.pages) counts.add(page);
         }
-        need_total += all;
+        const bool asks = filled && !keeps;
+        const int rank = need + block_scan(asks, part, &all) - 1;
+        if (asks) a.copies[rank] = Copy{page, -1, filled, r};      // (a page outside the cache is left out by the copy)
+        if (r < a.rows) a.lens_out[r] = len;
+        need += all;
     }
-    __threadfence();
-    __syncthreads();
-    const bool done = need_total <= free_pages;
-    if (done) {
-        for_ranked(a.pages, need_total, part, [&](int p) { return count_now(&a.refs_out[p]) == 0; }, [&](int page, int rank) {
-            a.copies[rank].dst = page;
+    settle();
+    bool done = false;
+    int free_pages = scan_pages(a.pages, part, [&](int p) { return counts.get(p) == 0; }, [&](int free) { done = need <= free; },
+        [&](int page, bool free, int rank) {
+            if (!free || !done || rank >= need) return;
+            Copy* c = a.copies + rank;
+            const int r = __hip_atomic_load(&c->extra, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            c->dst = page;
+            a.table_out[(long)r * a.width + (clamp_len(a.lens[parent_of(a, r)], capacity) >> a.shift)] = page;
+            counts.set(page, 1);
         });
-        __threadfence();
+    if (!done) {                                                   // too few free pages: the old state once more
+        const int missing = need - free_pages;
         __syncthreads();
-        for (int i = tid; i < need_total; i += PLAN) {
-            const int r = __hip_atomic_load(&a.copies[i].src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const int page = __hip_atomic_load(&a.copies[i].dst, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            int len;
-            const long t = tail_of(r, len);
-            a.copies[i].src = a.table_out[t];                      // (one outside the cache is left out by the copy)
-            a.table_out[t] = page;
-            a.refs_out[page] = 1;
+        for (int p = tid; p < a.pages; p += PLAN) counts.set(p, 0);
+        settle();
+        for (int r = tid >> 6; r < a.rows; r += WAVES) {
+            const int len = clamp_len(a.lens[r], capacity);
+            for (int at = lane_id(); at < a.width; at += 64) {
+                const int page = at < pages_of(len, a.shift) ? a.table[(long)r * a.width + at] : -1;
+                a.table_out[(long)r * a.width + at] = page;
+                if (page >= 0 && page < a.pages) counts.add(page);
+            }
+            if (lane_id() == 0) a.lens_out[r] = len;
         }
-        for (int r = tid; r < a.rows; r += PLAN) {
-            const int p = parent_of(a, r);
-            a.lens_out[r] = p < 0 ? 0 : clamp_len(a.lens[p], capacity);
-        }
-    } else {                                                       // too few free pages: the old state once more
-        for (int p = tid; p < a.pages; p += PLAN) a.refs_out[p] = 0;
-        __threadfence();
-        __syncthreads();
-        for (long i = tid; i < (long)a.rows * a.width; i += PLAN) {
-            const int r = (int)(i / a.width), at = (int)(i - (long)r * a.width);
-            const int page = at < pages_of(clamp_len(a.lens[r], capacity), a.shift) ? a.table[i] : -1;
-            a.table_out[i] = page;
-            if (page >= 0 && page < a.pages) atomicAdd(&a.refs_out[page], 1);
-        }
-        for (int r = tid; r < a.rows; r += PLAN) a.lens_out[r] = clamp_len(a.lens[r], capacity);
-        __threadfence();
-        __syncthreads();
+        settle();
+        free_pages = scan_pages(a.pages, part, [&](int p) { return counts.get(p) == 0; }, [](int) {}, [](int, bool, int) {});
+        if (tid == 0) a.info[1] = missing;
     }
-    int left = 0;
-    if (!done) left = for_ranked(a.pages, 0, part, [&](int p) { return count_now(&a.refs_out[p]) == 0; }, [](int, int) {});
+    if (LOCAL) {
+        __syncthreads();
+        for (int p = tid; p < a.pages; p += PLAN) a.refs_out[p] = counts.get(p);
+    }
     if (tid == 0) {
-        *a.copy_count = done ? need_total : 0;
-        a.info[0] = done ? free_pages - need_total : left;
-        a.info[1] = done ? 0 : need_total - free_pages;
-        a.info[2] = *a.bad;
-        a.info[3] = done ? need_total : 0;
+        *a.copy_count = done ? need : 0;
+        a.info[0] = done ? free_pages - need : free_pages;
+        if (done) a.info[1] = 0;
+        a.info[2] = bad;
+        a.info[3] = done ? need : 0;
     }
 }
 
+template <bool LOCAL>
 __global__ __launch_bounds__(PLAN) void cache_compact_plan_kernel(PlanArgs a) {
-    __shared__ int part[WAVES];
+    extern __shared__ int counted[];                               // LOCAL: [pages] counts
+    __shared__ int part[WAVES], bad, kept;
     const int tid = threadIdx.x, pages = a.pages;
-    const int live = for_ranked(pages, 0, part, [&](int p) { return a.refs[p] > 0; }, [](int, int) {});
-    const int moved = for_ranked(live, live, part, [&](int p) { return a.refs[p] == 0; }, [&](int page, int rank) {
-        a.copies[rank].dst = page;
-        a.copies[rank].filled = 1 << a.shift;
-    });
-    for_ranked(pages, pages, part, [&](int p) { return p >= live && a.refs[p] > 0; }, [&](int page, int rank) { a.copies[rank].src = page; });
-    for (int p = tid; p < pages; p += PLAN) if (p >= live || a.refs[p] > 0) a.refs_out[p] = p < live ? a.refs[p] : 0;
-    for (int p = tid; p < live; p += PLAN) a.map[p] = p;
-    __threadfence();
+    const Counts<LOCAL> counts{LOCAL ? counted : a.refs};
+    if (tid == 0) bad = LOCAL ? 0 : *a.bad;
     __syncthreads();
+    if constexpr (LOCAL) count_here<false>(a, counts, &bad);
+    // of the `live` pages in use, those from `live` on move into the holes below it: `kept` pages in use lie below
+    int live = 0;
+    scan_pages(pages, part, [&](int p) { return counts.get(p) > 0; },
+        [&](int total) {
+            live = total;
+            if (tid == 0) kept = total;                            // (when no page lies at or above it)
+            __syncthreads();
+        },
+        [&](int page, bool used, int below) {
+            if (page == live) kept = below;
+            if (page < live) a.map[page] = page;
+            if (used && page >= live) a.copies[below].extra = page;
+            if (!used && page < live) a.copies[page - below].dst = page;
+            if (used || page >= live) a.refs_out[page] = page < live ? counts.get(page) : 0;
+        });
+    settle();
+    const int moved = live - kept;
     for (int i = tid; i < moved; i += PLAN) {
-        const int src = __hip_atomic_load(&a.copies[i].src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const int src = __hip_atomic_load(&a.copies[kept + i].extra, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const int dst = __hip_atomic_load(&a.copies[i].dst, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        a.copies[i].src = src;
+        a.copies[i].filled = 1 << a.shift;
         a.map[src] = dst;
-        a.refs_out[dst] = a.refs[src];
+        a.refs_out[dst] = counts.get(src);
     }
     if (tid == 0) {
         *a.copy_count = moved;
         a.info[0] = pages - live;
         a.info[1] = 0;
-        a.info[2] = *a.bad;
+        a.info[2] = bad;
         a.info[3] = moved;
     }
 }
@@ -401,6 +434,9 @@ int allow_lds(K kernel, size_t bytes) {
     return DISCO_OK;
 }
 
+// Tables of up to 64 K entries over up to 32 K pages (and 4 K rows: 144 KB of LDS): one workgroup counts while it plans
+bool local(const disco_cache_desc& c) { return (long)c.rows * c.table_width <= 65536 && c.pages <= 32768 && c.rows <= 4096; }
+
 struct Scratch { Copy* copies; int *count, *bad, *map, *refs; };
 
 Scratch scratch(void* ws, int pages) {
@@ -409,7 +445,7 @@ Scratch scratch(void* ws, int pages) {
     s.bad = p; s.count = p + 1;
     s.refs = p + 4;
     s.map = s.refs + pages;
-    s.copies = (Copy*)(s.map + pages);
+    s.copies = (Copy*)((char*)s.refs + (8 * (size_t)pages + 15) / 16 * 16);
     return s;
 }
 
@@ -417,7 +453,7 @@ Scratch scratch(void* ws, int pages) {
 
 size_t cache_pages_ws_bytes(int rows, int pages) {
     const size_t copies = (size_t)(rows > pages ? rows : pages);
-    return 16 + 8 * (size_t)pages + sizeof(Copy) * copies;
+    return 16 + (8 * (size_t)pages + 15) / 16 * 16 + sizeof(Copy) * copies;
 }
 
 int launch_cache_reserve(int rows, int width, int pages, int page_shift, const int* table, const int* lens, const int* refs, const int* cu_new,
@@ -435,11 +471,16 @@ int launch_cache_select(const disco_cache_desc& c, const int* table, const int* 
     const Scratch w = scratch(ws, c.pages);
     PlanArgs a{table, lens, parents, table_out, lens_out, refs_out, refs_out, info, w.copies, w.count, w.map, w.bad, c.rows, c.table_width, c.pages,
                __builtin_ctz((unsigned)c.page_size)};
-    const size_t lds = (size_t)c.rows * 4;
-    if (lds > 32768) if (int rc = allow_lds(cache_select_plan_kernel, lds)) return rc;
-    clear_kernel<<<blocks_for(c.pages, 256, 256), 256, 0, s>>>(refs_out, c.pages, w.bad, 2);
-    cache_count_kernel<true><<<blocks_for((long)c.rows * c.table_width, 256, 1024), 256, 0, s>>>(a);
-    cache_select_plan_kernel<<<1, PLAN, lds, s>>>(a);
+    const size_t lds = ((size_t)c.rows + (local(c) ? c.pages : 0)) * 4;
+    if (local(c)) {
+        if (lds > 32768) if (int rc = allow_lds(cache_select_plan_kernel<true>, lds)) return rc;
+        cache_select_plan_kernel<true><<<1, PLAN, lds, s>>>(a);
+    } else {
+        if (lds > 32768) if (int rc = allow_lds(cache_select_plan_kernel<false>, lds)) return rc;
+        clear_kernel<<<blocks_for(c.pages, 256, 256), 256, 0, s>>>(refs_out, c.pages, w.bad, 2);
+        cache_count_kernel<true><<<blocks_for((long)c.rows * c.table_width, 256, 1024), 256, 0, s>>>(a);
+        cache_select_plan_kernel<false><<<1, PLAN, lds, s>>>(a);
+    }
     DISCO_LAUNCH_CHECK("cache_select_plan_kernel");
     CopyArgs p{};
     p.copies = w.copies; p.count = w.count;
@@ -451,9 +492,15 @@ int launch_cache_compact(const disco_cache_desc& c, const int* table, const int*
     const Scratch w = scratch(ws, c.pages);
     PlanArgs a{table, lens, nullptr, table_out, nullptr, w.refs, refs_out, info, w.copies, w.count, w.map, w.bad, c.rows, c.table_width, c.pages,
                __builtin_ctz((unsigned)c.page_size)};
-    clear_kernel<<<blocks_for(c.pages, 256, 256), 256, 0, s>>>(w.refs, c.pages, w.bad, 2);
-    cache_count_kernel<false><<<blocks_for((long)c.rows * c.table_width, 256, 1024), 256, 0, s>>>(a);
-    cache_compact_plan_kernel<<<1, PLAN, 0, s>>>(a);
+    if (local(c)) {
+        const size_t lds = (size_t)c.pages * 4;
+        if (lds > 32768) if (int rc = allow_lds(cache_compact_plan_kernel<true>, lds)) return rc;
+        cache_compact_plan_kernel<true><<<1, PLAN, lds, s>>>(a);
+    } else {
+        clear_kernel<<<blocks_for(c.pages, 256, 256), 256, 0, s>>>(w.refs, c.pages, w.bad, 2);
+        cache_count_kernel<false><<<blocks_for((long)c.rows * c.table_width, 256, 1024), 256, 0, s>>>(a);
+        cache_compact_plan_kernel<false><<<1, PLAN, 0, s>>>(a);
+    }
     DISCO_LAUNCH_CHECK("cache_compact_plan_kernel");
     CopyArgs p{};
     p.copies = w.copies; p.count = w.count;

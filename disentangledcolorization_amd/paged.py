@@ -219,8 +219,8 @@ def _state(page_table, rows, width, pages):
     table = rows * width
     flat = page_table.new_empty(table + rows + pages + 4)
     at = flat.data_ptr()
-    return ((flat[:table].view(rows, width), flat[table:table + rows], flat[table + rows:-4], flat[-4:]),
-            (at, at + 4 * table, at + 4 * (table + rows), at + 4 * (table + rows + pages)))
+    new, lens, refs, info = flat.split_with_sizes((table, rows, pages, 4))
+    return ((new.view(rows, width), lens, refs, info), (at, at + 4 * table, at + 4 * (table + rows), at + 4 * (table + rows + pages)))
 
 
 def cache_reserve(page_table, lens, refs, cu_new, page):

@@ -516,8 +516,8 @@ def fork_state(rows, page, seed, full=False):
     return lens, table, count
 
 
-@pytest.mark.parametrize("rows,page,layers,kv_heads,dim", [(1, 16, 1, 1, 8), (6, 8, 3, 2, 64), (40, 16, 2, 1, 80), (1200, 4, 1, 1, 16)])
-@pytest.mark.parametrize("spare", [0, 3, 2000])
+@pytest.mark.parametrize("rows,page,layers,kv_heads,dim,spare", [(*a, b) for a in [(1, 16, 1, 1, 8), (6, 8, 3, 2, 64), (40, 16, 2, 1, 80), (1200, 4, 1, 1, 16)] for b in (0, 3, 2000)]
+                         + [(5000, 2, 1, 1, 8, 0), (5000, 2, 1, 1, 8, 9000), (30, 16, 1, 1, 8, 70000)])      # (pools and tables beyond what one workgroup counts)
 def test_select(rows, page, layers, kv_heads, dim, spare):
     g = gen(rows + spare)
     lens, table, count = fork_state(rows, page, rows)
@@ -554,7 +554,7 @@ def test_select_counts_what_is_out_of_range():
     assert got[1].tolist() == [32, 0, 0] and got[0].tolist() == [[0, 3], [-1, -1], [-1, -1]] and got[3].tolist() == [2, 0, 1, 0]
 
 
-@pytest.mark.parametrize("rows,page,layers,kv_heads,dim,spare", [(1, 16, 1, 1, 8, 0), (6, 8, 3, 2, 64, 30), (40, 16, 2, 1, 80, 200), (1, 1, 1, 1, 16, 5000), (300, 4, 1, 1, 16, 9000)])
+@pytest.mark.parametrize("rows,page,layers,kv_heads,dim,spare", [(1, 16, 1, 1, 8, 0), (6, 8, 3, 2, 64, 30), (40, 16, 2, 1, 80, 200), (1, 1, 1, 1, 16, 5000), (300, 4, 1, 1, 16, 9000), (5000, 2, 1, 1, 8, 100), (20, 4, 1, 1, 8, 70000)])
 @pytest.mark.parametrize("slot_major", [False, True])
 def test_compact(rows, page, layers, kv_heads, dim, spare, slot_major):
     g = gen(rows + spare)
