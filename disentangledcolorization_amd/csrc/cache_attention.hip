@@ -177,8 +177,9 @@ __device__ __forceinline__ uint32_t word(uint4 w, int i) { return i == 0 ? w.x :
 
 // Values that are not finite, in a tile that not every row sees whole: 0 * inf would give NaN to rows that do not see them.  The finite ones are multiplied;
 // then, for each of NaN, inf and -inf, a product of indicators (which elements of V are it, which keys the row sees) counts what a row sees.
-template <typename T, typename Acc>
-__device__ __forceinline__ Acc multiply_seen(typename Mat<T>::x8 v, typename Mat<T>::x8 p, uint32_t seen, Acc o) {
+// (rest: what the rounding of p has left, where the form multiplies that as well)
+template <typename T, bool REST, typename Acc>
+__device__ __forceinline__ Acc multiply_seen(typename Mat<T>::x8 v, typename Mat<T>::x8 p, typename Mat<T>::x8 rest, uint32_t seen, Acc o) {
     typedef typename Mat<T>::x8 x8;
     const uint4 w = __builtin_bit_cast(uint4, v);
     uint32_t clean[4], rows[4];
@@ -188,7 +189,9 @@ __device__ __forceinline__ Acc multiply_seen(typename Mat<T>::x8 v, typename Mat
         clean[i] = y & ~((above(y, Mat<T>::INF - 1) >> 15) * 0xffffu);
         rows[i] = ((seen >> (2 * i) & 1) | (seen >> (2 * i + 1) & 1) << 16) * Mat<T>::ONE;
     }
-    o = Mat<T>::mul(__builtin_bit_cast(x8, uint4{clean[0], clean[1], clean[2], clean[3]}), p, o);
+    const x8 finite = __builtin_bit_cast(x8, uint4{clean[0], clean[1], clean[2], clean[3]});
+    o = Mat<T>::mul(finite, p, o);
+    if (REST) o = Mat<T>::mul(finite, rest, o);
     const x8 who = __builtin_bit_cast(x8, uint4{rows[0], rows[1], rows[2], rows[3]});
 #pragma unroll 1
     for (int kind = 0; kind < 3; ++kind) {
@@ -349,7 +352,7 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
                     s[t][r] = !sees ? -INFINITY : (ODD && (bad >> in_tile & 1) ? __builtin_nanf("") : s[t][r]);
                 }
         }
-        x8 p;
+        x8 p, rest;                                                // (reading the cache bounds this form: the second product of the probabilities' rounding is free)
         float sum;
         auto weights = [&] {
             const float base = run.base<T>();
@@ -359,6 +362,7 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
                 const float e = exp2_of(fmaf(s[i / 4][i % 4], a->c, -base));
                 sum += e;
                 p[i] = (T)e;
+                rest[i] = (T)(e - (float)p[i]);
             }
         };
         weights();
@@ -392,8 +396,8 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
 #pragma unroll
         for (int i = 0; i < DB; ++i) {
             const x8 v = value(i);
-            if (ODD && MASKED) o[i] = multiply_seen<T>(v, p, seen, o[i]);
-            else o[i] = Mat<T>::mul(v, p, o[i]);
+            if (ODD && MASKED) o[i] = multiply_seen<T, true>(v, p, rest, seen, o[i]);
+            else o[i] = Mat<T>::mul(v, rest, Mat<T>::mul(v, p, o[i]));
         }
         __builtin_amdgcn_wave_barrier();
     };
@@ -627,7 +631,7 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
         for (int x = 0; x < SUB * 2 * DB; ++x) {
             const int t = x / (2 * DB), m = x / DB % 2, i = x % DB;
             const x8 v = value(t, m, i);
-            if (ODD && MASKED) o[i] = multiply_seen<T>(v, p[t][m], seen[t] >> (8 * m), o[i]);
+            if (ODD && MASKED) o[i] = multiply_seen<T, false>(v, p[t][m], p[t][m], seen[t] >> (8 * m), o[i]);
             else o[i] = Mat<T>::mul(v, p[t][m], o[i]);
         }
     };
