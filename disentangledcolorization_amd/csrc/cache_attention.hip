@@ -81,12 +81,12 @@ struct Cut { int form, tiles, splits, begin, chunk; };
 //           heads); 64 parts of 8 key heads are two workgroups a CU
 // many rows: as many parts as make 256 workgroups of the sequence, of at least 1 024 keys (a part costs a write and a read of its rows in fp32: 24 sequences of up to 257 tokens over
 //           4 111 take 78 us, with parts of 512 keys 93)
-__host__ __device__ __forceinline__ int splits_of(int form, int tiles, int keys, int kv_heads) {
+__host__ __device__ __forceinline__ int splits_of(int form, int rows, int tiles, int keys, int kv_heads) {
     if (form == FEW) return keys <= 512 ? 1 : (keys > 64 * 384 ? 64 : (keys + 383) / 384);
     const int units = tiles * kv_heads;
     int s = units >= 256 ? 1 : 256 / units;
     if (s > 8) s = 8;
-    const int by_keys = keys <= 1024 ? 1 : (keys + 1023) / 1024;
+    const int least = rows <= 64 ? 512 : 1024, by_keys = keys <= least ? 1 : (keys + least - 1) / least;
     return s < by_keys ? s : by_keys;
 }
 
@@ -98,7 +98,7 @@ __host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv
     u.begin = window > 0 && len - n - window + 1 > 0 ? (len - n - window + 1) & ~63 : 0;
     const int keys = len - u.begin, tile = rows_of(u.form);
     u.tiles = (rows + tile - 1) / tile;
-    int s = splits_of(u.form, u.tiles, keys, kv_heads);
+    int s = splits_of(u.form, rows, u.tiles, keys, kv_heads);
     if (s > most) s = most;
     u.chunk = ((keys + s - 1) / s + 127) & ~127;
     if (u.chunk < 128) u.chunk = 128;
@@ -249,6 +249,9 @@ template <typename T> struct Quad { T e[4]; };
 // A wave takes every fourth 32-key tile of the workgroup's range.  Keys go from memory straight into the operand (lane: key lane % 16, 8 elements at
 // 32 ks + 8 (lane / 16)); values go through registers into the wave's own piece of LDS, from where they are read transposed.  The next tile's
 // loads are in flight under the current tile.  No barrier but for the join of the four waves at the end.
+// waves of a SIMD: what the registers of the loop allow (a third one at 128 elements would spill, and take twice the time)
+constexpr int few_waves(int dp) { return dp <= 32 ? 4 : dp <= 64 ? 3 : dp <= 128 ? 2 : 1; }
+
 template <typename T, int DP> struct Few {
     static constexpr int VROW = DP * 2 + 32;                       // (rows 32 bytes apart in bank phase)
     static constexpr int OROW = DP + 4;                            // floats of a row that is joined
@@ -339,6 +342,8 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
             for (int ks = 0; ks < KS; ++ks) s[t] = Mat<T>::mul(__builtin_bit_cast(x8, kf[t][ks]), q[ks], s[t]);
         }
         const bool more = k0 + 128 < end;
+        // (loads are waited for in order: the pages of the tile after the next go ahead of the next one's keys and values)
+        const int pg_after = pages_at(k0 + 256);
         if (more) fetch_k(k0 + 128, pg_next);
         uint32_t seen = 0;                                         // of this lane's eight keys
         if (MASKED) {
@@ -387,11 +392,9 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
             const int piece = i * 64 + lane, r = piece / (DP / 8), byte = (piece - r * (DP / 8)) * 16;
             *(uint4*)(mine + r * VROW + byte) = vf[i];
         }
-        if (more) {
-            fetch_v(k0 + 128, pg_next);
-            pg = pg_next;
-            pg_next = pages_at(k0 + 256);
-        }
+        if (more) fetch_v(k0 + 128, pg_next);
+        pg = pg_next;
+        pg_next = pg_after;
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int i = 0; i < DB; ++i) {
@@ -475,7 +478,7 @@ __device__ __noinline__ void few_unit_odd(uint64_t args, int want, uint32_t lds,
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void cache_attention_few_kernel(AttnArgs) {
+__global__ __launch_bounds__(256, few_waves(DP)) void cache_attention_few_kernel(AttnArgs) {
     const ArgsAt a = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
     __shared__ __align__(16) char lds[4 * Few<T, DP>::WAVE];
     __shared__ float part_m[4][16], part_l[4][16];
@@ -834,7 +837,7 @@ __global__ __launch_bounds__(256) void cache_attention_join_row_kernel(AttnArgs 
 }
 
 // ---- what the host decides ----------------------------------------------------------------------------------------------------------------------
-constexpr int FEW_LIMIT = 32, MANY_LIMIT = 1024;
+constexpr int FEW_LIMIT = 16, MANY_LIMIT = 1024;
 
 struct Plan {
     bool few, many, large;             // which forms are launched
@@ -860,11 +863,11 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     p.splits = 1;
     // (of the longest sequence: a part more or less because of the others in a call would show in the last bit)
     const long span = (long)d.window + 63 + (most_rows > FEW_LIMIT ? FEW_LIMIT : most_new);
-    if (p.few) p.splits = splits_of(FEW, 1, d.window > 0 && span < len ? (int)span : len, c.kv_heads);
+    if (p.few) p.splits = splits_of(FEW, 1, 1, d.window > 0 && span < len ? (int)span : len, c.kv_heads);
     if (p.many || p.large) {
         const int tile = rows_of(p.large ? LARGE : MANY);
         const int tiles = (int)(((long)d.tokens * group + tile - 1) / tile);
-        const int s = splits_of(MANY, alone ? tiles : 1, len, alone ? c.kv_heads : 1);
+        const int s = splits_of(MANY, alone ? (int)most_rows : 1, alone ? tiles : 1, len, alone ? c.kv_heads : 1);
         if (s > p.splits) p.splits = s;
     }
     const long rows = (long)d.tokens * group, some = c.rows < d.tokens ? c.rows : d.tokens, parts = (long)(p.splits < 8 ? p.splits : 8) * c.kv_heads;
@@ -891,7 +894,7 @@ int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
     }
     if (p.many) if (int rc = run_many<T, DP, MANY>(a, p.many_units, 512, s)) return rc;
     if (p.few) {
-        cache_attention_few_kernel<T, DP><<<grid_for(p.few_units, DP <= 128 ? 512 : 256), 256, 0, s>>>(a);
+        cache_attention_few_kernel<T, DP><<<grid_for(p.few_units, 256 * few_waves(DP)), 256, 0, s>>>(a);
         DISCO_LAUNCH_CHECK("cache_attention_few_kernel");
     }
     if (p.splits > 1) {
