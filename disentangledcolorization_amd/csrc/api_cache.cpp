@@ -20,6 +20,7 @@ int check_pages(const char* op, int rows, int width, int pages, int page_size) {
     if (page_size & (page_size - 1)) return bad_shape(op, "page_size must be a power of two");
     if ((int64_t)width * page_size > (1 << 30)) return bad_shape(op, "table_width * page_size beyond 2^30 tokens");
     if (rows > 16384) return bad_shape(op, "more than 16384 rows");
+    if ((int64_t)rows * width > 0x7fffffff) return bad_shape(op, "a page table of more than 2^31 entries");
     return DISCO_OK;
 }
 

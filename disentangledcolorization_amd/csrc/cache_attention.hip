@@ -9,7 +9,7 @@
 // is the accumulator's; V^T is read in the same order by the transposing LDS read).
 //
 // Three forms, chosen by a sequence's own rows (new tokens * group), so that its result does not depend on what else is in the call:
-//   few (up to 32 rows)    cache_attention_few_kernel: 16 rows a workgroup, its four waves deal 32-key tiles; bound by reading the cache
+//   few (up to 16 rows)    cache_attention_few_kernel: 16 rows a workgroup, its four waves deal 32-key tiles; bound by reading the cache
 //   many (up to 1 024)     cache_attention_many_kernel, 128 rows a workgroup, 32 a wave, keys and values staged in LDS for all of them; two workgroups
 //                          a CU, bound by what L2 delivers into LDS (7 TB/s over the chip) and, at short ranges, by latency
 //   large                  the same with 256 rows, which halves what is delivered; bound by the matrix cores and the exponentials, which overlap in part
@@ -49,11 +49,14 @@ template <> struct Mat<bf16> {
 
 struct AttnArgs {
     const char *q, *k, *v; char* out; float* lse;
-    float *part_o; float2* part_ml;                                // of a row (token * q_heads + head) and a split
+    float *part_o; float2* part_ml;                                // by part_at()
     const int *table, *lens, *cu_new;
     long q_token, q_head, out_token, out_head, page_stride, head_stride, slot_stride;    // bytes
     int tokens, q_heads, kv_heads, group, dim, rows, width, pages, page_shift, causal, window;
-    int splits;                                                    // parts of a row that the workspace has room for
+    // parts of a row that the workspace has room for, and where they are: by token, or by sequence
+    int few_splits, many_splits, few_by_sequence;
+    int many_room;                                                 // of a sequence; 0: by token
+    long many_from;
     int few, many;                                                 // sequences of at most so many rows take the form of few, of many rows
     float c;                                                       // |scale| log2 e, not 0
     int negate;                                                    // scale < 0: the queries change sign instead
@@ -91,7 +94,7 @@ __host__ __device__ __forceinline__ int splits_of(int form, int rows, int tiles,
 }
 
 // keys that some new token of the sequence sees: begin (a multiple of 64) .. len; every part takes `chunk` of them, a multiple of 128
-__host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv_heads, int window, int few, int many, int most) {
+__host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv_heads, int window, int few, int many, int most_few, int most_many) {
     Cut u;
     const int rows = n * group;
     u.form = rows <= few ? FEW : (rows <= many ? MANY : LARGE);
@@ -99,12 +102,21 @@ __host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv
     const int keys = len - u.begin, tile = rows_of(u.form);
     u.tiles = (rows + tile - 1) / tile;
     int s = splits_of(u.form, rows, u.tiles, keys, kv_heads);
+    const int most = u.form == FEW ? most_few : most_many;
     if (s > most) s = most;
     u.chunk = ((keys + s - 1) / s + 127) & ~127;
     if (u.chunk < 128) u.chunk = 128;
     u.splits = (keys + u.chunk - 1) / u.chunk;
     if (u.splits < 1) u.splits = 1;
     return u;
+}
+
+// where part 0 of a row lies: row `row` of the sequence's rows of key head `kv_head`, token t of the call, query head h
+template <typename Args>
+__device__ __forceinline__ long part_at(const Args& a, int form, int splits, int b, int row, int kv_head, int t, int h) {
+    const long by_token = (long)t * a.q_heads + h;
+    if (form == FEW) return (a.few_by_sequence ? ((long)b * a.kv_heads + kv_head) * rows_of(FEW) + row : by_token) * a.few_splits;
+    return a.many_from + (a.many_room ? (long)b * a.many_room + ((long)row * a.kv_heads + kv_head) * splits : by_token * a.many_splits);
 }
 
 struct Unit { int b, n, len, first, tile, split, head; Cut cut; };
@@ -125,7 +137,7 @@ __device__ __forceinline__ bool find_unit(ArgsAt a, int want, Unit& u) {
             len = clamp_len(a->lens[b], capacity);
             if (first < 0 || n < 0 || n > a->tokens || first > a->tokens - n) n = 0;       // (not offsets)
             if (n > 0) {
-                cut = cut_of(n, len, a->group, a->kv_heads, a->window, a->few, a->many, a->splits);
+                cut = cut_of(n, len, a->group, a->kv_heads, a->window, a->few, a->many, a->few_splits, a->many_splits);
                 if (cut.form == FORM) units = cut.tiles * cut.splits * a->kv_heads;
             }
         }
@@ -442,7 +454,7 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
         const int tok = rr / a->group, h = u.head * a->group + (rr - tok * a->group);
         const long t = u.first + tok, at_row = t * a->q_heads + h;
         if (u.cut.splits > 1) {
-            const long slot = at_row * a->splits + u.split;
+            const long slot = part_at(*a, FEW, u.cut.splits, u.b, rr, u.head, (int)t, h) + u.split;
             *(f32x4*)(a->part_o + slot * a->dim + d) = y;
             if (d == 0) a->part_ml[slot] = float2{m, l};
         } else {
@@ -679,7 +691,7 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
     if (row < rows) {
         const long t = u.first + token, at_row = t * a->q_heads + head;
         if (u.cut.splits > 1) {
-            const long slot = at_row * a->splits + u.split;
+            const long slot = part_at(*a, FORM, u.cut.splits, u.b, row, u.head, (int)t, head) + u.split;
             if (h == 0) a->part_ml[slot] = float2{run.m, run.l};
 #pragma unroll
             for (int i = 0; i < DB; ++i)
@@ -736,18 +748,26 @@ __global__ __launch_bounds__(2 * rows_of(FORM), DP <= 128 ? 2 : 1) void cache_at
 // joined does not depend on the parts that other rows have.  Both are bound by latency, the loads of a row's parts all under way at once.
 //   a few rows of many parts   four waves a row, a part a team of dim / 4 lanes (64 rows of 64 parts of 128: 7 us)
 //   many rows                  dim / 4 lanes a row, a wave takes 256 / dim heads of a token
-struct Joined { int n, len, first, splits; };
+struct Joined { int b, n, len, first, form, splits; };
 
 __device__ __forceinline__ Joined joined_of(const AttnArgs& a, int t) {
-    Joined j{0, 0, 0, 0};
-    const int b = seq_of_token(a.cu_new, a.rows, t);
+    Joined j{0, 0, 0, 0, 0, 0};
+    const int b = j.b = seq_of_token(a.cu_new, a.rows, t);
     if (b >= a.rows) return j;
     j.first = a.cu_new[b];
     j.n = a.cu_new[b + 1] - j.first;
     j.len = clamp_len(a.lens[b], a.width << a.page_shift);
     if (j.first < 0 || j.n < 0 || j.n > a.tokens || j.first > a.tokens - j.n || t < j.first || t >= j.first + j.n) j.n = 0;
-    if (j.n > 0) j.splits = cut_of(j.n, j.len, a.group, a.kv_heads, a.window, a.few, a.many, a.splits).splits;
+    if (j.n > 0) {
+        const Cut cut = cut_of(j.n, j.len, a.group, a.kv_heads, a.window, a.few, a.many, a.few_splits, a.many_splits);
+        j.form = cut.form;
+        j.splits = cut.splits;
+    }
     return j;
+}
+__device__ __forceinline__ long part_at(const AttnArgs& a, const Joined& j, int t, int h) {
+    const int kv_head = h / a.group;
+    return part_at(a, j.form, j.splits, j.b, (t - j.first) * a.group + h - kv_head * a.group, kv_head, t, h);
 }
 
 // the factor of a part of maximum m and sum l, `top` being the row's maximum; 0: a part that saw no key of the row, and left no numbers
@@ -772,7 +792,7 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(AttnArgs a, i
     const Joined j = joined_of(a, t);
     const int h = (wave - t * waves_a_token) * at_once + lane / quads, d = lane % quads * 4;
     if (j.splits <= 1 || lane / quads >= at_once || h >= a.q_heads) return;
-    const long slot = ((long)t * a.q_heads + h) * a.splits;
+    const long slot = part_at(a, j, t, h);
     float m = -INFINITY, l[8];
     f32x4 y[8];
 #pragma unroll
@@ -805,7 +825,7 @@ __global__ __launch_bounds__(256) void cache_attention_join_row_kernel(AttnArgs 
     const int lane = threadIdx.x & 63, t = blockIdx.x / a.q_heads, h = blockIdx.x - t * a.q_heads;
     const Joined j = joined_of(a, t);
     if (j.splits <= 1) return;
-    const long slot = (long)blockIdx.x * a.splits;
+    const long slot = part_at(a, j, t, h);
     const float2 ml = lane < j.splits ? a.part_ml[slot + lane] : float2{-INFINITY, 0.f};
     float m = ml.x;
 #pragma unroll
@@ -842,7 +862,10 @@ constexpr int FEW_LIMIT = 16, MANY_LIMIT = 1024;
 struct Plan {
     bool few, many, large;             // which forms are launched
     int few_limit, many_limit;         // rows (INT_MAX: all)
-    int splits;                        // a row's parts, at most
+    int few_splits, many_splits;       // a row's parts, at most
+    bool few_by_sequence;
+    int many_room;
+    long few_parts, many_parts;        // in the workspace
     long few_units, many_units, large_units;
 };
 
@@ -852,28 +875,37 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     const int group = d.q_heads / c.kv_heads;
     const int len = (int)(d.max_len > 0 && d.max_len < capacity ? d.max_len : capacity);
     const int most_new = d.max_new > 0 && d.max_new < d.tokens ? d.max_new : d.tokens;
-    const bool alone = c.rows == 1;                                // then its new tokens are all of them
-    const long most_rows = (long)(alone ? d.tokens : most_new) * group;
+    // One sequence is taken to have all of the new tokens, and the one form that they ask for is launched; where it has fewer (rows behind it), that form does
+    // as well.  Several may be of any size up to the bound.
+    const bool alone = c.rows == 1;
+    const long most_rows = (long)most_new * group;
     const bool wide = c.dim > 128;                                 // (256 rows of them do not fit the registers)
     p.large = most_rows > MANY_LIMIT && !wide;
     p.many = most_rows > FEW_LIMIT && !(alone && p.large);
     p.few = !(alone && most_rows > FEW_LIMIT);
-    p.few_limit = most_rows > FEW_LIMIT ? FEW_LIMIT : 0x7fffffff;
-    p.many_limit = p.large ? MANY_LIMIT : 0x7fffffff;
-    p.splits = 1;
+    p.few_limit = most_rows <= FEW_LIMIT ? 0x7fffffff : (p.few ? FEW_LIMIT : 0);
+    p.many_limit = !p.large ? 0x7fffffff : (p.many ? MANY_LIMIT : 0);
+    p.few_splits = p.many_splits = 1;
     // (of the longest sequence: a part more or less because of the others in a call would show in the last bit)
     const long span = (long)d.window + 63 + (most_rows > FEW_LIMIT ? FEW_LIMIT : most_new);
-    if (p.few) p.splits = splits_of(FEW, 1, 1, d.window > 0 && span < len ? (int)span : len, c.kv_heads);
+    if (p.few) p.few_splits = splits_of(FEW, 1, 1, d.window > 0 && span < len ? (int)span : len, c.kv_heads);
     if (p.many || p.large) {
         const int tile = rows_of(p.large ? LARGE : MANY);
-        const int tiles = (int)(((long)d.tokens * group + tile - 1) / tile);
-        const int s = splits_of(MANY, alone ? (int)most_rows : 1, alone ? tiles : 1, len, alone ? c.kv_heads : 1);
-        if (s > p.splits) p.splits = s;
+        const int tiles = (int)((most_rows + tile - 1) / tile);
+        p.many_splits = splits_of(MANY, alone ? (int)most_rows : 1, alone ? tiles : 1, len, alone ? c.kv_heads : 1);
     }
-    const long rows = (long)d.tokens * group, some = c.rows < d.tokens ? c.rows : d.tokens, parts = (long)(p.splits < 8 ? p.splits : 8) * c.kv_heads;
-    p.few_units = (some + rows / rows_of(FEW)) * p.splits * c.kv_heads;
-    p.many_units = (some + rows / rows_of(MANY)) * parts;
-    p.large_units = (some + rows / rows_of(LARGE)) * parts;
+    // Room for the parts: of every token's rows, or where that is less of every sequence's, which has at most FEW_LIMIT rows a key head there, or (tiles *
+    // key heads * parts <= 256) at most 256 tiles of rows here
+    const long rows = (long)d.tokens * group, heads = (long)d.tokens * d.q_heads;
+    p.few_by_sequence = p.few_limit == FEW_LIMIT && (long)c.rows * c.kv_heads * FEW_LIMIT < heads;
+    p.few_parts = p.few_splits > 1 ? (p.few_by_sequence ? (long)c.rows * c.kv_heads * FEW_LIMIT : heads) * p.few_splits : 0;
+    const int room = 256 * rows_of(p.large ? LARGE : MANY);
+    p.many_room = (long)c.rows * room < heads * p.many_splits ? room : 0;
+    p.many_parts = p.many_splits > 1 ? (p.many_room ? (long)c.rows * room : heads * p.many_splits) : 0;
+    const long some = c.rows < d.tokens ? c.rows : d.tokens;
+    p.few_units = (some + rows / rows_of(FEW)) * p.few_splits * c.kv_heads;
+    p.many_units = (some + rows / rows_of(MANY)) * p.many_splits * c.kv_heads;
+    p.large_units = (some + rows / rows_of(LARGE)) * p.many_splits * c.kv_heads;
     return p;
 }
 
@@ -897,9 +929,9 @@ int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
         cache_attention_few_kernel<T, DP><<<grid_for(p.few_units, 256 * few_waves(DP)), 256, 0, s>>>(a);
         DISCO_LAUNCH_CHECK("cache_attention_few_kernel");
     }
-    if (p.splits > 1) {
+    if (p.few_parts + p.many_parts > 0) {
         const long rows = (long)a.tokens * a.q_heads;
-        if (p.splits > 8 && rows <= 2048) cache_attention_join_row_kernel<T><<<(unsigned)rows, 256, 0, s>>>(a);
+        if (p.few_splits > 8 && rows <= 2048) cache_attention_join_row_kernel<T><<<(unsigned)rows, 256, 0, s>>>(a);
         else {
             const int waves_a_token = cdiv(a.q_heads, 256 / a.dim);
             cache_attention_join_kernel<T><<<(unsigned)(((long)a.tokens * waves_a_token + 3) / 4), 256, 0, s>>>(a, waves_a_token);
@@ -923,20 +955,18 @@ int run_dims(const AttnArgs& a, const Plan& p, hipStream_t s) {
 
 size_t cache_attention_ws_bytes(const disco_cache_desc& c, const disco_attention_desc& d) {
     const Plan p = plan_of(c, d);
-    if (p.splits == 1) return 0;
-    const size_t parts = (size_t)d.tokens * d.q_heads * p.splits;
-    return parts * ((size_t)c.dim * 4 + 8);
+    return (size_t)(p.few_parts + p.many_parts) * ((size_t)c.dim * 4 + 8);
 }
 
 int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc& d, const void* q, const int* table, const int* lens,
                            const int* cu_new, void* out, float* lse, void* ws, hipStream_t s) {
     const Plan p = plan_of(c, d);
-    const size_t parts = (size_t)d.tokens * d.q_heads * p.splits;
+    const size_t parts = (size_t)(p.few_parts + p.many_parts);
     const int window = d.window >= (long)c.table_width * c.page_size ? 0 : d.window;      // (no key is that far back)
-    AttnArgs a{(const char*)q, (const char*)c.d_k, (const char*)c.d_v, (char*)out, lse, (float*)ws, (float2*)((char*)ws + (p.splits > 1 ? parts * c.dim * 4 : 0)),
+    AttnArgs a{(const char*)q, (const char*)c.d_k, (const char*)c.d_v, (char*)out, lse, (float*)ws, (float2*)((char*)ws + parts * c.dim * 4),
                table, lens, cu_new, d.q_token * 2, d.q_head * 2, d.out_token * 2, d.out_head * 2, c.page_stride * 2, c.head_stride * 2, c.slot_stride * 2,
                d.tokens, d.q_heads, c.kv_heads, d.q_heads / c.kv_heads, c.dim, c.rows, c.table_width, c.pages, __builtin_ctz((unsigned)c.page_size), d.causal,
-               window, p.splits, p.few_limit, p.many_limit, fabsf(d.scale) * 1.4426950408889634f, d.scale < 0};
+               window, p.few_splits, p.many_splits, p.few_by_sequence, p.many_room, p.few_parts, p.few_limit, p.many_limit, fabsf(d.scale) * 1.4426950408889634f, d.scale < 0};
     if (a.c < 1e-37f) a.c = 1e-37f;                                // 0 * -inf is not the score of a key that is not seen
     return c.dtype == DISCO_F16 ? run_dims<f16>(a, p, s) : run_dims<bf16>(a, p, s);
 }

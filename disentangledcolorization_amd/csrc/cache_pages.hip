@@ -103,7 +103,8 @@ __device__ __forceinline__ int reserve_new(const ReserveArgs& a, int r) {
 
 __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
     extern __shared__ int upto[];                                  // [rows]: pages that the rows up to and with this one need
-    __shared__ int part[WAVES], over, bad;
+    __shared__ int part[WAVES], bad;
+    __shared__ unsigned long long over;                            // pages beyond the table's width
     const int capacity = a.width << a.shift;
     if (blockIdx.x) {
         const long total = (long)a.rows * a.width, stride = (long)(gridDim.x - 1) * PLAN;
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
         if (r < a.rows) {
             const int len = clamp_len(a.lens[r], capacity), have = pages_of(len, a.shift);
             const long want = ((long)len + reserve_new(a, r) + (1 << a.shift) - 1) >> a.shift;
-            if (want > a.width) atomicAdd(&over, (int)(want - a.width < 1 << 24 ? want - a.width : 1 << 24));
+            if (want > a.width) atomicAdd(&over, (unsigned long long)(want - a.width));
             else need = (int)want - have;
             if (len != a.lens[r] || a.cu_new[r + 1] < a.cu_new[r]) atomicAdd(&bad, 1);
         }
@@ -133,7 +134,8 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
         base += all;
     }
     __syncthreads();
-    const int total = base, too_long = over;
+    const int total = base;
+    const unsigned long long too_long = over;
     bool done = false;
     const int free_pages = scan_pages(a.pages, part,
         [&](int p) {
@@ -164,7 +166,8 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
     }
     if (threadIdx.x == 0) {
         a.info[0] = done ? free_pages - total : free_pages;
-        a.info[1] = done ? 0 : max(total - free_pages, 0) + too_long;
+        const unsigned long long missing = max(total - free_pages, 0) + too_long;
+        a.info[1] = done ? 0 : (int)(missing < 0x7fffffff ? missing : 0x7fffffff);
         a.info[2] = bad;
         a.info[3] = 0;
     }

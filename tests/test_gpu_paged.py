@@ -305,6 +305,37 @@ def test_rows_behind_the_last_sequence_stay():
     assert (out[5:] == 3).all() and torch.equal(out[:5], paged.cache_attention(s.q, *s.args()))
 
 
+@pytest.mark.parametrize("rows", [40, 300, 1500])
+@pytest.mark.parametrize("new", [1, 5, 33])
+def test_one_sequence_with_rows_behind_it(rows, new):
+    """A call of a fixed number of rows, as a captured one has, of which the one sequence uses the first few."""
+    s = Served([700], [new], 2, 2, 64, 16, BF, seed=new)
+    q = torch.cat((s.q, torch.full((rows - new, 4, 64), math.nan, dtype=BF, device=DEV)))
+    for kw in (dict(), dict(max_len=700), dict(max_new=new), dict(window=100)):
+        out = torch.full((rows, 4, 64), 3.0, dtype=BF, device=DEV)
+        got, lse = paged.cache_attention(q, *s.args(), out=out, return_lse=True, **kw)
+        assert (got[new:] == 3).all()
+        close_attended(got, lse, s.q, *s.args(), **{n: kw[n] for n in kw if n == "window"})
+
+
+def test_a_mixed_call_with_long_prompts():
+    """Every form in one call, keys split in each: long prompts, chunks, single tokens, idle rows, and parts kept by sequence and by token."""
+    s = Served([3000, 5000, 0, 900, 2600, 40, 1200], [600, 1, 0, 70, 9, 3, 1100], 1, 2, 64, 16, BF, seed=3)
+    check(s)
+    check(s, window=1500)
+    check(s, max_new=1100, max_len=5000)
+
+
+def test_attention_workspace_stays_small():
+    """What a call asks for in scratch does not grow with the page table's width times the rows of long prompts."""
+    import ctypes as C
+    n = C.c_size_t()
+    c = _ffi.CacheDesc(_ffi.BF16, 1, 9000, 8, 16, 128, 8, 8192, 0, 8 * 16 * 128, 16 * 128, 128, 1 << 20, 1 << 20)
+    a = _ffi.AttentionDesc(16384, 32, 1, 0, 0, 0, 0.1, 4096, 128, 4096, 128)
+    assert _ffi.lib().disco_op_cache_attention_workspace_bytes(C.byref(c), C.byref(a), C.byref(n)) == 0
+    assert 0 < n.value < 1 << 29
+
+
 def test_attention_of_nothing():
     s = Served([50, 0, 20], [0, 0, 0], 2, 2, 64, 16, BF)
     assert paged.cache_attention(s.q, *s.args()).shape == (0, 4, 64)
