@@ -82,13 +82,15 @@ struct Cut { int form, tiles, splits, begin, chunk; };
 // few rows: a workgroup's waves take 128 keys a round, and up to 512 keys (4 us) one workgroup is done sooner than two and a join.  Beyond, parts of 256 /
 //           384 / 512 keys take 14.4 / 16.0 / 17.7 us for one sequence of 4 096 and 134 / 129 / 125 us for 64 of up to 4 096 (32 heads of 128 on 8 key
 //           heads); 64 parts of 8 key heads are two workgroups a CU
-// many rows: as many parts as make 256 workgroups of the sequence, of at least 1 024 keys (a part costs a write and a read of its rows in fp32: 24 sequences of up to 257 tokens over
-//           4 111 take 78 us, with parts of 512 keys 93)
+// many rows: as many parts as make 256 workgroups of the sequence, of at least 1 024 keys (a part costs a write and a read of its rows in fp32: 24
+//           sequences of up to 257 tokens over 4 111 take 78 us, with parts of 512 keys 93).  Up to 64 rows half a workgroup's waves idle, the cache is
+//           read once, and 512 workgroups of at least 512 keys do (8 tokens of 32 heads of 128 over 65 536 keys of 8: 57 us, with 256 workgroups 66,
+//           with at most 8 parts, which are 64 workgroups, 228)
 __host__ __device__ __forceinline__ int splits_of(int form, int rows, int tiles, int keys, int kv_heads) {
     if (form == FEW) return keys <= 512 ? 1 : (keys > 64 * 384 ? 64 : (keys + 383) / 384);
-    const int units = tiles * kv_heads;
-    int s = units >= 256 ? 1 : 256 / units;
-    if (s > 8) s = 8;
+    const int units = tiles * kv_heads, fill = rows <= 64 ? 512 : 256;
+    int s = units >= fill ? 1 : fill / units;
+    if (s > 64) s = 64;
     const int least = rows <= 64 ? 512 : 1024, by_keys = keys <= least ? 1 : (keys + least - 1) / least;
     return s < by_keys ? s : by_keys;
 }
@@ -123,11 +125,14 @@ struct Unit { int b, n, len, first, tile, split, head; Cut cut; };
 
 // unit number `want` of a form over all sequences (key head fastest, then split, then tile - the last, longest tiles first); false behind the last.
 // Every lane of the wave calls it and gets the same.
+// The cursor keeps which 64 sequences were looked at last and how many units lie before them: a workgroup asks for ever larger numbers.
+struct Cursor { int b0, before; };
+
 template <int FORM>
-__device__ __forceinline__ bool find_unit(ArgsAt a, int want, Unit& u) {
+__device__ __forceinline__ bool find_unit(ArgsAt a, int want, Cursor& at_last, Unit& u) {
     const int lane = threadIdx.x & 63, capacity = a->width << a->page_shift;
-    int left = want;
-    for (int b0 = 0; b0 < a->rows; b0 += 64) {
+    int left = want - at_last.before;
+    for (int b0 = at_last.b0; b0 < a->rows; b0 += 64) {
         const int b = b0 + lane;
         int n = 0, len = 0, first = 0, units = 0;
         Cut cut{};
@@ -150,6 +155,7 @@ __device__ __forceinline__ bool find_unit(ArgsAt a, int want, Unit& u) {
         const unsigned long long here = __ballot(upto > left);
         if (here) {
             const int at = __ffsll((long long)here) - 1;
+            at_last = Cursor{b0, want - left};
             u.b = b0 + at;
             u.n = __builtin_amdgcn_readlane(n, at);
             u.len = __builtin_amdgcn_readlane(len, at);
@@ -260,7 +266,11 @@ template <typename T> struct Quad { T e[4]; };
 // ---- few rows -------------------------------------------------------------------------------------------------------------------------------
 // A wave takes every fourth 32-key tile of the workgroup's range.  Keys go from memory straight into the operand (lane: key lane % 16, 8 elements at
 // 32 ks + 8 (lane / 16)); values go through registers into the wave's own piece of LDS, from where they are read transposed.  The next tile's
-// loads are in flight under the current tile.  No barrier but for the join of the four waves at the end.
+// loads are in flight under the current tile.  No barrier but for the join of the four waves at the end.  What the rounding of the probabilities
+// leaves is multiplied as well: the matrix cores wait for memory here, so it costs nothing, and the error is fp32's.
+// Bound by reading the cache: 64 sequences of up to 4 096 keys, 8 key heads of 128, one token each: 125 us for 585 MB, 4.7 TB/s (a large copy: 5.1);
+// one sequence of 130 001 keys on two key heads is 128 workgroups: 84 us, of a CU's own latency; one short sequence 9 us, its chain of loads.
+
 // waves of a SIMD: what the registers of the loop allow (a third one at 128 elements would spill, and take twice the time)
 constexpr int few_waves(int dp) { return dp <= 32 ? 4 : dp <= 64 ? 3 : dp <= 128 ? 2 : 1; }
 
@@ -485,7 +495,8 @@ template <typename T, int DP>
 __device__ __noinline__ void few_unit_odd(uint64_t args, int want, uint32_t lds, uint32_t m, uint32_t l) {
     const ArgsAt a = args_at(args);
     Unit u;
-    if (!find_unit<FEW>(a, __builtin_amdgcn_readfirstlane(want), u)) return;
+    Cursor c{0, 0};
+    if (!find_unit<FEW>(a, __builtin_amdgcn_readfirstlane(want), c, u)) return;
     few_unit<T, DP, true>(a, u, lds_pointer(lds), *(float (*)[4][16])lds_pointer(m), *(float (*)[4][16])lds_pointer(l));
 }
 
@@ -494,9 +505,10 @@ __global__ __launch_bounds__(256, few_waves(DP)) void cache_attention_few_kernel
     const ArgsAt a = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
     __shared__ __align__(16) char lds[4 * Few<T, DP>::WAVE];
     __shared__ float part_m[4][16], part_l[4][16];
+    Cursor c{0, 0};
     for (int want = blockIdx.x;; want += gridDim.x) {
         Unit u;
-        if (!find_unit<FEW>(fresh(a), want, u)) break;
+        if (!find_unit<FEW>(fresh(a), want, c, u)) break;
         if (__syncthreads_or(few_unit<T, DP, false>(fresh(a), u, lds, part_m, part_l) != 0)) {
             few_unit_odd<T, DP>(kernel_args(), want, lds_offset(lds), lds_offset(part_m), lds_offset(part_l));
             __syncthreads();
@@ -724,7 +736,8 @@ template <typename T, int DP, int FORM>
 __device__ __noinline__ void many_unit_odd(uint64_t args, int want, uint32_t lds) {
     const ArgsAt a = args_at(args);
     Unit u;
-    if (!find_unit<FORM>(a, __builtin_amdgcn_readfirstlane(want), u)) return;
+    Cursor c{0, 0};
+    if (!find_unit<FORM>(a, __builtin_amdgcn_readfirstlane(want), c, u)) return;
     many_unit<T, DP, FORM, true>(a, u, lds_pointer(lds));
 }
 
@@ -736,9 +749,10 @@ __global__ __launch_bounds__(2 * rows_of(FORM), DP <= 128 ? 2 : 1) void cache_at
         for (int x = threadIdx.x * 16; x < many_lds<DP>(); x += 32 * rows_of(FORM)) *(uint4*)(lds + x) = uint4{0, 0, 0, 0};
         __syncthreads();
     }
+    Cursor c{0, 0};
     for (int want = blockIdx.x;; want += gridDim.x) {
         Unit u;
-        if (!find_unit<FORM>(fresh(a), want, u)) break;
+        if (!find_unit<FORM>(fresh(a), want, c, u)) break;
         if (__syncthreads_or(many_unit<T, DP, FORM, false>(fresh(a), u, lds) != 0)) many_unit_odd<T, DP, FORM>(kernel_args(), want, lds_offset(lds));
     }
 }
@@ -746,8 +760,9 @@ __global__ __launch_bounds__(2 * rows_of(FORM), DP <= 128 ? 2 : 1) void cache_at
 // ---- the parts of a row whose keys were split -------------------------------------------------------------------------------------------------
 // Part s counts into sum s % 8, the eight sums are added as ((0 + 1) + (2 + 3)) + ((4 + 5) + (6 + 7)), whichever of the two forms joins a row: how a row is
 // joined does not depend on the parts that other rows have.  Both are bound by latency, the loads of a row's parts all under way at once.
-//   a few rows of many parts   four waves a row, a part a team of dim / 4 lanes (64 rows of 64 parts of 128: 7 us)
-//   many rows                  dim / 4 lanes a row, a wave takes 256 / dim heads of a token
+//   a few rows of many parts   four waves a row, a part a team of dim / 4 lanes (64 rows of 64 parts of 128: 7 us; 256 rows of 64 parts: 10 us less
+//                              than the other form)
+//   many rows                  dim / 4 lanes a row, a wave takes 256 / dim heads of a token (10 000 rows of five parts of 64: 15 us)
 struct Joined { int b, n, len, first, form, splits; };
 
 __device__ __forceinline__ Joined joined_of(const AttnArgs& a, int t) {
@@ -772,6 +787,8 @@ __device__ __forceinline__ long part_at(const AttnArgs& a, const Joined& j, int 
 
 // the factor of a part of maximum m and sum l, `top` being the row's maximum; 0: a part that saw no key of the row, and left no numbers
 __device__ __forceinline__ float weight_of(float2 ml, float top) { return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_of(ml.x - top); }
+// (one rounding, written out: both forms of the join have to round alike)
+__device__ __forceinline__ float add_part(float sum, float w, float x) { return w != 0.f ? __builtin_fmaf(w, x, sum) : sum; }
 
 template <typename T>
 __device__ __forceinline__ void put_joined(const AttnArgs& a, const Joined& j, int t, int h, int d, f32x4 y, float m, float l) {
@@ -808,12 +825,12 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(AttnArgs a, i
             const float2 ml = s0 + g < j.splits ? a.part_ml[slot + s0 + g] : float2{-INFINITY, 0.f};
             w[g] = weight_of(ml, m);
             x[g] = s0 + g < j.splits ? *(const f32x4*)(a.part_o + (slot + s0 + g) * a.dim + d) : f32x4{0, 0, 0, 0};
-            l[g] += w[g] != 0.f ? w[g] * ml.y : 0.f;
+            l[g] = add_part(l[g], w[g], ml.y);
         }
 #pragma unroll
         for (int g = 0; g < 8; ++g)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[g][i] += w[g] != 0.f ? w[g] * x[g][i] : 0.f;
+            for (int i = 0; i < 4; ++i) y[g][i] = add_part(y[g][i], w[g], x[g][i]);
     }
     put_joined<T>(a, j, t, h, d, ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7])), m,
                   ((l[0] + l[1]) + (l[2] + l[3])) + ((l[4] + l[5]) + (l[6] + l[7])));
@@ -830,10 +847,10 @@ __global__ __launch_bounds__(256) void cache_attention_join_row_kernel(AttnArgs 
     float m = ml.x;
 #pragma unroll
     for (int i = 32; i; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
-    const float w = weight_of(ml, m), part_l = w != 0.f ? w * ml.y : 0.f;
+    const float w = weight_of(ml, m);
     float l = 0.f;
 #pragma unroll
-    for (int s0 = 0; s0 < 64; s0 += 8) l += __shfl(part_l, s0 + (lane & 7));
+    for (int s0 = 0; s0 < 64; s0 += 8) l = add_part(l, __shfl(w, s0 + (lane & 7)), __shfl(ml.y, s0 + (lane & 7)));
     l += __shfl_xor(l, 1);
     l += __shfl_xor(l, 2);
     l += __shfl_xor(l, 4);
@@ -844,7 +861,11 @@ __global__ __launch_bounds__(256) void cache_attention_join_row_kernel(AttnArgs 
 #pragma unroll
         for (int s0 = 0; s0 < 64; s0 += 8) {
             const float ws = __shfl(w, (s0 + g) & 63);
-            if (team < teams && g < 8 && s0 + g < j.splits && ws != 0.f) sum += ws * *(const f32x4*)(a.part_o + (slot + s0 + g) * a.dim + d);
+            if (team < teams && g < 8 && s0 + g < j.splits && ws != 0.f) {
+                const f32x4 x = *(const f32x4*)(a.part_o + (slot + s0 + g) * a.dim + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = add_part(sum[i], ws, x[i]);
+            }
         }
         if (team < teams && g < 8) *(f32x4*)&sums[g][d] = sum;
     }
@@ -894,8 +915,8 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
         const int tiles = (int)((most_rows + tile - 1) / tile);
         p.many_splits = splits_of(MANY, alone ? (int)most_rows : 1, alone ? tiles : 1, len, alone ? c.kv_heads : 1);
     }
-    // Room for the parts: of every token's rows, or where that is less of every sequence's, which has at most FEW_LIMIT rows a key head there, or (tiles *
-    // key heads * parts <= 256) at most 256 tiles of rows here
+    // Room for the parts: of every token's rows, or where that is less of every sequence's, which has at most FEW_LIMIT rows a key head there, and where its
+    // keys are split at most 256 tiles of rows here (tiles * key heads * parts <= 256; <= 512 of at most 64 rows)
     const long rows = (long)d.tokens * group, heads = (long)d.tokens * d.q_heads;
     p.few_by_sequence = p.few_limit == FEW_LIMIT && (long)c.rows * c.kv_heads * FEW_LIMIT < heads;
     p.few_parts = p.few_splits > 1 ? (p.few_by_sequence ? (long)c.rows * c.kv_heads * FEW_LIMIT : heads) * p.few_splits : 0;
@@ -931,7 +952,7 @@ int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
     }
     if (p.few_parts + p.many_parts > 0) {
         const long rows = (long)a.tokens * a.q_heads;
-        if (p.few_splits > 8 && rows <= 2048) cache_attention_join_row_kernel<T><<<(unsigned)rows, 256, 0, s>>>(a);
+        if ((p.few_splits > 8 || p.many_splits > 8) && rows <= 2048) cache_attention_join_row_kernel<T><<<(unsigned)rows, 256, 0, s>>>(a);
         else {
             const int waves_a_token = cdiv(a.q_heads, 256 / a.dim);
             cache_attention_join_kernel<T><<<(unsigned)(((long)a.tokens * waves_a_token + 3) / 4), 256, 0, s>>>(a, waves_a_token);

@@ -326,6 +326,30 @@ def test_a_mixed_call_with_long_prompts():
     check(s, max_new=1100, max_len=5000)
 
 
+def test_a_row_of_many_parts_is_joined_alike():
+    """A few rows of many parts are joined by another kernel than many rows are: the same bits."""
+    s = Served([20000, 26000, 700], [9, 1, 500], 2, 3, 64, 64, BF, seed=6)
+    together, sums = paged.cache_attention(s.q, *s.args(), return_lse=True)
+    alone, alone_sums = paged.cache_attention(s.q[:10], s.k, s.v, s.table[:2].contiguous(), s.lens[:2].contiguous(), ints([0, 9, 10]), return_lse=True)
+    assert torch.equal(alone, together[:10]) and torch.equal(alone_sums, sums[:10])
+
+
+@pytest.mark.parametrize("tokens,kv_heads,group,dim,dtype", [(16, 1, 4, 64, BF), (5, 2, 8, 128, HF), (9, 1, 2, 256, BF), (64, 1, 1, 96, HF), (128, 1, 1, 32, BF)])
+def test_a_few_tokens_over_a_long_history(tokens, kv_heads, group, dim, dtype):
+    """The many-rows form with the most parts: 17 to 128 rows over more keys than 64 parts of 512 hold."""
+    s = Served([40001, 12345], [tokens, tokens - 1], kv_heads, group, dim, 64, dtype, seed=dim)
+    check(s)
+    check(s, window=30000, max_new=tokens)
+    check(Served([40001], [tokens], kv_heads, group, dim, 64, dtype, seed=dim + 1), max_new=tokens, max_len=40001)
+
+
+def test_attention_of_many_sequences():
+    """More sequences than lanes look at at a time, in every form, idle ones among them."""
+    g = gen(5)
+    new = [0 if i % 9 == 4 else int(torch.randint(1, 12 if i % 50 else 60, (1,), generator=g)) for i in range(300)]
+    check(Served([n + int(torch.randint(0, 40, (1,), generator=g)) if n or i % 2 else 0 for i, n in enumerate(new)], new, 1, 2, 32, 8, HF, seed=1))
+
+
 def test_attention_workspace_stays_small():
     """What a call asks for in scratch does not grow with the page table's width times the rows of long prompts."""
     import ctypes as C
