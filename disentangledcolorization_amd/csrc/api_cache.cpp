@@ -71,7 +71,7 @@ int disco_op_rotary(const disco_rotary_desc* d, const void* d_x, const void* d_p
     if (d->dtype < DISCO_F16 || d->dtype > DISCO_F32) return bad_value(op, "fp16, bf16 or fp32");
     if (d->tokens < 0) return bad_shape(op, "negative size");
     if (!positive(op, {d->heads, d->dim})) return DISCO_ESHAPE;
-    if (d->heads > 1 << 16 || d->dim > 1024) return bad_shape(op, "more than 65536 heads, or 1024 elements a head");
+    if (d->heads > 1 << 16 || d->dim > 1024 || d->tokens > 1 << 30) return bad_shape(op, "more than 2^30 tokens, 65536 heads or 1024 elements a head");
     if (d->rotated < 2 || d->rotated % 2 || d->rotated > d->dim) return bad_shape(op, "rotated must be even, 2 .. dim");
     if (!within({d->x_token, d->x_head, d->out_token, d->out_head})) return bad_shape(op, "stride too large");
     if (!d->tokens) return DISCO_OK;
@@ -87,7 +87,7 @@ int disco_op_cache_append(const disco_cache_desc* c, const disco_append_desc* a,
     if (int rc = check_cache(op, c, true)) return rc;
     if (!a) return bad_value(op, "null argument");
     if (a->tokens < 0 || a->q_heads < 0) return bad_shape(op, "negative size");
-    if (a->q_heads > 1 << 16 || c->kv_heads > 1 << 16) return bad_shape(op, "more than 65536 heads");
+    if (a->q_heads > 1 << 16 || c->kv_heads > 1 << 16 || a->tokens > 1 << 30) return bad_shape(op, "more than 2^30 tokens or 65536 heads");
     if (a->rotated < 0 || a->rotated % 2 || a->rotated > c->dim) return bad_shape(op, "rotated must be even, 0 .. dim");
     if (!within({a->q_token, a->q_head, a->k_token, a->k_head, a->v_token, a->v_head, a->out_token, a->out_head})) return bad_shape(op, "stride too large");
     if (!a->tokens) return DISCO_OK;
@@ -102,6 +102,7 @@ static int check_attention(const char* op, const disco_cache_desc* c, const disc
     if (!a) return bad_value(op, "null argument");
     if (a->tokens < 0) return bad_shape(op, "negative size");
     if (!positive(op, {a->q_heads})) return DISCO_ESHAPE;
+    if (c->kv_heads > 1024) return bad_shape(op, "more than 1024 key heads");
     if (a->q_heads % c->kv_heads) return bad_shape(op, "q_heads must be a multiple of kv_heads");
     if ((int64_t)a->tokens * a->q_heads > (1 << 30)) return bad_shape(op, "more than 2^30 rows");
     if (a->window < 0 || (a->window && !a->causal)) return bad_value(op, "a window needs causal attention");

@@ -77,6 +77,8 @@ def _cache(k, v, page_table, layered=False):
     if page_table.dim() != 2:
         raise ValueError("page_table must be (rows, width)")
     rows, width = page_table.shape
+    if max(*shape, rows, width) > _MOST:
+        raise ValueError("a size beyond 2^31")
     if dims == 5:
         return _ffi.CacheDesc(dtype, shape[0], shape[1], shape[2], shape[3], shape[4], rows, width, st[0], st[1], st[2], st[3], k.data_ptr(), v.data_ptr())
     return _ffi.CacheDesc(dtype, 1, shape[0], shape[1], shape[2], shape[3], rows, width, 0, st[0], st[1], st[2], k.data_ptr(), v.data_ptr())
@@ -89,18 +91,25 @@ def _sequences(c, page_table, lens, cu_new):
 
 
 def _heads(name, t, tokens, heads, dim, dtype):
-    """(tokens, heads, dim) with a head's elements next to each other: the two strides."""
+    """(tokens, heads, dim) with a head's elements next to each other: the two strides (0 of an axis of one, which has none that matters)."""
     if t.shape != (tokens, heads, dim) or t.dtype is not dtype:
         raise ValueError("%s must be (%d, %d, %d) %s, got %s %s" % (name, tokens, heads, dim, dtype, tuple(t.shape), t.dtype))
     token, head, one = t.stride()
     if one != 1 and dim > 1:
         raise ValueError("%s: the elements of a head must lie next to each other" % name)
-    return token, head
+    return token if tokens > 1 else 0, head if heads > 1 else 0
+
+
+def _bound(n):
+    """A whole number for an int32 argument whose check tells only too small from too large."""
+    return max(-1, min(n, _MOST))
 
 
 def _three(name, t):
     if t.dim() != 3:
         raise ValueError("%s must be (tokens, heads, dim)" % name)
+    if t.shape[0] > _MOST:
+        raise ValueError("%s: more than 2^31 tokens" % name)
     return t.shape
 
 
@@ -139,7 +148,8 @@ def rotary(x, positions, inv_freq, gain=1.0, interleaved=False, inverse=False, o
     xs = _heads("x", x, tokens, heads, dim, x.dtype)
     wide, rotated = _positions(positions, tokens), _frequencies(inv_freq)
     if out is None:
-        out, os = x.new_empty((tokens, heads, dim)), (heads * dim, dim)
+        out = x.new_empty((tokens, heads, dim))
+        os = (heads * dim if tokens > 1 else 0, dim if heads > 1 else 0)
     else:
         _device((x, out))
         os = _heads("out", out, tokens, heads, dim, x.dtype)
@@ -192,7 +202,7 @@ def cache_attention(q, k_cache, v_cache, page_table, lens, cu_new, causal=True, 
 
     max_new, max_len: what the caller knows of the largest number of new tokens and the largest length; they size launches and
     workspace, a sequence beyond them still comes out right.  return_lse: also the logarithm of the softmax's sum, (tokens, q_heads)
-    fp32.  Rows behind cu_new[-1] are left as they are in a given `out` (and lse)."""
+    fp32.  Rows behind cu_new[-1] are left as they are in a given `out`, and undefined in lse and an `out` of its own."""
     device = _device((q, k_cache, v_cache), (page_table, lens, cu_new))
     c = _cache(k_cache, v_cache, page_table)
     _sequences(c, page_table, lens, cu_new)
@@ -204,7 +214,8 @@ def cache_attention(q, k_cache, v_cache, page_table, lens, cu_new, causal=True, 
         _device((q, out))
         os = _heads("out", out, tokens, q_heads, dim, q.dtype)
     lse = q.new_empty((tokens, q_heads), dtype=torch.float32) if return_lse else None
-    a = _ffi.AttentionDesc(tokens, q_heads, bool(causal), min(window, _MOST), min(max_new or 0, _MOST), min(max_len or 0, _MOST), 1 / math.sqrt(dim) if scale is None else scale, *qs, *os)
+    a = _ffi.AttentionDesc(tokens, q_heads, bool(causal), _bound(window), _bound(max_new or 0), _bound(max_len or 0),
+                           1 / math.sqrt(dim) if scale is None else scale, *qs, *os)
     lib, need, cd, ad = _ffi.lib(), C.c_size_t(), C.byref(c), C.byref(a)
     _ffi.check(lib.disco_op_cache_attention_workspace_bytes(cd, ad, C.byref(need)))
     need = need.value
@@ -231,12 +242,14 @@ def cache_reserve(page_table, lens, refs, cu_new, page):
         raise ValueError("page_table must be (rows, width), refs (pages,)")
     rows, width = page_table.shape
     pages = refs.numel()
+    if max(rows, width, pages) > _MOST:
+        raise ValueError("a size beyond 2^31")
     _ints("page_table", page_table, (rows, width))
     _ints("lens", lens, (rows,))
     _ints("refs", refs, (pages,))
     _ints("cu_new", cu_new, (rows + 1,))
     new, at = _state(page_table, rows, width, pages)
-    _call(device, _ffi.lib().disco_op_cache_reserve, rows, width, pages, page, page_table.data_ptr(), lens.data_ptr(), refs.data_ptr(), cu_new.data_ptr(), *at)
+    _call(device, _ffi.lib().disco_op_cache_reserve, rows, width, pages, _bound(page), page_table.data_ptr(), lens.data_ptr(), refs.data_ptr(), cu_new.data_ptr(), *at)
     return new
 
 
@@ -270,7 +283,8 @@ def cache_compact(page_table, lens, k_cache, v_cache):
 
 
 def cache_copy_pages(k_cache, v_cache, src, dst):
-    """Page src[i] is copied to page dst[i], in all layers (src, dst int32).  No page of dst may be among src; pairs out of range are skipped."""
+    """Page src[i] is copied to page dst[i], in all layers (src, dst int32).  No page of dst may be among src, or there twice;
+    pairs out of range are skipped."""
     device = _device((k_cache, v_cache), (src, dst))
     if src.dim() != 1:
         raise ValueError("src must be (count,)")

@@ -453,7 +453,7 @@ int disco_op_rotary_frequencies(int dim, int scaling, double base, double factor
 
 typedef struct disco_rotary_desc {
     int32_t dtype;                             /* DISCO_F16 / DISCO_BF16 / DISCO_F32 */
-    int32_t tokens, heads, dim, rotated;       /* the first `rotated` (even) of a head's dim (at most 1024) elements turn, the others are copied */
+    int32_t tokens, heads, dim, rotated;       /* tokens <= 2^30; the first `rotated` (even) of a head's dim (at most 1024) elements turn, the others are copied */
     int32_t interleaved;                       /* pairs (2i, 2i + 1); 0: (i, i + rotated / 2) */
     int32_t inverse;                           /* turns back (gain still multiplies): what a gradient takes */
     int32_t wide_positions;                    /* d_positions is int64 (0: int32) */
@@ -464,7 +464,7 @@ typedef struct disco_rotary_desc {
 int disco_op_rotary(const disco_rotary_desc *d, const void *d_x, const void *d_positions, const double *d_inv_freq, void *d_out, void *stream);
 
 typedef struct disco_append_desc {
-    int32_t tokens;                            /* rows of q, k, v; rows behind d_cu_new[rows] are left alone */
+    int32_t tokens;                            /* <= 2^30; rows of q, k, v; rows behind d_cu_new[rows] are left alone */
     int32_t q_heads;                           /* 0: no queries */
     int32_t rotated, interleaved;              /* as above; rotated = 0: nothing turns */
     int32_t wide_positions;
@@ -478,7 +478,8 @@ int disco_op_cache_append(const disco_cache_desc *c, const disco_append_desc *a,
                           const double *d_inv_freq, void *d_q_out, void *stream);
 
 typedef struct disco_attention_desc {
-    int32_t tokens, q_heads;                   /* q_heads a multiple of kv_heads: query head h reads key head h / (q_heads / kv_heads) */
+    int32_t tokens, q_heads;                   /* q_heads a multiple of kv_heads (at most 1024): query head h reads key head h / (q_heads / kv_heads);
+                                                  tokens * q_heads <= 2^30 */
     int32_t causal;                            /* 1: the token at position p sees the keys 0 .. p; 0: all of its sequence */
     int32_t window;                            /* > 0 (causal only): the keys p - window + 1 .. p */
     int32_t max_new, max_len;                  /* bounds that the host knows of new tokens and length of one sequence, 0: none.  They choose launch
@@ -509,7 +510,7 @@ int disco_op_cache_select(const disco_cache_desc *c, const int32_t *d_page_table
 int disco_op_cache_compact(const disco_cache_desc *c, const int32_t *d_page_table, const int32_t *d_lens, int32_t *d_page_table_out,
                            int32_t *d_refs_out, int32_t *d_info, void *d_ws, size_t ws_bytes, void *stream);
 size_t disco_op_cache_pages_workspace_bytes(int rows, int pages);   /* of select and compact */
-/* Page d_src[i] is copied to page d_dst[i] in all layers, i < count; no page of d_dst may be among d_src.  Pairs out of range are skipped. */
+/* Page d_src[i] is copied to page d_dst[i] in all layers, i < count; no page of d_dst may be among d_src, or there twice.  Pairs out of range are skipped. */
 int disco_op_cache_copy_pages(const disco_cache_desc *c, const int32_t *d_src, const int32_t *d_dst, int count, void *stream);
 
 #ifdef __cplusplus

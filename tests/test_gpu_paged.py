@@ -93,6 +93,21 @@ def test_rotary_places_and_strides(interleaved):
     assert torch.equal(y, joined)                       # nothing else was touched
 
 
+def test_an_axis_of_one_has_any_stride():
+    """A view's stride of an axis of one is what it was cut from: nothing may be refused, or read, because of it."""
+    f, p = paged.rotary_frequencies(64), torch.tensor([77], device=DEV)
+    x = torch.randn(1, 3, 64, generator=gen(0)).to(BF).to(DEV)
+    odd = x.as_strided((1, 3, 64), (5, 64, 1))
+    want = paged.rotary(x, p, f)
+    assert torch.equal(paged.rotary(odd, p, f), want)
+    y = x.clone()
+    assert torch.equal(paged.rotary(y.as_strided((1, 3, 64), (7, 64, 1)), p, f, out=y), want)
+    s = Served([50], [1], 1, 3, 64, 16, BF)
+    out = torch.empty_like(s.q)
+    paged.cache_attention(s.q.as_strided((1, 3, 64), (3, 64, 1)), *s.args(), out=out.as_strided((1, 3, 64), (1, 64, 1)))
+    assert torch.equal(out, paged.cache_attention(s.q, *s.args()))
+
+
 def test_rotary_there_and_back():
     """inverse is the transposed rotation: <y, rot(x)> = <rot'(y), x>, and without a gain it undoes the rotation."""
     x, y = (torch.randn(50, 3, 48, generator=gen(s)).to(DEV) for s in (1, 2))
@@ -749,6 +764,30 @@ def test_a_captured_step():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a.nan_to_num(7) if a.is_floating_point() else a, b.nan_to_num(7) if b.is_floating_point() else b)
+
+
+@pytest.mark.parametrize("group", [2, 20])
+def test_a_captured_token_while_its_sequences_grow(group):
+    """One graph serves every length up to its table's: how the keys are cut is found on the GPU, from the lengths of the replay."""
+    s = Served([9000, 6000], [1, 1], 2, group, 64, 64, BF, seed=2)
+    s.k.nan_to_num_(0.5)
+    s.v.nan_to_num_(0.5)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        paged.cache_attention(s.q, *s.args())
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = paged.cache_attention(s.q, *s.args())
+    for lens in ([0, 1], [511, 512], [513, 1025], [2048, 3], [8999, 6000], [1, 0]):
+        s.lens.copy_(ints(lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        got_now = got.clone()
+        want, lse = paged.cache_attention(s.q, *s.args(), return_lse=True, max_new=1, max_len=max(max(lens), 1))
+        assert torch.equal(got_now, want)
+        close_attended(want, lse, s.q, *s.args())
 
 
 def test_other_streams_and_calls_at_once():

@@ -60,7 +60,7 @@ def cache(**kw):
 
 
 BAD_CACHES = [dict(dtype=_ffi.F32), dict(dtype=7), dict(layers=0), dict(pages=0), dict(kv_heads=0), dict(page_size=24), dict(page_size=0), dict(page_size=-16),
-              dict(dim=4), dict(dim=60), dict(dim=264), dict(rows=0), dict(rows=16385), dict(table_width=0), dict(table_width=1 << 27), dict(d_k=None),
+              dict(dim=4), dict(dim=60), dict(dim=264), dict(rows=0), dict(rows=16385), dict(table_width=0), dict(table_width=1 << 27), dict(rows=16384, table_width=1 << 18, page_size=1), dict(d_k=None),
               dict(d_v=None), dict(d_k=(1 << 20) + 8), dict(page_stride=2044), dict(head_stride=1), dict(slot_stride=68), dict(page_stride=1 << 60)]
 
 
@@ -88,6 +88,29 @@ def test_bad_attention_is_refused(lib, kw):
     a, c, p, n = _ffi.AttentionDesc(*[d[f] for f, _ in _ffi.AttentionDesc._fields_]), cache(), C.c_void_p(1 << 20), C.c_size_t()
     assert lib.disco_op_cache_attention(C.byref(c), C.byref(a), p, p, p, p, p, None, p, 1 << 40, None) in (-1, -2)
     assert lib.disco_op_cache_attention_workspace_bytes(C.byref(c), C.byref(a), C.byref(n)) in (-1, -2)
+
+
+def test_more_heads_than_units_can_be_counted_for(lib):
+    c, p, n = cache(kv_heads=1025), C.c_void_p(1 << 20), C.c_size_t()
+    a = _ffi.AttentionDesc(4, 1025, 1, 0, 0, 0, 0.125, 1025 * 64, 64, 1025 * 64, 64)
+    assert lib.disco_op_cache_attention(C.byref(c), C.byref(a), p, p, p, p, p, None, p, 1 << 40, None) == -2
+    assert lib.disco_op_cache_attention_workspace_bytes(C.byref(c), C.byref(a), C.byref(n)) == -2
+    c.kv_heads = a.q_heads = 1024
+    assert lib.disco_op_cache_attention_workspace_bytes(C.byref(c), C.byref(a), C.byref(n)) == 0
+
+
+def test_sizes_that_an_int32_does_not_hold_are_refused():
+    """None of them may arrive as what is left of it in 32 bits (meta tensors: sizes without memory)."""
+    far, meta = (1 << 32) + 4, dict(device="meta", dtype=torch.int32)
+    with pytest.raises(ValueError, match="2\\^31"):
+        paged._three("x", torch.empty(far, 1, 8, device="meta"))
+    kv = torch.empty(far, 1, 16, 8, device="meta", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="2\\^31"):
+        paged._cache(kv, kv, torch.empty(1, 2, **meta))
+    kv = torch.empty(4, 1, 16, 8, device="meta", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="2\\^31"):
+        paged._cache(kv, kv, torch.empty(1, far, **meta))
+    assert [paged._bound(n) for n in (-far, -1, 0, 7, far)] == [-1, -1, 0, 7, (1 << 31) - 1]
 
 
 def test_missing_arguments_and_workspaces_are_refused(lib):
@@ -119,7 +142,8 @@ def test_missing_arguments_and_workspaces_are_refused(lib):
     assert lib.disco_op_cache_copy_pages(C.byref(c), p, p, -1, None) == -2
 
 
-@pytest.mark.parametrize("kw", [dict(dtype=9), dict(tokens=-1), dict(heads=0), dict(dim=0), dict(rotated=0), dict(rotated=3), dict(rotated=66), dict(dim=1026), dict(heads=1 << 17), dict(x_token=1 << 60)])
+@pytest.mark.parametrize("kw", [dict(dtype=9), dict(tokens=-1), dict(heads=0), dict(dim=0), dict(rotated=0), dict(rotated=3), dict(rotated=66), dict(dim=1026), dict(heads=1 << 17), dict(x_token=1 << 60),
+                                dict(tokens=(1 << 30) + 1), dict(tokens=(1 << 31) - 1)])
 def test_bad_rotations_are_refused(lib, kw):
     d = dict(dtype=_ffi.F32, tokens=4, heads=2, dim=64, rotated=64, interleaved=0, inverse=0, wide_positions=0, x_token=128, x_head=64, out_token=128,
              out_head=64, gain=1.0)
@@ -131,7 +155,7 @@ def test_bad_rotations_are_refused(lib, kw):
     assert lib.disco_op_rotary(None, p, p, p, p, None) == -1
 
 
-@pytest.mark.parametrize("kw", [dict(tokens=-1), dict(q_heads=-1), dict(rotated=-2), dict(rotated=5), dict(rotated=66), dict(k_token=1 << 60)])
+@pytest.mark.parametrize("kw", [dict(tokens=-1), dict(q_heads=-1), dict(rotated=-2), dict(rotated=5), dict(rotated=66), dict(k_token=1 << 60), dict(tokens=(1 << 31) - 1)])
 def test_bad_appends_are_refused(lib, kw):
     d = dict(tokens=4, q_heads=4, rotated=64, interleaved=0, wide_positions=0, q_token=256, q_head=64, k_token=128, k_head=64, v_token=128, v_head=64,
              out_token=256, out_head=64, gain=1.0)
