@@ -10,11 +10,14 @@
 //
 // Three forms, chosen by a sequence's own rows (new tokens * group), so that its result does not depend on what else is in the call:
 //   few (up to 16 rows)    cache_attention_few_kernel: 16 rows a workgroup, its four waves deal 32-key tiles; bound by reading the cache
-//   many (up to 1 024)     cache_attention_many_kernel, 128 rows a workgroup, 32 a wave, keys and values staged in LDS for all of them; two workgroups
+//   many                   cache_attention_many_kernel, 128 rows a workgroup, 32 a wave, keys and values staged in LDS for all of them; two workgroups
 //                          a CU, bound by what L2 delivers into LDS (7 TB/s over the chip) and, at short ranges, by latency
-//   large                  the same with 256 rows, which halves what is delivered; bound by the matrix cores and the exponentials, which overlap in part
-//                          (2 048 tokens of 32 heads of 128 behind 16 384 keys: 128 rows 588 us, 256 rows 530 us; 257 tokens behind 4 111 keys:
-//                          79 and 93 us, a CU then having nothing to do beside one workgroup's start and end).  Heads above 128: 128 rows.
+//   large (above 1 024 rows of heads of 72 .. 128)
+//                          the same with 256 rows, which halves what is delivered; bound by the matrix cores and the exponentials, which overlap in part.
+//                          32 heads of 128 on 8: 2 048 tokens behind 16 384 keys 595 us (128 rows: 649), 1 024 of them 336 (370), 8 192 tokens
+//                          583 (631), but 4 prompts of 1 024 tokens 120 (108); below 1 024 rows a CU has nothing to do beside one workgroup's start
+//                          and end.  Heads of 64 stay with 128 rows, there the exponentials bound both: 5 000 tokens of 16 heads 92 us (256 rows: 105),
+//                          4 x 2 048 tokens over 8 192 360 (410), 2 048 behind 16 384 220 (205); heads above 128 do not fit the registers.
 // Where a sequence alone does not fill the GPU its keys are split; the parts (m, sum, o in fp32) are joined by cache_attention_join_kernel.
 //
 // A tile that some row sees only in part, or that has a page outside the cache, takes the masked path: scores of unseen keys are replaced (never
@@ -82,28 +85,31 @@ struct Cut { int form, tiles, splits, begin, chunk; };
 // few rows: a workgroup's waves take 128 keys a round, and up to 512 keys (4 us) one workgroup is done sooner than two and a join.  Beyond, parts of 256 /
 //           384 / 512 keys take 14.4 / 16.0 / 17.7 us for one sequence of 4 096 and 134 / 129 / 125 us for 64 of up to 4 096 (32 heads of 128 on 8 key
 //           heads); 64 parts of 8 key heads are two workgroups a CU
-// many rows: as many parts as make 256 workgroups of the sequence, of at least 1 024 keys (a part costs a write and a read of its rows in fp32: 24
-//           sequences of up to 257 tokens over 4 111 take 78 us, with parts of 512 keys 93).  Up to 64 rows half a workgroup's waves idle, the cache is
-//           read once, and 512 workgroups of at least 512 keys do (8 tokens of 32 heads of 128 over 65 536 keys of 8: 57 us, with 256 workgroups 66,
-//           with at most 8 parts, which are 64 workgroups, 228)
-__host__ __device__ __forceinline__ int splits_of(int form, int rows, int tiles, int keys, int kv_heads) {
+// many rows: as many parts as fill the GPU, two workgroups a CU where two fit (128 rows, heads of up to 128) and the parts are long enough for that, else
+//           one; of at least 1 024 keys, 512 for up to 64 rows, as a part costs a write and a read of its rows in fp32 (24 sequences of up to 257
+//           tokens over 4 111 take 78 us, with parts of 512 keys 93).  32 heads of 128 on 8 key heads: 8 tokens over 65 536 take 57 us, with one workgroup
+//           a CU 66, with at most 8 parts 228; 256 tokens over 18 432 take 117 us, with one workgroup a CU 151.  What has a workgroup a CU as it
+//           is stays whole but for long histories, 16 heads of 64: four sequences of 2 048 tokens over 8 192 take 360 us (in two parts 421), one over
+//           18 432 301 (in two parts 220).
+__host__ __device__ __forceinline__ int splits_of(int form, int rows, int tiles, int keys, int kv_heads, bool narrow) {
     if (form == FEW) return keys <= 512 ? 1 : (keys > 64 * 384 ? 64 : (keys + 383) / 384);
-    const int units = tiles * kv_heads, fill = rows <= 64 ? 512 : 256;
-    int s = units >= fill ? 1 : fill / units;
-    if (s > 64) s = 64;
+    const int units = tiles * kv_heads;
+    if (units >= 256) return form == MANY && narrow && units < 512 && keys >= 16384 ? 2 : 1;
     const int least = rows <= 64 ? 512 : 1024, by_keys = keys <= least ? 1 : (keys + least - 1) / least;
-    return s < by_keys ? s : by_keys;
+    int s = form == MANY && narrow ? 512 / units : 256 / units;
+    if (s > by_keys) s = 256 / units < by_keys ? 256 / units : by_keys;
+    return s < 64 ? s : 64;
 }
 
 // keys that some new token of the sequence sees: begin (a multiple of 64) .. len; every part takes `chunk` of them, a multiple of 128
-__host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv_heads, int window, int few, int many, int most_few, int most_many) {
+__host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv_heads, int window, bool narrow, int few, int many, int most_few, int most_many) {
     Cut u;
     const int rows = n * group;
     u.form = rows <= few ? FEW : (rows <= many ? MANY : LARGE);
     u.begin = window > 0 && len - n - window + 1 > 0 ? (len - n - window + 1) & ~63 : 0;
     const int keys = len - u.begin, tile = rows_of(u.form);
     u.tiles = (rows + tile - 1) / tile;
-    int s = splits_of(u.form, rows, u.tiles, keys, kv_heads);
+    int s = splits_of(u.form, rows, u.tiles, keys, kv_heads, narrow);
     const int most = u.form == FEW ? most_few : most_many;
     if (s > most) s = most;
     u.chunk = ((keys + s - 1) / s + 127) & ~127;
@@ -142,7 +148,7 @@ __device__ __forceinline__ bool find_unit(ArgsAt a, int want, Cursor& at_last, U
             len = clamp_len(a->lens[b], capacity);
             if (first < 0 || n < 0 || n > a->tokens || first > a->tokens - n) n = 0;       // (not offsets)
             if (n > 0) {
-                cut = cut_of(n, len, a->group, a->kv_heads, a->window, a->few, a->many, a->few_splits, a->many_splits);
+                cut = cut_of(n, len, a->group, a->kv_heads, a->window, a->dim <= 128, a->few, a->many, a->few_splits, a->many_splits);
                 if (cut.form == FORM) units = cut.tiles * cut.splits * a->kv_heads;
             }
         }
@@ -774,7 +780,7 @@ __device__ __forceinline__ Joined joined_of(const AttnArgs& a, int t) {
     j.len = clamp_len(a.lens[b], a.width << a.page_shift);
     if (j.first < 0 || j.n < 0 || j.n > a.tokens || j.first > a.tokens - j.n || t < j.first || t >= j.first + j.n) j.n = 0;
     if (j.n > 0) {
-        const Cut cut = cut_of(j.n, j.len, a.group, a.kv_heads, a.window, a.few, a.many, a.few_splits, a.many_splits);
+        const Cut cut = cut_of(j.n, j.len, a.group, a.kv_heads, a.window, a.dim <= 128, a.few, a.many, a.few_splits, a.many_splits);
         j.form = cut.form;
         j.splits = cut.splits;
     }
@@ -900,8 +906,7 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     // as well.  Several may be of any size up to the bound.
     const bool alone = c.rows == 1;
     const long most_rows = (long)most_new * group;
-    const bool wide = c.dim > 128;                                 // (256 rows of them do not fit the registers)
-    p.large = most_rows > MANY_LIMIT && !wide;
+    p.large = most_rows > MANY_LIMIT && c.dim > 64 && c.dim <= 128;
     p.many = most_rows > FEW_LIMIT && !(alone && p.large);
     p.few = !(alone && most_rows > FEW_LIMIT);
     p.few_limit = most_rows <= FEW_LIMIT ? 0x7fffffff : (p.few ? FEW_LIMIT : 0);
@@ -909,18 +914,18 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     p.few_splits = p.many_splits = 1;
     // (of the longest sequence: a part more or less because of the others in a call would show in the last bit)
     const long span = (long)d.window + 63 + (most_rows > FEW_LIMIT ? FEW_LIMIT : most_new);
-    if (p.few) p.few_splits = splits_of(FEW, 1, 1, d.window > 0 && span < len ? (int)span : len, c.kv_heads);
+    if (p.few) p.few_splits = splits_of(FEW, 1, 1, d.window > 0 && span < len ? (int)span : len, c.kv_heads, true);
     if (p.many || p.large) {
-        const int tile = rows_of(p.large ? LARGE : MANY);
-        const int tiles = (int)((most_rows + tile - 1) / tile);
-        p.many_splits = splits_of(MANY, alone ? (int)most_rows : 1, alone ? tiles : 1, len, alone ? c.kv_heads : 1);
+        const int form = alone && p.large ? LARGE : MANY, tile = rows_of(form), tiles = (int)((most_rows + tile - 1) / tile);
+        p.many_splits = alone ? splits_of(form, (int)most_rows, tiles, len, c.kv_heads, c.dim <= 128) : splits_of(MANY, 1, 1, len, 1, true);
     }
-    // Room for the parts: of every token's rows, or where that is less of every sequence's, which has at most FEW_LIMIT rows a key head there, and where its
-    // keys are split at most 256 tiles of rows here (tiles * key heads * parts <= 256; <= 512 of at most 64 rows)
+    // Room for the parts: of every token's rows, or where that is less of every sequence's, which has at most FEW_LIMIT rows a key head there, and here, where
+    // its keys are split, at most 65 536 parts of rows (tiles * key heads * parts <= 512 of 128 rows, or 256 of 256) or two of each row of < 512 tiles
     const long rows = (long)d.tokens * group, heads = (long)d.tokens * d.q_heads;
     p.few_by_sequence = p.few_limit == FEW_LIMIT && (long)c.rows * c.kv_heads * FEW_LIMIT < heads;
     p.few_parts = p.few_splits > 1 ? (p.few_by_sequence ? (long)c.rows * c.kv_heads * FEW_LIMIT : heads) * p.few_splits : 0;
-    const int room = 256 * rows_of(p.large ? LARGE : MANY);
+    const long twice = 2 * c.kv_heads * (p.large ? MANY_LIMIT : rows);
+    const int room = twice <= 65536 ? 65536 : (twice < 131072 ? (int)twice : 131072);
     p.many_room = (long)c.rows * room < heads * p.many_splits ? room : 0;
     p.many_parts = p.many_splits > 1 ? (p.many_room ? (long)c.rows * room : heads * p.many_splits) : 0;
     const long some = c.rows < d.tokens ? c.rows : d.tokens;
@@ -932,20 +937,23 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
 
 unsigned grid_for(long units, long most) { return (unsigned)(units < 1 ? 1 : (units < most ? units : most)); }
 
+// More workgroups than are resident at once: under a causal mask tiles differ in length, and the next one, the longest that is left, goes where one has
+// ended (8 192 tokens of 32 heads of 128 on 8: 657 us with 256 workgroups of the large form, 583 with 1 024, as with 2 048, of which more lie idle in
+// a call of short sequences: the bound on units is the host's).
 template <typename T, int DP, int FORM>
-int run_many(const AttnArgs& a, long units, long most, hipStream_t s) {
+int run_many(const AttnArgs& a, long units, hipStream_t s) {
     static_assert(many_lds<DP>() <= 65536, "more LDS has to be asked for");
-    cache_attention_many_kernel<T, DP, FORM><<<grid_for(units, most), 2 * rows_of(FORM), many_lds<DP>(), s>>>(a);
+    cache_attention_many_kernel<T, DP, FORM><<<grid_for(units, 1024), 2 * rows_of(FORM), many_lds<DP>(), s>>>(a);
     DISCO_LAUNCH_CHECK("cache_attention_many_kernel");
     return DISCO_OK;
 }
 
 template <typename T, int DP>
 int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
-    if constexpr (DP <= 128) {
-        if (p.large) if (int rc = run_many<T, DP, LARGE>(a, p.large_units, 256, s)) return rc;
+    if constexpr (DP > 64 && DP <= 128) {
+        if (p.large) if (int rc = run_many<T, DP, LARGE>(a, p.large_units, s)) return rc;
     }
-    if (p.many) if (int rc = run_many<T, DP, MANY>(a, p.many_units, 512, s)) return rc;
+    if (p.many) if (int rc = run_many<T, DP, MANY>(a, p.many_units, s)) return rc;
     if (p.few) {
         cache_attention_few_kernel<T, DP><<<grid_for(p.few_units, 256 * few_waves(DP)), 256, 0, s>>>(a);
         DISCO_LAUNCH_CHECK("cache_attention_few_kernel");

@@ -358,6 +358,18 @@ def test_a_few_tokens_over_a_long_history(tokens, kv_heads, group, dim, dtype):
     check(Served([40001], [tokens], kv_heads, group, dim, 64, dtype, seed=dim + 1), max_new=tokens, max_len=40001)
 
 
+@pytest.mark.parametrize("other", [[], [40]])
+def test_a_long_chunk_of_many_heads_over_a_long_history(other):
+    """As many rows as workgroups are at once, and their keys in two parts; the first and last tokens against the reference."""
+    n, heads = 512, 64
+    s = Served([16500, *other], [n, *[3 for _ in other]], heads, 1, 8, 64, BF, seed=7)
+    got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True)
+    table = s.table[:1].contiguous()
+    for first in (0, 127, 250, n - 4):
+        close_attended(got[first:first + 4], lse[first:first + 4], s.q[first:first + 4], s.k, s.v, table, ints([16500 - n + first + 4]), ints([0, 4]))
+    assert got.isfinite().all() and torch.equal(got[:n], paged.cache_attention(s.q[:n], s.k, s.v, table, ints([16500]), ints([0, n])))
+
+
 def test_attention_of_many_sequences():
     """More sequences than lanes look at at a time, in every form, idle ones among them."""
     g = gen(5)
