@@ -79,36 +79,41 @@ __host__ __device__ constexpr int rows_of(int form) { return form == FEW ? 16 : 
 constexpr float LN2 = 0.6931471805599453f;
 
 // ---- how a sequence is cut ------------------------------------------------------------------------------------------------------------
-struct Cut { int form, tiles, splits, begin, chunk; };
+struct Cut { int form, tiles, splits, chunk; };
+__host__ __device__ __forceinline__ int min_of(int a, int b) { return a < b ? a : b; }
+// the first key that a token at position p sees, of its tile of 64
+__host__ __device__ __forceinline__ int begin_of(int p, int window) { return window > 0 && p - window + 1 > 0 ? (p - window + 1) & ~63 : 0; }
 
 // parts of a sequence's keys; grows with them
 // few rows: a workgroup's waves take 128 keys a round, and up to 512 keys (4 us) one workgroup is done sooner than two and a join.  Beyond, parts of 256 /
 //           384 / 512 keys take 14.4 / 16.0 / 17.7 us for one sequence of 4 096 and 134 / 129 / 125 us for 64 of up to 4 096 (32 heads of 128 on 8 key
 //           heads); 64 parts of 8 key heads are two workgroups a CU
 // many rows: as many parts as fill the GPU, two workgroups a CU where two fit (128 rows, heads of up to 128) and the parts are long enough for that, else
-//           one; of at least 1 024 keys, 512 for up to 64 rows, as a part costs a write and a read of its rows in fp32 (24 sequences of up to 257
-//           tokens over 4 111 take 78 us, with parts of 512 keys 93).  32 heads of 128 on 8 key heads: 8 tokens over 65 536 take 57 us, with one workgroup
-//           a CU 66, with at most 8 parts 228; 256 tokens over 18 432 take 117 us, with one workgroup a CU 151.  What has a workgroup a CU as it
-//           is stays whole but for long histories, 16 heads of 64: four sequences of 2 048 tokens over 8 192 take 360 us (in two parts 421), one over
-//           18 432 301 (in two parts 220).
+//           one; of at least 1 024 keys, as a part costs a write and a read of its rows in fp32 (24 sequences of up to 257 tokens over 4 111 take
+//           78 us, with parts of 512 keys 93), and of 512 for up to 64 rows and for heads above 128, whose keys take twice the time (200 tokens over
+//           8 192 keys of 8 heads of 256: 79 -> 55 us, 32 sequences of 64 over 2 048 of two: 109 -> 115).
+//           32 heads of 128 on 8 key heads: 8 tokens over 65 536 take 57 us, with one workgroup a CU 66, with at most 8 parts 228; 256 tokens over
+//           18 432 take 117 us, with one workgroup a CU 151.  What has a workgroup a CU as it is stays whole but for long histories, 16 heads of
+//           64: four sequences of 2 048 tokens over 8 192 take 360 us (in two parts 421), one over 18 432 301 (in two parts 220).
 __host__ __device__ __forceinline__ int splits_of(int form, int rows, int tiles, int keys, int kv_heads, bool narrow) {
     if (form == FEW) return keys <= 512 ? 1 : (keys > 64 * 384 ? 64 : (keys + 383) / 384);
     const int units = tiles * kv_heads;
     if (units >= 256) return form == MANY && narrow && units < 512 && keys >= 16384 ? 2 : 1;
-    const int least = rows <= 64 ? 512 : 1024, by_keys = keys <= least ? 1 : (keys + least - 1) / least;
+    const int least = rows <= 64 || !narrow ? 512 : 1024, by_keys = keys <= least ? 1 : (keys + least - 1) / least;
     int s = form == MANY && narrow ? 512 / units : 256 / units;
     if (s > by_keys) s = 256 / units < by_keys ? 256 / units : by_keys;
     return s < 64 ? s : 64;
 }
 
-// keys that some new token of the sequence sees: begin (a multiple of 64) .. len; every part takes `chunk` of them, a multiple of 128
+// How the keys that a tile of rows sees are cut: they begin at begin_of() its first token and are `keys` at most, every part takes `chunk` of them, a multiple
+// of 128.  (Parts of what the tile sees, not of the sequence: 701 tokens of heads of 256 that see 1 024 keys take 60 us, cut across the sequence 81.)
 __host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv_heads, int window, bool narrow, int few, int many, int most_few, int most_many) {
     Cut u;
     const int rows = n * group;
     u.form = rows <= few ? FEW : (rows <= many ? MANY : LARGE);
-    u.begin = window > 0 && len - n - window + 1 > 0 ? (len - n - window + 1) & ~63 : 0;
-    const int keys = len - u.begin, tile = rows_of(u.form);
+    const int tile = rows_of(u.form), across = (tile - 1) / group + 1;        // (a tile's first token and last are no further apart)
     u.tiles = (rows + tile - 1) / tile;
+    const int keys = window <= 0 ? len : (u.tiles == 1 ? len - begin_of(len - n, window) : min_of(len, window + 63 + across));
     int s = splits_of(u.form, rows, u.tiles, keys, kv_heads, narrow);
     const int most = u.form == FEW ? most_few : most_many;
     if (s > most) s = most;
@@ -127,7 +132,7 @@ __device__ __forceinline__ long part_at(const Args& a, int form, int splits, int
     return a.many_from + (a.many_room ? (long)b * a.many_room + ((long)row * a.kv_heads + kv_head) * splits : by_token * a.many_splits);
 }
 
-struct Unit { int b, n, len, first, tile, split, head; Cut cut; };
+struct Unit { int b, n, len, first, tile, split, head, begin; Cut cut; };
 
 // unit number `want` of a form over all sequences (key head fastest, then split, then tile - the last, longest tiles first); false behind the last.
 // Every lane of the wave calls it and gets the same.
@@ -168,12 +173,12 @@ __device__ __forceinline__ bool find_unit(ArgsAt a, int want, Cursor& at_last, U
             u.first = __builtin_amdgcn_readlane(first, at);
             u.cut.tiles = __builtin_amdgcn_readlane(cut.tiles, at);
             u.cut.splits = __builtin_amdgcn_readlane(cut.splits, at);
-            u.cut.begin = __builtin_amdgcn_readlane(cut.begin, at);
             u.cut.chunk = __builtin_amdgcn_readlane(cut.chunk, at);
             int x = left - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(units, at));
             u.head = x % a->kv_heads; x /= a->kv_heads;
             u.split = x % u.cut.splits;
             u.tile = u.cut.tiles - 1 - x / u.cut.splits;
+            u.begin = begin_of(u.len - u.n + u.tile * rows_of(FORM) / a->group, a->window) + u.split * u.cut.chunk;
             return true;
         }
         left -= __builtin_amdgcn_readlane(upto, 63);
@@ -302,7 +307,7 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
     const int pos = a->causal ? u.len - u.n + token : u.len - 1;
     const int last_token = (min(u.tile * rows_of(FEW) + rows_of(FEW), rows) - 1) / a->group, first_token = u.tile * rows_of(FEW) / a->group;
     const int high = a->causal ? u.len - u.n + last_token : u.len - 1, low = a->causal ? u.len - u.n + first_token : u.len - 1;
-    const int begin = u.cut.begin + u.split * u.cut.chunk, end = min(min(begin + u.cut.chunk, u.len), high + 1);
+    const int begin = u.begin, end = min(min(begin + u.cut.chunk, u.len), high + 1);
     // the keys that this lane's row sees here
     const int first_seen = a->window > 0 ? pos - a->window + 1 : 0;
     const uint32_t count_seen = max(0, min(pos + 1, end) - first_seen);
@@ -556,9 +561,7 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
     const bool any_row = row0 < rows;                          // of this wave
     auto pos_of = [&](int r) { return a->causal ? u.len - u.n + min(r, rows - 1) / a->group : u.len - 1; };
     const int low = pos_of(row0), high = pos_of(row0 + 31), tile_low = pos_of(u.tile * ROWS), tile_high = pos_of(u.tile * ROWS + ROWS - 1);
-    const int split_begin = u.cut.begin + u.split * u.cut.chunk, end = min(min(split_begin + u.cut.chunk, u.len), tile_high + 1);
-    int begin = split_begin;                                   // keys before the tile's first window are left out
-    if (a->window > 0 && tile_low - a->window + 1 > begin) begin = (tile_low - a->window + 1) & ~63;
+    const int begin = u.begin, end = min(min(begin + u.cut.chunk, u.len), tile_high + 1);
     // the keys that this lane's row sees here
     const int first_seen = a->window > 0 ? pos - a->window + 1 : 0;
     const uint32_t count_seen = max(0, min(pos + 1, end) - first_seen);
@@ -913,11 +916,12 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     p.many_limit = !p.large ? 0x7fffffff : (p.many ? MANY_LIMIT : 0);
     p.few_splits = p.many_splits = 1;
     // (of the longest sequence: a part more or less because of the others in a call would show in the last bit)
-    const long span = (long)d.window + 63 + (most_rows > FEW_LIMIT ? FEW_LIMIT : most_new);
-    if (p.few) p.few_splits = splits_of(FEW, 1, 1, d.window > 0 && span < len ? (int)span : len, c.kv_heads, true);
+    const long far = (long)d.window + 63 + rows_of(LARGE);
+    const int keys = d.window > 0 && far < len ? (int)far : len;
+    if (p.few) p.few_splits = splits_of(FEW, 1, 1, keys, c.kv_heads, true);
     if (p.many || p.large) {
         const int form = alone && p.large ? LARGE : MANY, tile = rows_of(form), tiles = (int)((most_rows + tile - 1) / tile);
-        p.many_splits = alone ? splits_of(form, (int)most_rows, tiles, len, c.kv_heads, c.dim <= 128) : splits_of(MANY, 1, 1, len, 1, true);
+        p.many_splits = alone ? splits_of(form, (int)most_rows, tiles, keys, c.kv_heads, c.dim <= 128) : splits_of(MANY, 1, 1, keys, 1, true);
     }
     // Room for the parts: of every token's rows, or where that is less of every sequence's, which has at most FEW_LIMIT rows a key head there, and here, where
     // its keys are split, at most 65 536 parts of rows (tiles * key heads * parts <= 512 of 128 rows, or 256 of 256) or two of each row of < 512 tiles

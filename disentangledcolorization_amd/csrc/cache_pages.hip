@@ -89,7 +89,8 @@ __device__ __forceinline__ int scan_pages(int pages, int* part, Look look, Then 
 
 // ---- reserve ------------------------------------------------------------------------------------------------------------------------
 // Block 0 plans: the rows' needs (scanned into LDS), the free pages in ascending order, each finding its row by bisection.  The other blocks copy the
-// entries that every row has already; who writes an entry depends on the input alone, so nothing waits.
+// entries that every row has already; who writes an entry depends on the input alone, so nothing waits.  Bound by latency: one launch of 4 to 8 us (64 rows of
+// 256 entries over 8 000 pages: 4 us).
 struct ReserveArgs {
     const int *table, *lens, *refs, *cu_new;
     int *table_out, *lens_out, *refs_out, *info;
@@ -174,6 +175,8 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
 }
 
 // ---- pieces of select and compact ------------------------------------------------------------------------------------------------------
+// A plan of one workgroup (new table, counts, a list of copies), then the copies.  A plan is a chain of passes over the table and the pages with the
+// workgroup's barriers between them: 13 us for 64 rows of 63 entries over 3 100 pages, 15 us for the compaction of 1 800 pages.
 __global__ void clear_kernel(int* p, int n, int* q, int m) {
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
     for (int j = i; j < n; j += gridDim.x * blockDim.x) p[j] = 0;
@@ -378,7 +381,8 @@ struct CopyArgs {
     int rows, width, shift;
 };
 
-// One wave copies the filled slots of one head of a page; every 16 bytes once in, once out: bound by memory
+// One wave copies the filled slots of one head of a page; every 16 bytes once in, once out: bound by memory (409 MB in and out: 80 us, 5.1 TB/s, what a large
+// copy reaches)
 __global__ __launch_bounds__(256) void cache_copy_kernel(CopyArgs a) {
     if (a.table) {
         const int capacity = a.width << a.shift;
@@ -437,7 +441,8 @@ int allow_lds(K kernel, size_t bytes) {
     return DISCO_OK;
 }
 
-// Tables of up to 64 K entries over up to 32 K pages (and 4 K rows: 144 KB of LDS): one workgroup counts while it plans
+// Tables of up to 64 K entries over up to 32 K pages (and 4 K rows: 144 KB of LDS): one workgroup counts while it plans (64 beams: 17 us a call, with two
+// more launches 24); beyond, its passes over the table would take longer than the launches
 bool local(const disco_cache_desc& c) { return (long)c.rows * c.table_width <= 65536 && c.pages <= 32768 && c.rows <= 4096; }
 
 struct Scratch { Copy* copies; int *count, *bad, *map, *refs; };
