@@ -89,8 +89,8 @@ __device__ __forceinline__ int scan_pages(int pages, int* part, Look look, Then 
 
 // ---- reserve ------------------------------------------------------------------------------------------------------------------------
 // Block 0 plans: the rows' needs (scanned into LDS), the free pages in ascending order, each finding its row by bisection.  The other blocks copy the
-// entries that every row has already; who writes an entry depends on the input alone, so nothing waits.  Bound by latency: one launch of 4 to 8 us (64 rows of
-// 256 entries over 8 000 pages: 4 us).
+// entries that every row has already; who writes an entry depends on the input alone, so nothing waits.  Bound by latency: one launch of 4 us (64 rows
+// that take a token each) to 8 (five that take 80 pages each).
 struct ReserveArgs {
     const int *table, *lens, *refs, *cu_new;
     int *table_out, *lens_out, *refs_out, *info;
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
 
 // ---- pieces of select and compact ------------------------------------------------------------------------------------------------------
 // A plan of one workgroup (new table, counts, a list of copies), then the copies.  A plan is a chain of passes over the table and the pages with the
-// workgroup's barriers between them: 13 us for 64 rows of 63 entries over 3 100 pages, 15 us for the compaction of 1 800 pages.
+// workgroup's barriers between them: 13 us for 64 rows of 63 entries over 2 400 pages, 15 us for the compaction of 32 rows over 3 200.
 __global__ void clear_kernel(int* p, int n, int* q, int m) {
     const int i = blockIdx.x * blockDim.x + threadIdx.x;
     for (int j = i; j < n; j += gridDim.x * blockDim.x) p[j] = 0;

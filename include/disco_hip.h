@@ -13,6 +13,8 @@
  *   disco_workspace_bytes             (allocation the reference leaves to torch's caching allocator)
  *   disco_op_*                        the individual stock-PyTorch operators of SURVEY §2b
  *                                     (K1..K16), exposed so each kernel can be parity-tested
+ *   disco_op_rotary*, disco_op_cache_*  (no counterpart in the reference) token sequences served from a
+ *                                     paged cache: rotary positions, append, attention, pages
  *
  * Conventions
  *   - plain pointers and sizes only; no torch types.  `d_` arguments are DEVICE pointers on the
