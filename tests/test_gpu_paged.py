@@ -358,6 +358,20 @@ def test_a_few_tokens_over_a_long_history(tokens, kv_heads, group, dim, dtype):
     check(Served([40001], [tokens], kv_heads, group, dim, 64, dtype, seed=dim + 1), max_new=tokens, max_len=40001)
 
 
+@pytest.mark.parametrize("lens,new,kv_heads,group,dim,window", [
+    ([3000, 77], [300, 5], 2, 4, 256, 1024), ([1900, 1900], [500, 1], 1, 3, 64, 1300), ([1700], [1700], 1, 1, 192, 600), ([5000, 40, 2100], [120, 40, 3], 1, 8, 128, 2050),
+    ([2600], [30], 1, 4, 96, 2560), ([2600], [17], 1, 1, 32, 2499), ([2049], [400], 1, 3, 128, 2047),
+])
+def test_windows_whose_keys_are_cut_by_tile(lens, new, kv_heads, group, dim, window):
+    """What a tile of rows sees is split, from the first key of its first token on: windows longer than a part, shorter than the chunk, and almost everything."""
+    s = Served(lens, new, kv_heads, group, dim, 16, BF, seed=window)
+    got, _ = check(s, window=window)
+    assert torch.equal(got, paged.cache_attention(s.q, *s.args(), window=window, max_new=max(new), max_len=max(lens)))
+    a, e = int(s.cu[0]), int(s.cu[1])
+    alone = paged.cache_attention(s.q[a:e], s.k, s.v, s.table[:1].contiguous(), s.lens[:1].contiguous(), ints([0, e - a]), window=window)
+    assert torch.equal(alone, got[a:e])
+
+
 @pytest.mark.parametrize("other", [[], [40]])
 def test_a_long_chunk_of_many_heads_over_a_long_history(other):
     """As many rows as workgroups are at once, and their keys in two parts; the first and last tokens against the reference."""
