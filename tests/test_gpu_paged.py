@@ -816,6 +816,50 @@ def test_a_captured_token_while_its_sequences_grow(group):
         close_attended(want, lse, s.q, *s.args())
 
 
+@pytest.mark.parametrize("rows,pages", [(9000, 12000), (64, 40000)])
+def test_captured_page_calls_over_large_pools(rows, pages):
+    """Plans with more shared memory than a launch has unasked, and plans of several launches, replayed over tables that change between the replays."""
+    kv = torch.randn(pages, 1, 8, 8, generator=gen(1)).to(BF).to(DEV)
+    k, v = kv.clone(), -kv
+    g = gen(2)
+    lens = torch.randint(0, 9, (rows,), generator=g, dtype=torch.int32)
+    table = torch.full((rows, 3), -1, dtype=torch.int32)
+    used = torch.randperm(pages, generator=g)[:rows].int()
+    table[:, 0] = torch.where(lens > 0, used, table[:, 0])
+    table, lens = table.to(DEV), lens.to(DEV)
+    refs = torch.zeros(pages, dtype=torch.int32, device=DEV)
+    refs[table[lens > 0, 0].long()] = 1
+    cu = ints(list(range(rows + 1)))
+    parents = torch.arange(rows, dtype=torch.int32, device=DEV)
+
+    def step():
+        t, n, r, info = paged.cache_reserve(table, lens, refs, cu, 8)
+        t, n, r, more = paged.cache_select(t, n, parents, k, v)
+        return (*paged.cache_compact(t, n, k, v), n, info, more)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(3):
+        parents.copy_(torch.arange(rows) // (i + 1) * (i + 1) % rows)
+        k.copy_(kv)
+        v.copy_(-kv)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in outs] + [k.clone(), v.clone()]
+        k.copy_(kv)
+        v.copy_(-kv)
+        want = [*step(), k, v]
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
 def test_other_streams_and_calls_at_once():
     """Each call runs on the current stream; calls on several streams at once have workspaces of their own."""
     s = [Served([3000 + 7 * i, 40], [1, 30], 2, 4, 64, 16, BF, seed=i) for i in range(4)]
