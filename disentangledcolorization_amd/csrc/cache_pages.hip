@@ -119,6 +119,7 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
         return;
     }
     if (threadIdx.x == 0) { over = 0; bad = 0; }
+    __syncthreads();                                               // (every wave counts into them)
     int base = 0;
     for (int r0 = 0; r0 < a.rows; r0 += PLAN) {
         const int r = r0 + threadIdx.x;

@@ -592,6 +592,21 @@ def test_reserve_counts_what_is_out_of_range():
     assert got[1].tolist() == [32, 3] and got[3].tolist() == [2, 0, 2, 0] and got[0].tolist() == [[0, -1], [1, -1]]
 
 
+@pytest.mark.parametrize("row", [0, 64, 150, 1023, 1024, 1999])
+def test_reserve_counts_the_rows_of_every_wave(row):
+    """One row that is too long for the table, or out of range, wherever among the rows: the call fails as a whole, or counts it."""
+    rows = 2000
+    table, lens, refs = ints([[b, -1] for b in range(rows)]), [9] * rows, ints([1] * rows + [0] * rows)
+    cu = [0]
+    for b in range(rows):
+        cu.append(cu[-1] + (40 if b == row else 1))       # 49 tokens: four pages, two more than the table is wide
+    got = paged.cache_reserve(table, ints(lens), refs, ints(cu), 16)
+    assert torch.equal(got[0], table) and got[1].tolist() == lens and torch.equal(got[2], refs) and got[3].tolist() == [rows, 2, 0, 0]
+    lens[row] = -3
+    got = paged.cache_reserve(table, ints(lens), refs, ints(list(range(rows + 1))), 16)
+    assert got[3].tolist()[1:] == [0, 1, 0] and got[1].tolist() == [10 if b != row else 1 for b in range(rows)]
+
+
 def fork_state(rows, page, seed, full=False):
     """Rows of which some share their first pages."""
     g = gen(seed)
