@@ -110,6 +110,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         const int b = seq_of_token(a.cu_new, a.rows, token);
         if (b >= a.rows) return;                                   // behind the last sequence
         const int first = a.cu_new[b], n = a.cu_new[b + 1] - first;
+        if (token < first) return;                                 // ahead of the first one
         const int len = clamp_len(a.lens[b], a.width << a.page_shift), p = len - n + (token - first);
         position = p;
         if (p >= 0 && p < len) {

@@ -4,7 +4,7 @@ The cache is two tensors of pages, `k_cache` and `v_cache`, bf16 or fp16, (pages
 dim) for the page calls, whose layers share one table; other orders of the inner axes are fine as strides as long as the elements of a head
 lie next to each other.  Row b of `page_table` (rows, width) int32 names the pages of sequence b, `lens` (rows,) int32 says how many tokens
 it holds, `refs` (pages,) int32 how many rows name a page (0: free).  The new tokens of all sequences lie behind each other; `cu_new`
-(rows + 1,) int32 holds where each sequence's begin.
+(rows + 1,) int32 holds where each sequence's begin; rows ahead of its first entry and behind its last belong to no sequence.
 
     inv_freq = rotary_frequencies(128, base=10000.0)
     page_table, lens, refs, info = cache_reserve(page_table, lens, refs, cu_new, page)      # pages for the new tokens
@@ -202,7 +202,7 @@ def cache_attention(q, k_cache, v_cache, page_table, lens, cu_new, causal=True, 
 
     max_new, max_len: what the caller knows of the largest number of new tokens and the largest length; they size launches and
     workspace, a sequence beyond them still comes out right.  return_lse: also the logarithm of the softmax's sum, (tokens, q_heads)
-    fp32.  Rows behind cu_new[-1] are left as they are in a given `out`, and undefined in lse and an `out` of its own."""
+    fp32.  Rows of no sequence are left as they are in a given `out`, and undefined in lse and an `out` of its own."""
     device = _device((q, k_cache, v_cache), (page_table, lens, cu_new))
     c = _cache(k_cache, v_cache, page_table)
     _sequences(c, page_table, lens, cu_new)

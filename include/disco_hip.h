@@ -466,7 +466,7 @@ typedef struct disco_rotary_desc {
 int disco_op_rotary(const disco_rotary_desc *d, const void *d_x, const void *d_positions, const double *d_inv_freq, void *d_out, void *stream);
 
 typedef struct disco_append_desc {
-    int32_t tokens;                            /* <= 2^30; rows of q, k, v; rows behind d_cu_new[rows] are left alone */
+    int32_t tokens;                            /* <= 2^30; rows of q, k, v; rows ahead of d_cu_new[0] and behind d_cu_new[rows] are left alone */
     int32_t q_heads;                           /* 0: no queries */
     int32_t rotated, interleaved;              /* as above; rotated = 0: nothing turns */
     int32_t wide_positions;
@@ -490,7 +490,7 @@ typedef struct disco_attention_desc {
     int64_t q_token, q_head, out_token, out_head;
 } disco_attention_desc;
 /* out = softmax(scale q k^T) v of every new token over its sequence's cache; d_lse (tokens x q_heads fp32, may be NULL): the logarithm of the
- * softmax's sum.  A token that sees no key gets zeros and -inf; rows behind d_cu_new[rows] are left alone.  Keys that a query does not see cannot
+ * softmax's sum.  A token that sees no key gets zeros and -inf; rows ahead of d_cu_new[0] and behind d_cu_new[rows] are left alone.  Keys that a query does not see cannot
  * reach it, whatever they hold.  A sequence's result does not depend on the others in the call. */
 int disco_op_cache_attention_workspace_bytes(const disco_cache_desc *c, const disco_attention_desc *a, size_t *bytes);
 int disco_op_cache_attention(const disco_cache_desc *c, const disco_attention_desc *a, const void *d_q, const int32_t *d_page_table,

@@ -558,6 +558,21 @@ def test_append_positions_place_and_bad_pages():
     paged.cache_append(None, k[:0], v[:0], kc, vc, s.table, s.lens, ints([0, 0, 0]), inv_freq=f)
 
 
+def test_rows_before_the_first_sequence_are_not_appended():
+    """cu_new of some sequences of a larger batch: the rows in front of the first one belong to none, and are written nowhere."""
+    s = Served([60, 30], [10, 3], 2, 1, 64, 16, BF, seed=2)
+    qkv = torch.randn(18, 6, 64, generator=gen(3)).to(BF).to(DEV)
+    q, k, v = qkv.split([2, 2, 2], 1)
+    f = paged.rotary_frequencies(64)
+    want_k, want_v, kc, vc = s.k.clone(), s.v.clone(), s.k.clone(), s.v.clone()
+    want = paged.cache_append(q[5:], k[5:], v[5:], want_k, want_v, s.table, s.lens, s.cu, inv_freq=f)
+    out = torch.full((18, 2, 64), 5.0, dtype=BF, device=DEV)
+    paged.cache_append(q, k, v, kc, vc, s.table, s.lens, s.cu + 5, inv_freq=f, q_out=out)
+    assert torch.equal(out[5:], want) and (out[:5] == 5).all()
+    for a, b in ((kc, want_k), (vc, want_v)):
+        assert torch.equal(a.nan_to_num(9), b.nan_to_num(9))
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows,pages,page,width", [(1, 3, 16, 4), (5, 40, 8, 9), (70, 3000, 1, 64), (1100, 9000, 16, 16), (3, 70000, 4, 1000), (9, 64, 16, 8), (16384, 20000, 16, 2)])
