@@ -153,6 +153,7 @@ SIGNATURES = {
     "disco_op_rotary_frequencies": (_I, [_I, _I, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, _P]),
     "disco_op_rotary": (_I, [C.POINTER(RotaryDesc), _P, _P, _P, _P, _P]),
     "disco_op_cache_append": (_I, [C.POINTER(CacheDesc), C.POINTER(AppendDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    "disco_op_cache_append_reserved": (_I, [C.POINTER(CacheDesc), C.POINTER(AppendDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "disco_op_cache_attention_workspace_bytes": (_I, [C.POINTER(CacheDesc), C.POINTER(AttentionDesc), C.POINTER(_SZ)]),
     "disco_op_cache_attention": (_I, [C.POINTER(CacheDesc), C.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "disco_op_cache_reserve": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P]),

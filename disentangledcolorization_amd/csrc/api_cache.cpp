@@ -83,6 +83,12 @@ int disco_op_rotary(const disco_rotary_desc* d, const void* d_x, const void* d_p
 int disco_op_cache_append(const disco_cache_desc* c, const disco_append_desc* a, const void* d_q, const void* d_k, const void* d_v,
                           const int32_t* d_page_table, const int32_t* d_lens, const int32_t* d_cu_new, const void* d_positions,
                           const double* d_inv_freq, void* d_q_out, void* stream) {
+    return disco_op_cache_append_reserved(c, a, d_q, d_k, d_v, d_page_table, d_lens, d_cu_new, d_positions, d_inv_freq, d_q_out, nullptr, stream);
+}
+
+int disco_op_cache_append_reserved(const disco_cache_desc* c, const disco_append_desc* a, const void* d_q, const void* d_k, const void* d_v,
+                                   const int32_t* d_page_table, const int32_t* d_lens, const int32_t* d_cu_new, const void* d_positions,
+                                   const double* d_inv_freq, void* d_q_out, const int32_t* d_info, void* stream) {
     const char* op = "cache_append";
     if (int rc = check_cache(op, c, true)) return rc;
     if (!a) return bad_value(op, "null argument");
@@ -94,7 +100,7 @@ int disco_op_cache_append(const disco_cache_desc* c, const disco_append_desc* a,
     if (!d_k || !d_v || !d_page_table || !d_lens || !d_cu_new || (a->q_heads && (!d_q || !d_q_out)) || (a->rotated && !d_inv_freq))
         return bad_value(op, "null argument");
     if (a->q_heads && d_q == d_q_out && (a->q_token != a->out_token || a->q_head != a->out_head)) return bad_value(op, "in place with other strides");
-    return launch_cache_append(*c, *a, d_q, d_k, d_v, d_page_table, d_lens, d_cu_new, d_positions, d_inv_freq, d_q_out, (hipStream_t)stream);
+    return launch_cache_append(*c, *a, d_q, d_k, d_v, d_page_table, d_lens, d_cu_new, d_positions, d_inv_freq, d_q_out, d_info, (hipStream_t)stream);
 }
 
 static int check_attention(const char* op, const disco_cache_desc* c, const disco_attention_desc* a) {

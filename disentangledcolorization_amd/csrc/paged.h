@@ -22,7 +22,7 @@ __device__ __host__ __forceinline__ int clamp_len(int len, int capacity) { retur
 
 int launch_rotary(const disco_rotary_desc& d, const void* x, const void* positions, const double* inv_freq, void* out, hipStream_t s);
 int launch_cache_append(const disco_cache_desc& c, const disco_append_desc& a, const void* q, const void* k, const void* v, const int* table,
-                        const int* lens, const int* cu_new, const void* positions, const double* inv_freq, void* q_out, hipStream_t s);
+                        const int* lens, const int* cu_new, const void* positions, const double* inv_freq, void* q_out, const int* info, hipStream_t s);
 
 size_t cache_attention_ws_bytes(const disco_cache_desc& c, const disco_attention_desc& a);
 int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc& a, const void* q, const int* table, const int* lens,

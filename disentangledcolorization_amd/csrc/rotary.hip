@@ -93,7 +93,7 @@ struct RotaryArgs {
     int slices;                                                    // a token's heads are dealt to this many waves
     // append: the cache
     char *ck, *cv;
-    const int *table, *lens, *cu_new;
+    const int *table, *lens, *cu_new, *info;
     long page_stride, head_stride, slot_stride;                    // bytes
     int kv_heads, pages, page_shift, rows, width;
 };
@@ -113,7 +113,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         if (token < first) return;                                 // ahead of the first one
         const int len = clamp_len(a.lens[b], a.width << a.page_shift), p = len - n + (token - first);
         position = p;
-        if (p >= 0 && p < len) {
+        const bool reserved = !a.info || a.info[1] == 0;           // (else the length does not count the new tokens: their places are other tokens')
+        if (reserved && p >= 0 && p < len) {
             const int page = a.table[(long)b * a.width + (p >> a.page_shift)];
             if (page >= 0 && page < a.pages) page_at = page * a.page_stride + (p & ((1 << a.page_shift) - 1)) * a.slot_stride;
         }
@@ -269,13 +270,13 @@ int launch_rotary(const disco_rotary_desc& d, const void* x, const void* positio
 }
 
 int launch_cache_append(const disco_cache_desc& c, const disco_append_desc& d, const void* q, const void* k, const void* v, const int* table,
-                        const int* lens, const int* cu_new, const void* positions, const double* inv_freq, void* q_out, hipStream_t s) {
+                        const int* lens, const int* cu_new, const void* positions, const double* inv_freq, void* q_out, const int* info, hipStream_t s) {
     RotaryArgs a{};
     a.x = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.out = (char*)q_out; a.positions = positions; a.inv_freq = inv_freq;
     a.x_token = d.q_token * 2; a.x_head = d.q_head * 2; a.k_token = d.k_token * 2; a.k_head = d.k_head * 2; a.v_token = d.v_token * 2; a.v_head = d.v_head * 2;
     a.out_token = d.out_token * 2; a.out_head = d.out_head * 2;
     a.gain = (float)d.gain; a.tokens = d.tokens; a.heads = d.q_heads; a.dim = c.dim; a.rotated = d.rotated; a.wide = d.wide_positions;
-    a.ck = (char*)c.d_k; a.cv = (char*)c.d_v; a.table = table; a.lens = lens; a.cu_new = cu_new;
+    a.ck = (char*)c.d_k; a.cv = (char*)c.d_v; a.table = table; a.lens = lens; a.cu_new = cu_new; a.info = info;
     a.page_stride = c.page_stride * 2; a.head_stride = c.head_stride * 2; a.slot_stride = c.slot_stride * 2;
     a.kv_heads = c.kv_heads; a.pages = c.pages; a.page_shift = __builtin_ctz((unsigned)c.page_size); a.rows = c.rows; a.width = c.table_width;
     unsigned long long qs = 0;

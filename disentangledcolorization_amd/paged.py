@@ -8,7 +8,7 @@ it holds, `refs` (pages,) int32 how many rows name a page (0: free).  The new to
 
     inv_freq = rotary_frequencies(128, base=10000.0)
     page_table, lens, refs, info = cache_reserve(page_table, lens, refs, cu_new, page)      # pages for the new tokens
-    q = cache_append(q, k, v, k_cache, v_cache, page_table, lens, cu_new, inv_freq=inv_freq)   # every layer
+    q = cache_append(q, k, v, k_cache, v_cache, page_table, lens, cu_new, inv_freq=inv_freq, info=info)   # every layer
     out = cache_attention(q, k_cache, v_cache, page_table, lens, cu_new)
     page_table, lens, refs, info = cache_select(page_table, lens, parents, k_cache, v_cache)   # fork, reorder, free
     page_table, refs, info = cache_compact(page_table, lens, k_cache, v_cache)
@@ -16,6 +16,10 @@ it holds, `refs` (pages,) int32 how many rows name a page (0: free).  The new to
 Serving only: nothing here is differentiable, and tensors that ask for a gradient are refused (`rotary(inverse=True)` is the transposed
 rotation).  No call synchronises; on the current stream of the tensors' device all of them may be captured into a graph.  No CPU fallback:
 CPU tensors raise DiscoError.
+
+Whether there were pages enough only the GPU knows when a step is under way: info[1] tells, and cache_append, given info, leaves the cache of
+a step that found none as it was (what cache_attention then returns is not the new tokens').  The program looks at info when it suits it, frees pages and does
+the step again.
 """
 import ctypes as C
 import math
@@ -159,10 +163,13 @@ def rotary(x, positions, inv_freq, gain=1.0, interleaved=False, inverse=False, o
     return out
 
 
-def cache_append(q, k, v, k_cache, v_cache, page_table, lens, cu_new, inv_freq=None, gain=1.0, interleaved=False, positions=None, q_out=None):
+def cache_append(q, k, v, k_cache, v_cache, page_table, lens, cu_new, inv_freq=None, gain=1.0, interleaved=False, positions=None, q_out=None, info=None):
     """The new tokens' keys and values are written into their pages, keys (and queries, which are returned) turned by their positions on the
     way.  `lens` counts the new tokens already; `positions` replaces a token's place in its sequence as the angle's position; inv_freq=None turns
-    nothing; q=None has no queries.  q_out may be q."""
+    nothing; q=None has no queries.  q_out may be q.
+
+    info: cache_reserve's.  Where pages were missing nothing is written to the cache: a failed cache_reserve leaves `lens` as it was, and a step that goes on
+    without info writes its tokens over the last cached ones of every sequence, and of those that share their pages."""
     device = _device((k, v, k_cache, v_cache), (page_table, lens, cu_new))
     c = _cache(k_cache, v_cache, page_table)
     _sequences(c, page_table, lens, cu_new)
@@ -175,6 +182,9 @@ def cache_append(q, k, v, k_cache, v_cache, page_table, lens, cu_new, inv_freq=N
     if positions is not None:
         _device((k,), (positions,))
         wide = _positions(positions, tokens)
+    if info is not None:
+        _device((k,), (info,))
+        _ints("info", info, (4,))
     if q is not None:
         _device((k, q))
         q_heads = _three("q", q)[1]
@@ -188,9 +198,9 @@ def cache_append(q, k, v, k_cache, v_cache, page_table, lens, cu_new, inv_freq=N
         raise ValueError("q_out without q")
     if tokens:
         a = _ffi.AppendDesc(tokens, q_heads, rotated, bool(interleaved), wide, *qs, *ks, *vs, *os, gain)
-        _call(device, _ffi.lib().disco_op_cache_append, C.byref(c), C.byref(a), q.data_ptr() if q_heads else None, k.data_ptr(), v.data_ptr(),
+        _call(device, _ffi.lib().disco_op_cache_append_reserved, C.byref(c), C.byref(a), q.data_ptr() if q_heads else None, k.data_ptr(), v.data_ptr(),
               page_table.data_ptr(), lens.data_ptr(), cu_new.data_ptr(), None if positions is None else positions.data_ptr(),
-              None if inv_freq is None else inv_freq.data_ptr(), q_out.data_ptr() if q_heads else None)
+              None if inv_freq is None else inv_freq.data_ptr(), q_out.data_ptr() if q_heads else None, None if info is None else info.data_ptr())
     return q_out
 
 

@@ -478,6 +478,12 @@ typedef struct disco_append_desc {
 int disco_op_cache_append(const disco_cache_desc *c, const disco_append_desc *a, const void *d_q, const void *d_k, const void *d_v,
                           const int32_t *d_page_table, const int32_t *d_lens, const int32_t *d_cu_new, const void *d_positions,
                           const double *d_inv_freq, void *d_q_out, void *stream);
+/* The same behind a disco_op_cache_reserve that may have failed: d_info is what that call wrote (NULL: not looked at).  Where pages were missing
+ * (d_info[1] != 0) no key and no value is written; d_q_out is, as ever.  Without it a failed reserve, which leaves d_lens as it was, makes the last cached
+ * tokens of every sequence the new ones: they are overwritten. */
+int disco_op_cache_append_reserved(const disco_cache_desc *c, const disco_append_desc *a, const void *d_q, const void *d_k, const void *d_v,
+                                   const int32_t *d_page_table, const int32_t *d_lens, const int32_t *d_cu_new, const void *d_positions,
+                                   const double *d_inv_freq, void *d_q_out, const int32_t *d_info, void *stream);
 
 typedef struct disco_attention_desc {
     int32_t tokens, q_heads;                   /* q_heads a multiple of kv_heads (at most 1024): query head h reads key head h / (q_heads / kv_heads);

@@ -573,6 +573,63 @@ def test_rows_before_the_first_sequence_are_not_appended():
         assert torch.equal(a.nan_to_num(9), b.nan_to_num(9))
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_append_behind_a_failed_reserve(captured):
+    """Pages are missing: the step's append leaves the cache as it is, bit for bit, also pages that rows share; with enough of them it appends."""
+    page, f = 16, paged.rotary_frequencies(64)
+    s = Served([60, 60, 30], [0, 0, 0], 2, 1, 64, page, BF, seed=2, spare=2)
+    s.table[1, :3] = s.table[0, :3]                       # a fork: three full pages shared, a last page each
+    refs = torch.zeros(s.pool, dtype=torch.int32, device=DEV)
+    for b, u in enumerate(s.used):
+        refs[s.table[b, :u].long()] += 1
+    refs[refs == 0] = -1
+    free = (refs == -1).nonzero()[:3, 0]
+    refs[free] = 0
+    cu, qkv = ints([0, 1, 10, 20]), torch.randn(20, 6, 64, generator=gen(3)).to(BF).to(DEV)
+    q, k, v = qkv.split([2, 2, 2], 1)
+    table = torch.cat((s.table, torch.full((3, 2), -1, dtype=torch.int32, device=DEV)), 1).contiguous()
+    kc, vc = s.k.clone(), s.v.clone()
+
+    def step():
+        t, n, r, info = paged.cache_reserve(table, s.lens, refs, cu, page)
+        out = paged.cache_append(q, k, v, kc, vc, t, n, cu, inv_freq=f, info=info)
+        return t, n, r, info, out, paged.cache_attention(out, kc, vc, t, n, cu)
+
+    if captured:
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            step()
+        torch.cuda.current_stream().wait_stream(stream)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+    for some in (3, 0, 1, 2, 3):                          # free pages; two are needed: the second row's ten tokens and the third's
+        refs[free] = -1
+        refs[free[:some]] = 0
+        kc.copy_(s.k)
+        vc.copy_(s.v)
+        if captured:
+            graph.replay()
+            torch.cuda.synchronize()
+        else:
+            outs = step()
+        t, n, r, info, out, _ = outs
+        assert info.tolist() == ([some - 2, 0, 0, 0] if some >= 2 else [some, 2 - some, 0, 0])
+        pos = (n - (cu[1:] - cu[:-1])).repeat_interleave(cu[1:] - cu[:-1]) + torch.cat([torch.arange(int(m), device=DEV) for m in cu[1:] - cu[:-1]])
+        close_turned(out, q, pos, f, 1.0, False)
+        if some < 2:
+            assert torch.equal(kc.nan_to_num(9), s.k.nan_to_num(9)) and torch.equal(vc.nan_to_num(9), s.v.nan_to_num(9))
+        else:
+            want_k, want_v = s.k.clone(), s.v.clone()
+            paged.cache_append(q, k, v, want_k, want_v, t, n, cu, inv_freq=f)
+            assert not torch.equal(kc.nan_to_num(9), s.k.nan_to_num(9))
+            assert torch.equal(kc.nan_to_num(9), want_k.nan_to_num(9)) and torch.equal(vc.nan_to_num(9), want_v.nan_to_num(9))
+    for bad in (info[:3], info.long(), torch.zeros(8, dtype=torch.int32, device=DEV)[::2]):
+        with pytest.raises(ValueError, match="info"):
+            paged.cache_append(q, k, v, kc, vc, t, n, cu, info=bad)
+
+
 # ---- pages --------------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("rows,pages,page,width", [(1, 3, 16, 4), (5, 40, 8, 9), (70, 3000, 1, 64), (1100, 9000, 16, 16), (3, 70000, 4, 1000), (9, 64, 16, 8), (16384, 20000, 16, 2)])

@@ -164,6 +164,18 @@ def test_bad_appends_are_refused(lib, kw):
     assert lib.disco_op_cache_append(C.byref(c), C.byref(a), p, p, p, p, p, p, None, p, p, None) in (-1, -2)
 
 
+@pytest.mark.parametrize("kw", [dict(tokens=-1), dict(q_heads=-1), dict(rotated=5), dict(k_token=1 << 60)])
+def test_bad_appends_behind_a_reserve_are_refused(lib, kw):
+    """With and without the reserve's info the same checks."""
+    d = dict(tokens=4, q_heads=4, rotated=64, interleaved=0, wide_positions=0, q_token=256, q_head=64, k_token=128, k_head=64, v_token=128, v_head=64,
+             out_token=256, out_head=64, gain=1.0)
+    d.update(kw)
+    a, c, p = _ffi.AppendDesc(*[d[f] for f, _ in _ffi.AppendDesc._fields_]), cache(), C.c_void_p(1 << 20)
+    for info in (None, p):
+        assert lib.disco_op_cache_append_reserved(C.byref(c), C.byref(a), p, p, p, p, p, p, None, p, p, info, None) in (-1, -2)
+        assert lib.disco_op_cache_append_reserved(None, C.byref(a), p, p, p, p, p, p, None, p, p, info, None) == -1
+
+
 def test_cpu_tensors_are_refused():
     t = torch.zeros(2, 2, 64)
     with pytest.raises(_ffi.DiscoError, match="no CPU fallback"):
