@@ -36,6 +36,13 @@ int check_cache(const char* op, const disco_cache_desc* c, bool one_layer) {
     return DISCO_OK;
 }
 
+// what copies pages: a head of a page is counted in 16-byte pieces
+int check_copied_cache(const char* op, const disco_cache_desc* c) {
+    if (int rc = check_cache(op, c, false)) return rc;
+    if ((int64_t)c->page_size * (c->dim / 8) > 0x7fffffff) return bad_shape(op, "a head of a page of more than 2^31 pieces of 16 bytes");
+    return DISCO_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -155,7 +162,7 @@ int disco_op_cache_select(const disco_cache_desc* c, const int32_t* d_page_table
                           int32_t* d_page_table_out, int32_t* d_lens_out, int32_t* d_refs_out, int32_t* d_info, void* d_ws, size_t ws_bytes,
                           void* stream) {
     const char* op = "cache_select";
-    if (int rc = check_cache(op, c, false)) return rc;
+    if (int rc = check_copied_cache(op, c)) return rc;
     if (!d_page_table || !d_lens || !d_parents || !d_page_table_out || !d_lens_out || !d_refs_out || !d_info || !d_ws) return bad_value(op, "null argument");
     if (d_page_table == d_page_table_out || d_lens == d_lens_out) return bad_value(op, "the new state needs buffers of its own");
     if (ws_bytes < cache_pages_ws_bytes(c->rows, c->pages) || (uintptr_t)d_ws % 16) { set_error("%s: workspace too small or not aligned", op); return DISCO_ENOMEM; }
@@ -165,7 +172,7 @@ int disco_op_cache_select(const disco_cache_desc* c, const int32_t* d_page_table
 int disco_op_cache_compact(const disco_cache_desc* c, const int32_t* d_page_table, const int32_t* d_lens, int32_t* d_page_table_out,
                            int32_t* d_refs_out, int32_t* d_info, void* d_ws, size_t ws_bytes, void* stream) {
     const char* op = "cache_compact";
-    if (int rc = check_cache(op, c, false)) return rc;
+    if (int rc = check_copied_cache(op, c)) return rc;
     if (!d_page_table || !d_lens || !d_page_table_out || !d_refs_out || !d_info || !d_ws) return bad_value(op, "null argument");
     if (d_page_table == d_page_table_out) return bad_value(op, "the new table needs a buffer of its own");
     if (ws_bytes < cache_pages_ws_bytes(c->rows, c->pages) || (uintptr_t)d_ws % 16) { set_error("%s: workspace too small or not aligned", op); return DISCO_ENOMEM; }
@@ -174,7 +181,7 @@ int disco_op_cache_compact(const disco_cache_desc* c, const int32_t* d_page_tabl
 
 int disco_op_cache_copy_pages(const disco_cache_desc* c, const int32_t* d_src, const int32_t* d_dst, int count, void* stream) {
     const char* op = "cache_copy_pages";
-    if (int rc = check_cache(op, c, false)) return rc;
+    if (int rc = check_copied_cache(op, c)) return rc;
     if (count < 0) return bad_shape(op, "negative count");
     if (!count) return DISCO_OK;
     if (!d_src || !d_dst) return bad_value(op, "null argument");

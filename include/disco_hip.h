@@ -437,7 +437,7 @@ int disco_op_mark_color_hints(const float *d_gray, const float *d_target_ab, con
 typedef struct disco_cache_desc {
     int32_t dtype;                             /* DISCO_F16 / DISCO_BF16 */
     int32_t layers;                            /* layers that share the page table; append and attention use the first */
-    int32_t pages, kv_heads, page_size, dim;   /* page_size: a power of two; dim: a multiple of 8, 8 .. 256 */
+    int32_t pages, kv_heads, page_size, dim;   /* page_size: a power of two (where pages are copied page_size * dim / 8 < 2^31); dim: a multiple of 8, 8 .. 256 */
     int32_t rows, table_width;                 /* of the page table; table_width * page_size <= 2^30 */
     int64_t layer_stride, page_stride, head_stride, slot_stride;   /* multiples of 8; d_k and d_v aligned to 16 bytes */
     void *d_k, *d_v;

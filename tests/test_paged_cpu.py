@@ -80,6 +80,19 @@ def test_bad_caches_are_refused(lib, kw):
         assert rc in (-1, -2) and lib.disco_last_error().startswith(b"cache_"), (rc, lib.disco_last_error())
 
 
+def test_pages_whose_pieces_an_int_does_not_count_are_refused(lib):
+    """A head of a page is copied in pieces of 16 bytes, counted in 32 bits: where they do not fit nothing may be reported as copied."""
+    p, o = C.c_void_p(1 << 20), C.c_void_p(2 << 20)
+    need = lib.disco_op_cache_pages_workspace_bytes(2, 8)
+    for page_size, dim in ((1 << 26, 256), (1 << 28, 64), (1 << 30, 16)):
+        c = cache(page_size=page_size, dim=dim, table_width=1)
+        for rc in (lib.disco_op_cache_select(C.byref(c), p, p, p, o, o, o, o, p, need, None), lib.disco_op_cache_compact(C.byref(c), p, p, o, o, o, p, need, None),
+                   lib.disco_op_cache_copy_pages(C.byref(c), p, p, 1, None)):
+            assert rc == -2 and b"pieces" in lib.disco_last_error()
+    c = cache(page_size=1 << 25, dim=256, table_width=1)      # (just below: as far as the workspace's check)
+    assert lib.disco_op_cache_select(C.byref(c), p, p, p, o, o, o, o, p, 0, None) == -6
+
+
 @pytest.mark.parametrize("kw", [dict(tokens=-1), dict(q_heads=0), dict(q_heads=3), dict(window=-1), dict(window=4, causal=0), dict(max_new=-1), dict(max_len=-1),
                                 dict(scale=math.nan), dict(scale=math.inf), dict(q_token=4), dict(out_head=1 << 60), dict(tokens=1 << 30)])
 def test_bad_attention_is_refused(lib, kw):
