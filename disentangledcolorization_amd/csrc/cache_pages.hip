@@ -104,7 +104,7 @@ __device__ __forceinline__ int reserve_new(const ReserveArgs& a, int r) {
 
 __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
     extern __shared__ int upto[];                                  // [rows]: pages that the rows up to and with this one need
-    __shared__ int part[WAVES], bad;
+    __shared__ int part[WAVES], bad, shared;
     __shared__ unsigned long long over;                            // pages beyond the table's width
     const int capacity = a.width << a.shift;
     if (blockIdx.x) {
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
         }
         return;
     }
-    if (threadIdx.x == 0) { over = 0; bad = 0; }
+    if (threadIdx.x == 0) { over = 0; bad = 0; shared = 0; }
     __syncthreads();                                               // (every wave counts into them)
     int base = 0;
     for (int r0 = 0; r0 < a.rows; r0 += PLAN) {
@@ -130,6 +130,10 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
             if (want > a.width) atomicAdd(&over, (unsigned long long)(want - a.width));
             else need = (int)want - have;
             if (len != a.lens[r] || a.cu_new[r + 1] < a.cu_new[r]) atomicAdd(&bad, 1);
+            if (len & ((1 << a.shift) - 1) && reserve_new(a, r)) { // the first new token goes into a page that is there: no other row may name it
+                const int page = a.table[(long)r * a.width + (len >> a.shift)];
+                if (page >= 0 && page < a.pages && a.refs[page] > 1) atomicAdd(&shared, 1);
+            }
         }
         const int incl = block_scan(need, part, &all) + base;
         if (r < a.rows) upto[r] = incl;
@@ -137,7 +141,7 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
     }
     __syncthreads();
     const int total = base;
-    const unsigned long long too_long = over;
+    const unsigned long long short_of = over + shared;
     bool done = false;
     const int free_pages = scan_pages(a.pages, part,
         [&](int p) {
@@ -145,7 +149,7 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
             a.refs_out[p] = refs;
             return refs == 0;
         },
-        [&](int free) { done = total <= free && too_long == 0; },
+        [&](int free) { done = total <= free && short_of == 0; },
         [&](int page, bool free, int rank) {
             if (!free || !done || rank >= total) return;
             int lo = 0, hi = a.rows - 1;                           // the first row with upto > rank
@@ -168,10 +172,10 @@ __global__ __launch_bounds__(PLAN) void cache_reserve_kernel(ReserveArgs a) {
     }
     if (threadIdx.x == 0) {
         a.info[0] = done ? free_pages - total : free_pages;
-        const unsigned long long missing = max(total - free_pages, 0) + too_long;
+        const unsigned long long missing = max(total - free_pages, 0) + short_of;
         a.info[1] = done ? 0 : (int)(missing < 0x7fffffff ? missing : 0x7fffffff);
         a.info[2] = bad;
-        a.info[3] = 0;
+        a.info[3] = shared;
     }
 }
 
@@ -207,6 +211,7 @@ template <bool LOCAL> struct Counts {
     int* at;
     __device__ __forceinline__ int get(int p) const { return LOCAL ? at[p] : count_now(at + p); }
     __device__ __forceinline__ void add(int p) const { atomicAdd(at + p, 1); }
+    __device__ __forceinline__ void lower(int p, int n) const { atomicMin(at + p, n); }
     __device__ __forceinline__ void set(int p, int n) const {
         if (LOCAL) at[p] = n;
         else __hip_atomic_store(at + p, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -269,16 +274,29 @@ __global__ __launch_bounds__(PLAN) void cache_select_plan_kernel(PlanArgs a) {
         if (p >= 0) atomicMin(&keeper[p], p == r ? -1 : r);
     }
     __syncthreads();
-    // last pages that are not full: the keeper's is in use, the others need copies, numbered by row
+    // Last pages that are not full.  The rows that end in one ask for it, below 0 in its count; a row that is its own parent goes first, then the lowest.
+    // A page that is full for some row (whose neighbours have been cut back into it) has a count and stays that row's: all that end in it need copies.
+    auto asked = [&](int r, int p) { return (p == r ? r : a.rows + r) - (1 << 30); };
+    for (int r = tid; r < a.rows; r += PLAN) {
+        const int p = parent_of(a, r), len = p < 0 ? 0 : clamp_len(a.lens[p], capacity);
+        if (!(len & ((1 << a.shift) - 1))) continue;
+        const int page = a.table_out[(long)r * a.width + (len >> a.shift)];
+        if (page >= 0 && page < a.pages && counts.get(page) <= 0) counts.lower(page, asked(r, p));
+    }
+    settle();
+    // the keeper's is in use, the others need copies, numbered by row
     int need = 0;
     for (int r0 = 0; r0 < a.rows; r0 += PLAN) {
         const int r = r0 + tid, p = r < a.rows ? parent_of(a, r) : -1;
         const int len = p < 0 ? 0 : clamp_len(a.lens[p], capacity), filled = len & ((1 << a.shift) - 1);
-        const bool keeps = p >= 0 && keeper[p] == (p == r ? -1 : r);
+        bool keeps = p >= 0 && keeper[p] == (p == r ? -1 : r);     // (of a page outside the cache)
         int page = -1, all;
         if (filled) {
             page = a.table_out[(long)r * a.width + (len >> a.shift)];
-            if (keeps && page >= 0 && page < a.pages) counts.add(page);
+            if (page >= 0 && page < a.pages) {
+                keeps = counts.get(page) == asked(r, p);           // (who finds 1 there comes behind the keeper)
+                if (keeps) counts.set(page, 1);
+            }
         }
         const bool asks = filled && !keeps;
         const int rank = need + block_scan(asks, part, &all) - 1;

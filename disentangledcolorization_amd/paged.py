@@ -246,7 +246,11 @@ def _state(page_table, rows, width, pages):
 
 def cache_reserve(page_table, lens, refs, cu_new, page):
     """Pages for the new tokens of every row: (page_table, lens, refs, info) with them.  The lowest free pages are taken, rows ascending.
-    info (4,) int32: free pages afterwards; pages that were missing - then the state returned is the old one -; lengths out of range; 0."""
+    info (4,) int32: free pages afterwards; pages that were missing - then the state returned is the old one -; lengths out of range; rows whose new
+    tokens would go into a page that other rows name as well, each of which counts as a missing page.
+
+    A row is cut back by a smaller length, as for drafted tokens that were rejected.  Where that leaves it inside a page which it shares, or for the pages behind
+    its new end to become free, cache_select with every row its own parent comes first."""
     device = _device((page_table,), (lens, refs, cu_new))
     if page_table.dim() != 2 or refs.dim() != 1:
         raise ValueError("page_table must be (rows, width), refs (pages,)")
@@ -273,7 +277,8 @@ def _page_call(k_cache, v_cache, page_table, lens):
 
 def cache_select(page_table, lens, parents, k_cache, v_cache):
     """Row r becomes what row parents[r] was, -1: empty; forks, reorders and frees rows in one call: (page_table, lens, refs, info).  Rows of one
-    parent share its full pages; of a last page that is not full one row keeps the original and the others get copies, in all layers.
+    parent share its full pages; of a last page that is not full one row keeps the original and the others get copies, in all layers, also where
+    it was a full page before its rows were cut back; and all get copies where it still is one for another row.
     info (4,) int32: free pages afterwards; pages that were missing - then the state returned is the old one -; entries out of range; pages copied."""
     device = _device((k_cache, v_cache), (page_table, lens, parents))
     c, ws, need = _page_call(k_cache, v_cache, page_table, lens)

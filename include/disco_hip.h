@@ -505,12 +505,16 @@ int disco_op_cache_attention(const disco_cache_desc *c, const disco_attention_de
 /* Page calls: from a table, lengths and counts to new ones (other buffers than the old ones); entries behind a row's last page become -1.
  * d_refs[pages]: how many rows name a page, 0 = free.  d_info[4]: free pages afterwards; pages that were missing (then nothing has changed: the new
  * state is the old one); entries or lengths out of range; pages copied.  rows <= 16384. */
-/* Pages for the new tokens of every row (d_lens: without them, d_lens_out: with them), the lowest free numbers first, rows ascending. */
+/* Pages for the new tokens of every row (d_lens: without them, d_lens_out: with them), the lowest free numbers first, rows ascending.  A row may be cut back
+ * (its length lowered), but new tokens do not go into a page that other rows name as well (d_refs above 1): d_info[3] counts the rows that ask for that, each
+ * counts as a missing page, and disco_op_cache_select with every row its own parent makes the pages theirs.  The pages that a row no longer
+ * reaches leave the table; d_refs does not hear of it before select or compact count anew. */
 int disco_op_cache_reserve(int rows, int table_width, int pages, int page_size, const int32_t *d_page_table, const int32_t *d_lens,
                            const int32_t *d_refs, const int32_t *d_cu_new, int32_t *d_page_table_out, int32_t *d_lens_out, int32_t *d_refs_out,
                            int32_t *d_info, void *stream);
 /* Row r becomes what row d_parents[r] was (-1: empty).  Rows of one parent share its full pages; of a last page that is not full one of them keeps
- * the original (the parent itself, else the lowest) and the others get a copy of its filled slots, in all layers: new tokens never meet in a page. */
+ * the original (the parent itself, else the lowest) and the others get a copy of its filled slots, in all layers; so do the rows that have been cut back into
+ * one page, and all that end in a page which is full for another row: new tokens never meet in a page. */
 int disco_op_cache_select(const disco_cache_desc *c, const int32_t *d_page_table, const int32_t *d_lens, const int32_t *d_parents,
                           int32_t *d_page_table_out, int32_t *d_lens_out, int32_t *d_refs_out, int32_t *d_info, void *d_ws, size_t ws_bytes,
                           void *stream);

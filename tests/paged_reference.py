@@ -109,6 +109,41 @@ def selected(table, lens, parents, ps, pages):
     return [row + [-1] * (width - len(row)) for row in new], new_lens, refs, [refs.count(0), 0, len(copies)], copies
 
 
+def selected_by_page(table, lens, parents, ps, pages):
+    """The same for rows of any lengths whose pages (all of them inside the cache) may be shared in any way: of the rows that end inside a page one keeps it - a row
+    that is its own parent, else the lowest - unless it is a full page of some row."""
+    width = len(table[0])
+    new_lens = [lens[p] if p >= 0 else 0 for p in parents]
+    new = [(table[p][:-(-lens[p] // ps)] if p >= 0 else []) for p in parents]
+    full = {page for row, n in zip(new, new_lens) for page in row[:n // ps]}
+    ends = {}
+    for r in sorted(range(len(parents)), key=lambda r: (parents[r] != r, r)):
+        if new_lens[r] % ps:
+            ends.setdefault(new[r][-1], []).append(r)
+    need = sorted(r for page, rows in ends.items() for r in (rows if page in full else rows[1:]))
+
+    def count(rows):
+        refs = [0] * pages
+        for row in rows:
+            for p in row:
+                refs[p] += 1
+        return refs
+
+    needs = set(need)
+    refs = count([row[:-1] if r in needs else row for r, row in enumerate(new)])
+    free = [p for p in range(pages) if refs[p] == 0]
+    if len(need) > len(free):
+        held = [row[:-(-n // ps)] for row, n in zip(table, lens)]
+        refs = count(held)
+        return [row + [-1] * (width - len(row)) for row in held], list(lens), refs, [refs.count(0), len(need) - len(free), 0], []
+    copies = []
+    for r, page in zip(need, free):
+        copies.append((new[r][-1], page, new_lens[r] % ps))
+        new[r] = new[r][:-1] + [page]
+        refs[page] = 1
+    return [row + [-1] * (width - len(row)) for row in new], new_lens, refs, [refs.count(0), 0, len(copies)], copies
+
+
 def compacted(table, lens, ps, pages):
     """cache_compact on lists: (table, refs, [free, moved], moves [(src, dst)])."""
     width = len(table[0])

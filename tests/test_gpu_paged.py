@@ -726,6 +726,67 @@ def test_select(rows, page, layers, kv_heads, dim, spare):
             assert torch.equal(new, old)
 
 
+@pytest.mark.parametrize("rows,page,spare", [(2, 16, 3), (7, 8, 30), (60, 4, 200), (60, 16, 2), (1200, 4, 3000), (5000, 2, 9000), (30, 16, 70000)])
+def test_select_of_rows_that_were_cut_back(rows, page, spare):
+    """Rows of different parents that share a page which a shortened length has made a last page that is not full, for one of them or for several: no two rows may
+    end inside the same page, nor inside one that another row has full."""
+    g = gen(rows + page)
+    lens, table, count = fork_state(rows, page, rows)
+    lens = [n if b % 3 == 0 else max(0, n - int(torch.randint(0, 2 * page + 1, (1,), generator=g))) for b, n in enumerate(lens)]
+    pages, width = count + spare, max(max(map(len, table)), 1) + 1
+    place = torch.randperm(pages, generator=g).tolist()
+    table = [[place[p] for p in row] + [-5] * (width - len(row)) for row in table]
+    k, v = (torch.randn(1, pages, 1, page, 8, generator=g).half().to(DEV) for _ in range(2))
+    identity = list(range(rows))
+    for parents in (identity, [int(x) for x in torch.randint(-1, rows, (rows,), generator=g)], identity[::-1], [0] * rows):
+        want = R.selected_by_page([row[:] for row in table], lens, parents, page, pages)
+        kk, vv = k.clone(), v.clone()
+        got = paged.cache_select(ints(table), ints(lens), ints(parents), kk, vv)
+        assert got[0].tolist() == want[0] and got[1].tolist() == want[1] and got[2].tolist() == want[2]
+        free, missing, copied = want[3]
+        assert got[3].tolist() == [free, missing, 0, copied]
+        for new, old in ((kk, k), (vv, v)):
+            old = old.cpu().clone()
+            for src, dst, slots in want[4]:
+                old[:, dst, :, :slots] = old[:, src, :, :slots]
+            assert torch.equal(new.cpu(), old)
+        if not missing:                                   # a new token of every row, and no two of them in one place
+            got = paged.cache_reserve(got[0], got[1], got[2], ints(list(range(rows + 1))), page)
+            info = got[3].tolist()
+            assert info[3] == 0
+            if info[1] == 0:
+                at = [(row[(n - 1) // page], (n - 1) % page) for row, n in zip(got[0].tolist(), got[1].tolist())]
+                assert len(set(at)) == rows and (got[2][[p for p, _ in at]] == 1).all()
+
+
+def test_reserve_refuses_new_tokens_in_shared_pages():
+    """Rows 0 and 1 share a full page and row 1 is cut back into it; rows 3 and 4 end in the same page.  Nothing is taken, the two that may not write are counted
+    (of 3 and 4 only row 4 has new tokens), cache_select makes the pages their own, and the step goes through."""
+    page, f = 16, paged.rotary_frequencies(8)
+    table, lens = ints([[0, 1, -1], [0, -1, -1], [2, -1, -1], [3, -1, -1], [3, -1, -1]]), ints([20, 10, 5, 9, 7])
+    refs = ints([2, 1, 1, 2, 0, 0, 0])
+    k = torch.randn(7, 1, page, 8, generator=gen(1)).half().to(DEV)
+    v, cu = -k, ints([0, 1, 2, 3, 3, 5])
+    got = paged.cache_reserve(table, lens, refs, cu, page)
+    assert got[3].tolist() == [3, 2, 0, 2]
+    assert torch.equal(got[0], table) and torch.equal(got[1], lens) and torch.equal(got[2], refs)
+    x = torch.randn(5, 1, 8, generator=gen(2)).half().to(DEV)
+    kc, vc = k.clone(), v.clone()
+    paged.cache_append(None, x, x, kc, vc, got[0], got[1], cu, inv_freq=f, info=got[3])
+    assert torch.equal(kc, k) and torch.equal(vc, v)
+    t, n, r, info = paged.cache_select(table, lens, ints([0, 1, 2, 3, 4]), k, v)
+    assert info.tolist() == [1, 0, 0, 2] and t[:, 0].tolist() == [0, 4, 2, 3, 5] and torch.equal(n, lens)
+    assert torch.equal(k[4, :, :10], k[0, :, :10]) and torch.equal(v[5, :, :7], v[3, :, :7])
+    got = paged.cache_reserve(t, n, r, cu, page)
+    assert got[3].tolist() == [1, 0, 0, 0] and got[1].tolist() == [21, 11, 6, 9, 9]
+    before, s = k.clone(), n.tolist()
+    paged.cache_append(None, x, x, k, v, got[0], got[1], cu, inv_freq=f, info=got[3])
+    for b, row in enumerate(got[0].tolist()):             # what the rows held is still there
+        for p in range(s[b]):
+            assert torch.equal(k[row[p // page], 0, p % page], before[row[p // page], 0, p % page])
+    assert all(torch.equal(v[row, 0, at], x[i, 0]) for i, (row, at) in enumerate([(1, 4), (4, 10), (2, 5), (5, 7), (5, 8)]))
+
+
 def test_select_counts_what_is_out_of_range():
     """Parents that are no rows are empty rows; page numbers outside the cache are passed on, never followed; lengths are cut."""
     k = torch.zeros(4, 1, 16, 8, dtype=BF, device=DEV)
