@@ -70,13 +70,15 @@ def _call(device, fn, *args):
 
 def _cache(k, v, page_table, layered=False):
     dims = 5 if layered and k.dim() == 5 else 4
-    shape, st = k.shape, k.stride()
-    if len(shape) != dims or v.shape != shape or v.dtype is not k.dtype or v.stride() != st:
+    shape, st, other = k.shape, k.stride(), v.stride()
+    if 1 in shape and v.shape == shape:                   # (the stride of an axis of one does not matter)
+        st, other = (tuple(s if n > 1 else 0 for n, s in zip(shape, x)) for x in (st, other))
+    if len(shape) != dims or v.shape != shape or v.dtype is not k.dtype or other != st:
         raise ValueError("k_cache and v_cache must be alike, (%spages, kv_heads, page, dim)" % ("[layers,] " if layered else ""))
     dtype = _DTYPES.get(k.dtype, _ffi.F32)
     if dtype == _ffi.F32:
         raise ValueError("the cache holds fp16 or bf16, got %s" % k.dtype)
-    if st[-1] != 1:
+    if st[-1] != 1 and shape[-1] > 1:
         raise ValueError("the elements of a head must lie next to each other")
     if page_table.dim() != 2:
         raise ValueError("page_table must be (rows, width)")

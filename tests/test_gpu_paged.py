@@ -108,6 +108,20 @@ def test_an_axis_of_one_has_any_stride():
     assert torch.equal(out, paged.cache_attention(s.q, *s.args()))
 
 
+def test_a_cache_axis_of_one_has_any_stride():
+    s = Served([50], [3], 1, 4, 64, 16, BF)
+    want = paged.cache_attention(s.q, *s.args())
+    k = torch.empty(s.pool, 3, 16, 64, dtype=BF, device=DEV)[:, 1:2]
+    v = torch.empty(s.pool, 16, 3, 64, dtype=BF, device=DEV).transpose(1, 2)[:, :1]
+    assert k.stride() != v.stride()
+    k.copy_(s.k)
+    with pytest.raises(ValueError, match="alike"):
+        paged.cache_attention(s.q, k, v, *s.args()[2:])
+    v = k.new_empty(s.pool, 3, 16, 64)[:, 1:2].as_strided(k.shape, (k.stride(0), 7, 64, 1))
+    v.copy_(s.v)
+    assert torch.equal(paged.cache_attention(s.q, k, v, *s.args()[2:]), want)
+
+
 def test_rotary_there_and_back():
     """inverse is the transposed rotation: <y, rot(x)> = <rot'(y), x>, and without a gain it undoes the rotation."""
     x, y = (torch.randn(50, 3, 48, generator=gen(s)).to(DEV) for s in (1, 2))

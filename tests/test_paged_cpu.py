@@ -126,6 +126,21 @@ def test_sizes_that_an_int32_does_not_hold_are_refused():
     assert [paged._bound(n) for n in (-far, -1, 0, 7, far)] == [-1, -1, 0, 7, (1 << 31) - 1]
 
 
+@pytest.mark.parametrize("shape", [(1, 2, 16, 8), (4, 1, 16, 8), (4, 2, 1, 8), (1, 1, 1, 8), (1, 4, 2, 16, 8), (3, 1, 1, 4, 8)])
+def test_the_stride_of_a_cache_axis_of_one_does_not_matter(shape):
+    """Keys and values cut from different places are alike where the axes that have a stride have the same."""
+    strides = torch.empty(shape, device="meta").stride()
+    views = [torch.empty(1 << 14, device="meta", dtype=torch.bfloat16).as_strided(shape, tuple(st if n > 1 else odd for n, st in zip(shape, strides))) for odd in (5, 129)]
+    table = torch.empty(2, 2, device="meta", dtype=torch.int32)
+    c = paged._cache(*views, table, layered=len(shape) == 5)
+    got = [c.layer_stride, c.page_stride, c.head_stride, c.slot_stride][-len(shape) + 1:]
+    assert got == [st if n > 1 else 0 for n, st in zip(shape[:-1], strides)]
+    other = torch.empty(1 << 14, device="meta", dtype=torch.bfloat16).as_strided(shape, tuple(2 * st if n > 1 else st for n, st in zip(shape[:-1], strides)) + (1,))
+    if any(n > 1 for n in shape[:-1]):
+        with pytest.raises(ValueError, match="alike"):
+            paged._cache(views[0], other, table, layered=len(shape) == 5)
+
+
 def test_missing_arguments_and_workspaces_are_refused(lib):
     c, p, o = cache(), C.c_void_p(1 << 20), C.c_void_p(2 << 20)
     a = _ffi.AttentionDesc(4, 4, 1, 0, 0, 0, 0.125, 256, 64, 256, 64)
