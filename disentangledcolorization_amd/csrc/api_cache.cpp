@@ -142,6 +142,7 @@ int disco_op_cache_attention(const disco_cache_desc* c, const disco_attention_de
     if (((uintptr_t)d_q | (uintptr_t)d_out) % 16) return bad_value(op, "q and out must be aligned to 16 bytes");
     const size_t need = cache_attention_ws_bytes(*c, *a);
     if (need && (!d_ws || ws_bytes < need || (uintptr_t)d_ws % 16)) { set_error("%s: workspace too small or not aligned (%zu < %zu)", op, ws_bytes, need); return DISCO_ENOMEM; }
+    if (d_q == d_out) return bad_value(op, "out may not be q");
     return launch_cache_attention(*c, *a, d_q, d_page_table, d_lens, d_cu_new, d_out, d_lse, d_ws, (hipStream_t)stream);
 }
 

@@ -126,6 +126,14 @@ def test_sizes_that_an_int32_does_not_hold_are_refused():
     assert [paged._bound(n) for n in (-far, -1, 0, 7, far)] == [-1, -1, 0, 7, (1 << 31) - 1]
 
 
+def test_attention_in_place_is_refused(lib):
+    """Queries are read again where a result is not finite: they must still be there."""
+    c, p, o = cache(), C.c_void_p(1 << 20), C.c_void_p(2 << 20)
+    a = _ffi.AttentionDesc(4, 4, 1, 0, 0, 0, 0.125, 256, 64, 256, 64)
+    assert lib.disco_op_cache_attention(C.byref(c), C.byref(a), p, p, p, p, p, None, p, 1 << 40, None) == -1
+    assert b"may not be q" in lib.disco_last_error()
+
+
 @pytest.mark.parametrize("shape", [(1, 2, 16, 8), (4, 1, 16, 8), (4, 2, 1, 8), (1, 1, 1, 8), (1, 4, 2, 16, 8), (3, 1, 1, 4, 8)])
 def test_the_stride_of_a_cache_axis_of_one_does_not_matter(shape):
     """Keys and values cut from different places are alike where the axes that have a stride have the same."""
