@@ -813,7 +813,7 @@ __device__ __forceinline__ void put_joined(const AttnArgs& a, const Joined& j, i
 template <typename T>
 __global__ __launch_bounds__(256) void cache_attention_join_kernel(AttnArgs a, int waves_a_token) {
     const int lane = threadIdx.x & 63, quads = a.dim / 4, at_once = 64 / quads;
-    const int wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = wave / waves_a_token;
+    const int wave = (int)block_of() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = wave / waves_a_token;
     if (t >= a.tokens) return;
     const Joined j = joined_of(a, t);
     const int h = (wave - t * waves_a_token) * at_once + lane / quads, d = lane % quads * 4;
@@ -967,7 +967,7 @@ int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
         if ((p.few_splits > 8 || p.many_splits > 8) && rows <= 2048) cache_attention_join_row_kernel<T><<<(unsigned)rows, 256, 0, s>>>(a);
         else {
             const int waves_a_token = cdiv(a.q_heads, 256 / a.dim);
-            cache_attention_join_kernel<T><<<(unsigned)(((long)a.tokens * waves_a_token + 3) / 4), 256, 0, s>>>(a, waves_a_token);
+            cache_attention_join_kernel<T><<<grid_of(((long)a.tokens * waves_a_token + 3) / 4), 256, 0, s>>>(a, waves_a_token);
         }
         DISCO_LAUNCH_CHECK("cache_attention_join_kernel");
     }

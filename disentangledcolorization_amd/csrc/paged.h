@@ -17,6 +17,13 @@ __device__ __forceinline__ int seq_of_token(const int* __restrict__ cu_new, int 
     return b;
 }
 
+// A grid of any number of workgroups: a launch has fewer than 2^32 threads along an axis.  block_of() counts them; the last ones may lie behind the end.
+inline dim3 grid_of(long blocks) {
+    constexpr long AXIS = 1 << 22;
+    return blocks <= AXIS ? dim3((unsigned)blocks) : dim3((unsigned)AXIS, (unsigned)((blocks + AXIS - 1) / AXIS));
+}
+__device__ __forceinline__ long block_of() { return (long)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // a length as the kernels use it: never beyond what the row of the page table can name
 __device__ __host__ __forceinline__ int clamp_len(int len, int capacity) { return len < 0 ? 0 : (len < capacity ? len : capacity); }
 

@@ -101,7 +101,7 @@ struct RotaryArgs {
 // APPEND: the wave's heads are the queries' (to out), the keys' and the values' (to their page); else the heads of x
 template <typename T, int V, int MODE, bool INTER, bool APPEND>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
-    const int wave = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wave = (int)block_of() * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;       // (below 2^31: 2^30 tokens, or 2^9 of 2^17 heads)
     const int token = wave / a.slices, slice = wave - token * a.slices;
     if (token >= a.tokens) return;
     long page_at = -1;                                             // where the token's slot lies in a cache, bytes
@@ -233,7 +233,7 @@ int run_rotary(RotaryArgs& a, bool inter, hipStream_t s) {
     a.slices = 1;
     while (a.slices * 2 <= passes && (long)a.tokens * a.slices < 4096) a.slices *= 2;
     if (a.tokens < 512) a.slices = passes;
-    const dim3 grid((unsigned)(((long)a.tokens * a.slices + 3) / 4));
+    const dim3 grid = grid_of(((long)a.tokens * a.slices + 3) / 4);
     if (inter) rotary_kernel<T, V, (V > 1 ? WITHIN : ACROSS), true, APPEND><<<grid, 256, 0, s>>>(a);
     else if (exchange) rotary_kernel<T, V, EXCHANGE, false, APPEND><<<grid, 256, 0, s>>>(a);
     else rotary_kernel<T, V, ACROSS, false, APPEND><<<grid, 256, 0, s>>>(a);

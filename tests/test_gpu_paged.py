@@ -1037,6 +1037,28 @@ def test_other_streams_and_calls_at_once():
             assert torch.equal(a, b)
 
 
+def test_more_threads_than_an_axis_of_a_launch_has():
+    """2^26 rows at a wave each are 2^32 threads: a rotation of that many, and an append and an attention in a buffer of that many, most of them of no sequence."""
+    tokens, f = (1 << 26) + 5, paged.rotary_frequencies(8)
+    x = torch.randn(tokens, 1, 8, device=DEV, dtype=HF)
+    p = torch.arange(tokens, device=DEV, dtype=torch.int32)
+    got = paged.rotary(x, p, f)
+    for at in (0, 1 << 25, tokens - 1000):
+        assert torch.equal(got[at:at + 1000], paged.rotary(x[at:at + 1000], p[at:at + 1000], f))
+    del got, p
+    s = Served([2000, 700], [3, 1], 1, 1, 8, 16, HF, seed=1)
+    kc, vc, want_k, want_v = s.k.clone(), s.v.clone(), s.k.clone(), s.v.clone()
+    for cu in (s.cu, s.cu + (tokens - 4)):                # the sequences' rows at the buffer's start, and at its end
+        here = x[int(cu[0]):int(cu[0]) + 4]
+        paged.cache_append(None, x, x, kc, vc, s.table, s.lens, cu, inv_freq=f)
+        paged.cache_append(None, here, here, want_k, want_v, s.table, s.lens, s.cu, inv_freq=f)
+        assert torch.equal(kc.nan_to_num(9), want_k.nan_to_num(9)) and torch.equal(vc.nan_to_num(9), want_v.nan_to_num(9))
+        out = torch.full_like(x, 3.0)
+        paged.cache_attention(x, kc, vc, s.table, s.lens, cu, out=out)
+        want = paged.cache_attention(here.contiguous(), kc, vc, s.table, s.lens, s.cu)
+        assert torch.equal(out[int(cu[0]):int(cu[0]) + 4], want) and int((out != 3).any(-1).sum()) == 4
+
+
 def test_offsets_beyond_32_bits():
     """A pool of more than 4 GiB a side: the last pages are read, written and copied where they are."""
     page, kv_heads, dim = 128, 8, 256
