@@ -3,8 +3,9 @@
 //   (a, b) -> g (a cos t - b sin t, a sin t + b cos t),   t = position * f_i
 //
 // Memory-bound: every element is read once and written once.  The angle is what needs care: at position 10^6 an fp32 product is off by
-// 0.06 rad, so t / 2 pi is formed in fp64 and only its fraction is kept, as 32 bits of a turn (6e-10 rad); sine and cosine are then Taylor sums
-// over [-pi/4, pi/4] in fp32 (next term below 3e-8).  That is ~50 instructions a pair, six of them in fp64: a wave handles one token (or a slice of
+// 0.06 rad, and at 2^40 an fp64 one still by 1e-4, so t / 2 pi is formed as a sum of two fp64 numbers and only its fraction is kept, to the nearest
+// 2^-32 of a turn (off by 7e-10 rad at most, whatever the position); sine and cosine are then Taylor sums
+// over [-pi/4, pi/4] in fp32 (next term below 3e-8).  That is ~50 instructions a pair, ten of them in fp64: a wave handles one token (or a slice of
 // its heads where tokens are few), each pair's angle is computed by one lane, and the heads read it from LDS (16 384 tokens of 32 heads of
 // 128, bf16: 45 us, 5.9 TB/s, what copying the tensor takes).
 #include <type_traits>
@@ -38,9 +39,13 @@ __device__ __forceinline__ void turn_sincos(uint32_t p, float& c, float& s) {
     if (quad & 2) s = -s;                                          // quarters 2 and 3
 }
 
+// position * inv_freq / 2 pi, its fraction in 2^-32.  Products and 1 / 2 pi are carried with what their rounding leaves (fma gives that of a product).
 __device__ __forceinline__ uint32_t turns(double position, double inv_freq) {
-    const double t = position * (inv_freq * 0.15915494309189535);  // 1 / 2 pi
-    return (uint32_t)(unsigned long long)((t - floor(t)) * 4294967296.0);     // 2^32 itself wraps to 0
+#pragma clang fp contract(off)                                     // (t - floor(t) is of the rounded product)
+    constexpr double PER = 0x1.45f306dc9c883p-3, PER_REST = -0x1.6b01ec5417056p-57;            // 1 / 2 pi
+    const double f = inv_freq * PER, f_rest = fma(inv_freq, PER, -f) + inv_freq * PER_REST;
+    const double t = position * f, t_rest = fma(position, f, -t) + position * f_rest;
+    return (uint32_t)(long long)rint(((t - floor(t)) + t_rest) * 4294967296.0);                 // whole turns, either way, wrap to 0
 }
 
 // What a lane handles of a head, in runs of V elements (the widest that dimensions, strides and addresses allow).  A run a lane, so that a wave reads whole

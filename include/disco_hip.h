@@ -462,7 +462,8 @@ typedef struct disco_rotary_desc {
     int64_t x_token, x_head, out_token, out_head;   /* strides in elements; a head's elements lie next to each other */
     double gain;                               /* multiplies the turned elements */
 } disco_rotary_desc;
-/* out = rotation of x by positions; d_out may be d_x (with equal strides).  The angle is computed in 64 bits: positions up to 2^40 keep theirs. */
+/* out = rotation of x by positions; d_out may be d_x (with equal strides).  The angle is off by 2^-33 of a turn at most, for positions up to 2^53
+ * (and frequencies as d_inv_freq holds them). */
 int disco_op_rotary(const disco_rotary_desc *d, const void *d_x, const void *d_positions, const double *d_inv_freq, void *d_out, void *stream);
 
 typedef struct disco_append_desc {

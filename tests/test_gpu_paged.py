@@ -93,6 +93,20 @@ def test_rotary_places_and_strides(interleaved):
     assert torch.equal(y, joined)                       # nothing else was touched
 
 
+def test_far_positions_keep_their_angles():
+    """fp32 against angles from whole numbers: position * frequency / 2 pi as fractions, with pi to 60 digits.  The tolerance has no part that grows with the position."""
+    from fractions import Fraction
+    pi = Fraction(314159265358979323846264338327950288419716939937510582097494, 10 ** 59)
+    f = paged.rotary_frequencies(64, base=5e5)
+    positions = [s * (far - i * 7919) for far in (1 << 20, 1 << 31, 1 << 40, 1 << 52) for i in range(20) for s in (1, -1)]
+    x = torch.randn(len(positions), 2, 64, generator=gen(4)).to(DEV)
+    got = paged.rotary(x, torch.tensor(positions, device=DEV), f).double().cpu()
+    turn = torch.tensor([[float((p * Fraction(w) / (2 * pi)) % 1) for w in f.tolist()] for p in positions], dtype=torch.float64)[:, None]
+    c, s, a, b = (2 * math.pi * turn).cos(), (2 * math.pi * turn).sin(), x[..., :32].double().cpu(), x[..., 32:].double().cpu()
+    size = torch.cat((a.abs() + b.abs(),) * 2, -1)
+    assert ((got - torch.cat((a * c - b * s, a * s + b * c), -1)).abs() <= (8 + 1) * 2.0 ** -24 * size).all()
+
+
 def test_an_axis_of_one_has_any_stride():
     """A view's stride of an axis of one is what it was cut from: nothing may be refused, or read, because of it."""
     f, p = paged.rotary_frequencies(64), torch.tensor([77], device=DEV)
