@@ -22,6 +22,7 @@
 //
 // A tile that some row sees only in part, or that has a page outside the cache, takes the masked path: scores of unseen keys are replaced (never
 // added to), and values that are not finite are kept out of the product and given to the rows that see them.
+#include <algorithm>
 #include <type_traits>
 #include "paged.h"
 
@@ -810,14 +811,12 @@ __device__ __forceinline__ void put_joined(const AttnArgs& a, const Joined& j, i
     if (a.lse && d == 0) a.lse[(long)t * a.q_heads + h] = none ? -INFINITY : ((m == -INFINITY ? 0.f : m - Mat<T>::BIAS) + log2f(l)) * LN2;
 }
 
+// (heads: h0 + the lane's of the at_once that a wave takes)
 template <typename T>
-__global__ __launch_bounds__(256) void cache_attention_join_kernel(AttnArgs a, int waves_a_token) {
-    const int lane = threadIdx.x & 63, quads = a.dim / 4, at_once = 64 / quads;
-    const int wave = (int)block_of() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = wave / waves_a_token;
-    if (t >= a.tokens) return;
-    const Joined j = joined_of(a, t);
-    const int h = (wave - t * waves_a_token) * at_once + lane / quads, d = lane % quads * 4;
-    if (j.splits <= 1 || lane / quads >= at_once || h >= a.q_heads) return;
+__device__ __forceinline__ void join_token(const AttnArgs& a, const Joined& j, int t, int h0, int at_once) {
+    const int lane = threadIdx.x & 63, quads = a.dim / 4;
+    const int h = h0 + lane / quads, d = lane % quads * 4;
+    if (lane / quads >= at_once || h >= a.q_heads) return;
     const long slot = part_at(a, j, t, h);
     float m = -INFINITY, l[8];
     f32x4 y[8];
@@ -843,6 +842,22 @@ __global__ __launch_bounds__(256) void cache_attention_join_kernel(AttnArgs a, i
     }
     put_joined<T>(a, j, t, h, d, ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7])), m,
                   ((l[0] + l[1]) + (l[2] + l[3])) + ((l[4] + l[5]) + (l[6] + l[7])));
+}
+
+// A wave takes every so-manieth token and passes over all of a sequence whose keys are not split (2 048 tokens of one, nothing to join: 8 us less).
+template <typename T>
+__global__ __launch_bounds__(256) void cache_attention_join_kernel(AttnArgs a, int waves_a_token) {
+    const int at_once = 256 / a.dim, wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int step = (int)(gridDim.x * 4 / waves_a_token), part = wave % waves_a_token;
+    int t = wave / waves_a_token;
+    if (t >= step) return;
+    while (t < a.tokens) {
+        const Joined j = joined_of(a, t);
+        if (j.b >= a.rows) return;                                 // behind the last sequence
+        if (j.splits > 1) join_token<T>(a, j, t, part * at_once, at_once);
+        else if (j.n > 0) t += (j.first + j.n - 1 - t) / step * step;
+        t += step;
+    }
 }
 
 template <typename T>
@@ -905,11 +920,12 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     const int group = d.q_heads / c.kv_heads;
     const int len = (int)(d.max_len > 0 && d.max_len < capacity ? d.max_len : capacity);
     const int most_new = d.max_new > 0 && d.max_new < d.tokens ? d.max_new : d.tokens;
-    // One sequence is taken to have all of the new tokens, and the one form that they ask for is launched; where it has fewer (rows behind it), that form does
-    // as well.  Several may be of any size up to the bound.
-    const bool alone = c.rows == 1;
+    // Every form that a sequence of up to so many rows may ask for is launched, also where there is one sequence: it may have fewer new tokens than
+    // the call has rows.  Where the caller says that it has as many, one form is enough (a launch that finds nothing takes 5 us: 2 048 tokens behind 16 384
+    // 553 us, with the launches of all forms and a join 566, a fresh prompt of 2 048 tokens 76 and 91, 33 tokens over 4 096 43 and 48).
+    const bool narrow = c.dim <= 128, alone = c.rows == 1 && d.max_new == d.tokens;
     const long most_rows = (long)most_new * group;
-    p.large = most_rows > MANY_LIMIT && c.dim > 64 && c.dim <= 128;
+    p.large = most_rows > MANY_LIMIT && c.dim > 64 && narrow;
     p.many = most_rows > FEW_LIMIT && !(alone && p.large);
     p.few = !(alone && most_rows > FEW_LIMIT);
     p.few_limit = most_rows <= FEW_LIMIT ? 0x7fffffff : (p.few ? FEW_LIMIT : 0);
@@ -918,10 +934,11 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     // (of the longest sequence: a part more or less because of the others in a call would show in the last bit)
     const long far = (long)d.window + 63 + rows_of(LARGE);
     const int keys = d.window > 0 && far < len ? (int)far : len;
-    if (p.few) p.few_splits = splits_of(FEW, 1, 1, keys, c.kv_heads, true);
+    if (p.few) p.few_splits = splits_of(FEW, 1, 1, keys, c.kv_heads, narrow);
     if (p.many || p.large) {
         const int form = alone && p.large ? LARGE : MANY, tile = rows_of(form), tiles = (int)((most_rows + tile - 1) / tile);
-        p.many_splits = alone ? splits_of(form, (int)most_rows, tiles, keys, c.kv_heads, c.dim <= 128) : splits_of(MANY, 1, 1, keys, 1, true);
+        p.many_splits = alone ? splits_of(form, (int)most_rows, tiles, keys, c.kv_heads, narrow)
+                              : std::max(splits_of(MANY, 1, 1, keys, c.kv_heads, narrow), narrow && keys >= 16384 ? 2 : 1);
     }
     // Room for the parts: of every token's rows, or where that is less of every sequence's, which has at most FEW_LIMIT rows a key head there, and here, where
     // its keys are split, at most 65 536 parts of rows (tiles * key heads * parts <= 512 of 128 rows, or 256 of 256) or two of each row of < 512 tiles
@@ -933,7 +950,7 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     p.many_room = (long)c.rows * room < heads * p.many_splits ? room : 0;
     p.many_parts = p.many_splits > 1 ? (p.many_room ? (long)c.rows * room : heads * p.many_splits) : 0;
     const long some = c.rows < d.tokens ? c.rows : d.tokens;
-    p.few_units = (some + rows / rows_of(FEW)) * p.few_splits * c.kv_heads;
+    p.few_units = (some + (p.few_limit == FEW_LIMIT ? 0 : rows / rows_of(FEW))) * p.few_splits * c.kv_heads;      // (at most FEW_LIMIT rows are one tile)
     p.many_units = (some + rows / rows_of(MANY)) * p.many_splits * c.kv_heads;
     p.large_units = (some + rows / rows_of(LARGE)) * p.many_splits * c.kv_heads;
     return p;
@@ -967,7 +984,8 @@ int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
         if ((p.few_splits > 8 || p.many_splits > 8) && rows <= 2048) cache_attention_join_row_kernel<T><<<(unsigned)rows, 256, 0, s>>>(a);
         else {
             const int waves_a_token = cdiv(a.q_heads, 256 / a.dim);
-            cache_attention_join_kernel<T><<<grid_of(((long)a.tokens * waves_a_token + 3) / 4), 256, 0, s>>>(a, waves_a_token);
+            const long most = cdiv(waves_a_token, 4) > 2048 ? cdiv(waves_a_token, 4) : 2048;      // (a wave for each part of a token at least)
+            cache_attention_join_kernel<T><<<grid_for(((long)a.tokens * waves_a_token + 3) / 4, most), 256, 0, s>>>(a, waves_a_token);
         }
         DISCO_LAUNCH_CHECK("cache_attention_join_kernel");
     }

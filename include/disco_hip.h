@@ -492,13 +492,15 @@ typedef struct disco_attention_desc {
     int32_t causal;                            /* 1: the token at position p sees the keys 0 .. p; 0: all of its sequence */
     int32_t window;                            /* > 0 (causal only): the keys p - window + 1 .. p */
     int32_t max_new, max_len;                  /* bounds that the host knows of new tokens and length of one sequence, 0: none.  They choose launch
-                                                  sizes, no result goes wrong where a sequence is longer. */
+                                                  sizes, no result goes wrong where a sequence is longer.  max_new = tokens with rows = 1: every row is
+                                                  a new token, which saves launches (where rows follow all the same, results may differ in the last bits). */
     float scale;                               /* of the scores */
     int64_t q_token, q_head, out_token, out_head;
 } disco_attention_desc;
 /* out = softmax(scale q k^T) v of every new token over its sequence's cache; d_lse (tokens x q_heads fp32, may be NULL): the logarithm of the
  * softmax's sum.  A token that sees no key gets zeros and -inf; rows ahead of d_cu_new[0] and behind d_cu_new[rows] are left alone.  Keys that a query does not see cannot
- * reach it, whatever they hold.  d_out shares no memory with d_q.  A sequence's result does not depend on the others in the call. */
+ * reach it, whatever they hold.  d_out shares no memory with d_q.  A sequence's result does not depend on the others in the call, nor
+ * on rows of none. */
 int disco_op_cache_attention_workspace_bytes(const disco_cache_desc *c, const disco_attention_desc *a, size_t *bytes);
 int disco_op_cache_attention(const disco_cache_desc *c, const disco_attention_desc *a, const void *d_q, const int32_t *d_page_table,
                              const int32_t *d_lens, const int32_t *d_cu_new, void *d_out, float *d_lse, void *d_ws, size_t ws_bytes, void *stream);

@@ -361,6 +361,21 @@ def test_one_sequence_with_rows_behind_it(rows, new):
         close_attended(got, lse, s.q, *s.args(), **{n: kw[n] for n in kw if n == "window"})
 
 
+@pytest.mark.parametrize("group,dim", [(2, 64), (16, 128), (3, 256)])
+@pytest.mark.parametrize("new", [1, 5, 33, 400])
+def test_one_sequence_is_cut_by_its_own_rows(new, group, dim):
+    """The same bits as it is, in buffers of more rows, beside an idle row, and whatever true bounds are given."""
+    s = Served([9000], [new], 1, group, dim, 16, BF, seed=new)
+    want, sums = paged.cache_attention(s.q, *s.args(), return_lse=True)
+    two = (s.k, s.v, torch.cat((s.table, s.table)), ints([9000, 50]), ints([0, new, new]))
+    for rows in (new, 40, 300, 1500):
+        q = torch.cat((s.q, s.q.new_zeros(max(0, rows - new), *s.q.shape[1:])))
+        for args in (s.args(), two):
+            for kw in (dict(), dict(max_new=new), dict(max_new=max(rows - 1, new), max_len=9000), dict(max_len=20000)):
+                got, lse = paged.cache_attention(q, *args, return_lse=True, **kw)
+                assert torch.equal(got[:new], want) and torch.equal(lse[:new], sums), (rows, kw)
+
+
 def test_a_mixed_call_with_long_prompts():
     """Every form in one call, keys split in each: long prompts, chunks, single tokens, idle rows, and parts kept by sequence and by token."""
     s = Served([3000, 5000, 0, 900, 2600, 40, 1200], [600, 1, 0, 70, 9, 3, 1100], 1, 2, 64, 16, BF, seed=3)
