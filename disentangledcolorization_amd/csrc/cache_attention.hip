@@ -57,8 +57,9 @@ struct AttnArgs {
     const int *table, *lens, *cu_new;
     long q_token, q_head, out_token, out_head, page_stride, head_stride, slot_stride;    // bytes
     int tokens, q_heads, kv_heads, group, dim, rows, width, pages, page_shift, causal, window;
-    // parts of a row that the workspace has room for, and where they are: by token, or by sequence
+    // parts of a row that there may be, and where they are: by token, or by sequence
     int few_splits, many_splits, few_by_sequence;
+    int few_fold, many_fold;                                       // a workgroup computes 2^fold parts of its rows and keeps their sum (0 or FOLD)
     int many_room;                                                 // of a sequence; 0: by token
     long many_from;
     int few, many;                                                 // sequences of at most so many rows take the form of few, of many rows
@@ -78,6 +79,11 @@ __device__ __forceinline__ ArgsAt fresh(ArgsAt p) {
 enum Form { FEW, MANY, LARGE };
 __host__ __device__ constexpr int rows_of(int form) { return form == FEW ? 16 : (form == MANY ? 128 : 256); }      // of a workgroup
 constexpr float LN2 = 0.6931471805599453f;
+
+// The parts of a row are added up in the order of the keys, in groups of 2^FOLD, and the groups in their order: whether a workgroup computes one part and a join adds
+// up the group, or computes the whole group and adds as it goes, the result has the same bits.
+constexpr int FOLD = 3;
+__host__ __device__ __forceinline__ int slots_of(int splits, int fold) { return (splits + (1 << fold) - 1) >> fold; }
 
 // ---- how a sequence is cut ------------------------------------------------------------------------------------------------------------
 struct Cut { int form, tiles, splits, chunk; };
@@ -125,15 +131,15 @@ __host__ __device__ __forceinline__ Cut cut_of(int n, int len, int group, int kv
     return u;
 }
 
-// where part 0 of a row lies: row `row` of the sequence's rows of key head `kv_head`, token t of the call, query head h
+// where the first slot of a row lies, `slots` being those of each of its sequence's rows: row `row` of the sequence's rows of key head `kv_head`, token t of the call, query head h
 template <typename Args>
-__device__ __forceinline__ long part_at(const Args& a, int form, int splits, int b, int row, int kv_head, int t, int h) {
+__device__ __forceinline__ long part_at(const Args& a, int form, int slots, int b, int row, int kv_head, int t, int h) {
     const long by_token = (long)t * a.q_heads + h;
-    if (form == FEW) return (a.few_by_sequence ? ((long)b * a.kv_heads + kv_head) * rows_of(FEW) + row : by_token) * a.few_splits;
-    return a.many_from + (a.many_room ? (long)b * a.many_room + ((long)row * a.kv_heads + kv_head) * splits : by_token * a.many_splits);
+    if (form == FEW) return (a.few_by_sequence ? ((long)b * a.kv_heads + kv_head) * rows_of(FEW) + row : by_token) * slots_of(a.few_splits, a.few_fold);
+    return a.many_from + (a.many_room ? (long)b * a.many_room + ((long)row * a.kv_heads + kv_head) * slots : by_token * slots_of(a.many_splits, a.many_fold));
 }
 
-struct Unit { int b, n, len, first, tile, split, head, begin; Cut cut; };
+struct Unit { int b, n, len, first, tile, split, parts, head, begin; Cut cut; };     // parts: that the workgroup has still to compute, `split` the next
 
 // unit number `want` of a form over all sequences (key head fastest, then split, then tile - the last, longest tiles first); false behind the last.
 // Every lane of the wave calls it and gets the same.
@@ -142,7 +148,7 @@ struct Cursor { int b0, before; };
 
 template <int FORM>
 __device__ __forceinline__ bool find_unit(ArgsAt a, int want, Cursor& at_last, Unit& u) {
-    const int lane = threadIdx.x & 63, capacity = a->width << a->page_shift;
+    const int lane = threadIdx.x & 63, capacity = a->width << a->page_shift, fold = FORM == FEW ? a->few_fold : a->many_fold;
     int left = want - at_last.before;
     for (int b0 = at_last.b0; b0 < a->rows; b0 += 64) {
         const int b = b0 + lane;
@@ -155,7 +161,7 @@ __device__ __forceinline__ bool find_unit(ArgsAt a, int want, Cursor& at_last, U
             if (first < 0 || n < 0 || n > a->tokens || first > a->tokens - n) n = 0;       // (not offsets)
             if (n > 0) {
                 cut = cut_of(n, len, a->group, a->kv_heads, a->window, a->dim <= 128, a->few, a->many, a->few_splits, a->many_splits);
-                if (cut.form == FORM) units = cut.tiles * cut.splits * a->kv_heads;
+                if (cut.form == FORM) units = cut.tiles * slots_of(cut.splits, fold) * a->kv_heads;
             }
         }
         int upto = units;
@@ -177,8 +183,10 @@ __device__ __forceinline__ bool find_unit(ArgsAt a, int want, Cursor& at_last, U
             u.cut.chunk = __builtin_amdgcn_readlane(cut.chunk, at);
             int x = left - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(units, at));
             u.head = x % a->kv_heads; x /= a->kv_heads;
-            u.split = x % u.cut.splits;
-            u.tile = u.cut.tiles - 1 - x / u.cut.splits;
+            const int slots = slots_of(u.cut.splits, fold);
+            u.split = x % slots << fold;
+            u.parts = min(1 << fold, u.cut.splits - u.split);
+            u.tile = u.cut.tiles - 1 - x / slots;
             u.begin = begin_of(u.len - u.n + u.tile * rows_of(FORM) / a->group, a->window) + u.split * u.cut.chunk;
             return true;
         }
@@ -274,6 +282,30 @@ struct Run {
 };
 
 template <typename T> struct Quad { T e[4]; };
+
+// the factor of a part of maximum m and sum l, `top` being the row's maximum; 0: a part that saw no key of the row, and left no numbers
+__device__ __forceinline__ float weight_of(float2 ml, float top) { return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_of(ml.x - top); }
+
+// Two parts added: the factors of each, and the sum of a number of each.  (Every rounding is written out: whoever adds rounds alike.)
+struct Fold {
+    float m, of_sum, of_part;
+    __device__ __forceinline__ Fold(float2 sum, float2 part) {
+        m = fmaxf(sum.x, part.x);
+        of_sum = weight_of(sum, m);
+        of_part = weight_of(part, m);
+    }
+    static __device__ __forceinline__ float add(float of_sum, float sum, float of_part, float part) {
+        const float kept = of_sum != 0.f ? of_sum * sum : 0.f;
+        return of_part != 0.f ? __builtin_fmaf(of_part, part, kept) : kept;
+    }
+    static __device__ __forceinline__ f32x4 add(float of_sum, f32x4 sum, float of_part, f32x4 part) {
+        f32x4 y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = add(of_sum, sum[i], of_part, part[i]);
+        return y;
+    }
+    template <typename T> __device__ __forceinline__ T add(T sum, T part) const { return add(of_sum, sum, of_part, part); }
+};
 
 // ---- few rows -------------------------------------------------------------------------------------------------------------------------------
 // A wave takes every fourth 32-key tile of the workgroup's range.  Keys go from memory straight into the operand (lane: key lane % 16, 8 elements at
@@ -460,25 +492,42 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
     for (int i = 0; i < DB; ++i) *(f32x4*)(om + col * OROW + 16 * i + 4 * g) = o[i];
     if (g == 0) { part_m[wave][col] = run.m; part_l[wave][col] = run.l; }
     __syncthreads();
+    const bool again = u.cut.splits > 1 && (u.split & ((1 << a->few_fold) - 1));      // not the first part that this workgroup computes of its rows
+    auto slot_of = [&](int rr, int t, int h) {
+        return part_at(*a, FEW, slots_of(u.cut.splits, a->few_fold), u.b, rr, u.head, t, h) + (u.split >> a->few_fold);
+    };
+    auto sums_of = [&](int r, float& m, float& l) {
+        m = fmaxf(fmaxf(part_m[0][r], part_m[1][r]), fmaxf(part_m[2][r], part_m[3][r]));
+        l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = weight_of(float2{part_m[w][r], part_l[w][r]}, m);
+            if (f != 0.f) l = __builtin_fmaf(f, part_l[w][r], l);  // (NaN is not 0)
+        }
+    };
     for (int x = threadIdx.x; x < 16 * (DP / 4); x += 256) {
         const int r = x / (DP / 4), d = (x - r * (DP / 4)) * 4, rr = u.tile * rows_of(FEW) + r;
         if (rr >= rows || d >= a->dim) continue;
-        float m = fmaxf(fmaxf(part_m[0][r], part_m[1][r]), fmaxf(part_m[2][r], part_m[3][r])), l = 0;
+        float m, l;
+        sums_of(r, m, l);
         f32x4 y = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float f = part_m[w][r] == -INFINITY ? (part_l[w][r] == 0.f ? 0.f : 1.f) : exp2_of(part_m[w][r] - m);
-            if (f != 0.f) {                                    // (a wave that saw nothing of the row; NaN is not 0)
-                l += f * part_l[w][r];
-                y += f * *(const f32x4*)((const float*)(lds + w * WAVE) + r * OROW + d);
+            const float f = weight_of(float2{part_m[w][r], part_l[w][r]}, m);
+            if (f != 0.f) {                                        // (0: a wave that saw nothing of the row)
+                const f32x4 x = *(const f32x4*)((const float*)(lds + w * WAVE) + r * OROW + d);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = __builtin_fmaf(f, x[i], y[i]);
             }
         }
         const int tok = rr / a->group, h = u.head * a->group + (rr - tok * a->group);
         const long t = u.first + tok, at_row = t * a->q_heads + h;
         if (u.cut.splits > 1) {
-            const long slot = part_at(*a, FEW, u.cut.splits, u.b, rr, u.head, (int)t, h) + u.split;
-            *(f32x4*)(a->part_o + slot * a->dim + d) = y;
-            if (d == 0) a->part_ml[slot] = float2{m, l};
+            const long slot = slot_of(rr, (int)t, h);
+            f32x4* to = (f32x4*)(a->part_o + slot * a->dim + d);
+            if (again) y = Fold(a->part_ml[slot], float2{m, l}).add(*to, y);
+            else if (d == 0) a->part_ml[slot] = float2{m, l};
+            *to = y;
         } else {
             const int p = a->causal ? u.len - u.n + tok : u.len - 1;
             const bool none = p < 0;
@@ -488,6 +537,18 @@ __device__ __forceinline__ uint32_t few_unit(ArgsAt a, const Unit& u, char* lds,
             for (int i = 0; i < 4; ++i) z.e[i] = (T)(none ? 0.f : y[i] * f);
             *(Quad<T>*)(a->out + t * a->out_token + h * a->out_head + d * 2) = z;
             if (a->lse && d == 0) a->lse[at_row] = none ? -INFINITY : ((m == -INFINITY ? 0.f : m - Mat<T>::BIAS) + log2f(l)) * LN2;
+        }
+    }
+    if (again) {                                                   // (all have read the sums so far)
+        __syncthreads();
+        const int r = threadIdx.x, rr = u.tile * rows_of(FEW) + r;
+        if (r < 16 && rr < rows) {
+            const int tok = rr / a->group;
+            const long slot = slot_of(rr, u.first + tok, u.head * a->group + (rr - tok * a->group));
+            float m, l;
+            sums_of(r, m, l);
+            const Fold f(a->part_ml[slot], float2{m, l});
+            a->part_ml[slot] = float2{f.m, f.add(a->part_ml[slot].y, l)};
         }
     }
     return odd;
@@ -509,7 +570,10 @@ __device__ __noinline__ void few_unit_odd(uint64_t args, int want, uint32_t lds,
     Unit u;
     Cursor c{0, 0};
     if (!find_unit<FEW>(a, __builtin_amdgcn_readfirstlane(want), c, u)) return;
-    few_unit<T, DP, true>(a, u, lds_pointer(lds), *(float (*)[4][16])lds_pointer(m), *(float (*)[4][16])lds_pointer(l));
+    for (; u.parts > 0; --u.parts, ++u.split, u.begin += u.cut.chunk) {
+        few_unit<T, DP, true>(a, u, lds_pointer(lds), *(float (*)[4][16])lds_pointer(m), *(float (*)[4][16])lds_pointer(l));
+        __syncthreads();
+    }
 }
 
 template <typename T, int DP>
@@ -521,10 +585,9 @@ __global__ __launch_bounds__(256, few_waves(DP)) void cache_attention_few_kernel
     for (int want = blockIdx.x;; want += gridDim.x) {
         Unit u;
         if (!find_unit<FEW>(fresh(a), want, c, u)) break;
-        if (__syncthreads_or(few_unit<T, DP, false>(fresh(a), u, lds, part_m, part_l) != 0)) {
-            few_unit_odd<T, DP>(kernel_args(), want, lds_offset(lds), lds_offset(part_m), lds_offset(part_l));
-            __syncthreads();
-        }
+        int odd = 0;
+        for (; u.parts > 0; --u.parts, ++u.split, u.begin += u.cut.chunk) odd |= __syncthreads_or(few_unit<T, DP, false>(fresh(a), u, lds, part_m, part_l) != 0);
+        if (odd) few_unit_odd<T, DP>(kernel_args(), want, lds_offset(lds), lds_offset(part_m), lds_offset(part_l));
     }
 }
 
@@ -713,14 +776,20 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
     if (row < rows) {
         const long t = u.first + token, at_row = t * a->q_heads + head;
         if (u.cut.splits > 1) {
-            const long slot = part_at(*a, FORM, u.cut.splits, u.b, row, u.head, (int)t, head) + u.split;
-            if (h == 0) a->part_ml[slot] = float2{run.m, run.l};
+            const long slot = part_at(*a, FORM, slots_of(u.cut.splits, a->many_fold), u.b, row, u.head, (int)t, head) + (u.split >> a->many_fold);
+            const bool again = u.split & ((1 << a->many_fold) - 1);        // not the first part that this workgroup computes of its rows
+            const float2 part = float2{run.m, run.l}, sum = again ? a->part_ml[slot] : float2{-INFINITY, 0.f};
+            const Fold f(sum, part);
+            if (h == 0) a->part_ml[slot] = again ? float2{f.m, f.add(sum.y, part.y)} : part;
 #pragma unroll
             for (int i = 0; i < DB; ++i)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4) {
                     const int d = 32 * i + 2 * r + 4 * h;
-                    if (d < a->dim) *(f32x4*)(a->part_o + slot * a->dim + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+                    if (d >= a->dim) continue;
+                    f32x4* to = (f32x4*)(a->part_o + slot * a->dim + d);
+                    const f32x4 y = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+                    *to = again ? f.add(*to, y) : y;
                 }
         } else {
             const bool none = pos < 0;
@@ -748,7 +817,10 @@ __device__ __noinline__ void many_unit_odd(uint64_t args, int want, uint32_t lds
     Unit u;
     Cursor c{0, 0};
     if (!find_unit<FORM>(a, __builtin_amdgcn_readfirstlane(want), c, u)) return;
-    many_unit<T, DP, FORM, true>(a, u, lds_pointer(lds));
+    for (; u.parts > 0; --u.parts, ++u.split, u.begin += u.cut.chunk) {
+        many_unit<T, DP, FORM, true>(a, u, lds_pointer(lds));
+        __syncthreads();
+    }
 }
 
 template <typename T, int DP, int FORM>
@@ -763,20 +835,22 @@ __global__ __launch_bounds__(2 * rows_of(FORM), DP <= 128 ? 2 : 1) void cache_at
     for (int want = blockIdx.x;; want += gridDim.x) {
         Unit u;
         if (!find_unit<FORM>(fresh(a), want, c, u)) break;
-        if (__syncthreads_or(many_unit<T, DP, FORM, false>(fresh(a), u, lds) != 0)) many_unit_odd<T, DP, FORM>(kernel_args(), want, lds_offset(lds));
+        int odd = 0;
+        for (; u.parts > 0; --u.parts, ++u.split, u.begin += u.cut.chunk) odd |= __syncthreads_or(many_unit<T, DP, FORM, false>(fresh(a), u, lds) != 0);
+        if (odd) many_unit_odd<T, DP, FORM>(kernel_args(), want, lds_offset(lds));
     }
 }
 
 // ---- the parts of a row whose keys were split -------------------------------------------------------------------------------------------------
-// Part s counts into sum s % 8, the eight sums are added as ((0 + 1) + (2 + 3)) + ((4 + 5) + (6 + 7)), whichever of the two forms joins a row: how a row is
-// joined does not depend on the parts that other rows have.  Both are bound by latency, the loads of a row's parts all under way at once.
-//   a few rows of many parts   four waves a row, a part a team of dim / 4 lanes (64 rows of 64 parts of 128: 7 us; 256 rows of 64 parts: 10 us less
-//                              than the other form)
-//   many rows                  dim / 4 lanes a row, a wave takes 256 / dim heads of a token (10 000 rows of five parts of 64: 15 us)
-struct Joined { int b, n, len, first, form, splits; };
+// Groups of eight parts are added up in the order of the keys, and then the groups in theirs, whichever of the two forms joins a row: how a row is
+// joined does not depend on the parts that other rows have, nor on how many of them a workgroup has added up before.  Both are bound by latency, the loads
+// of a group's parts all under way at once.
+//   a few rows of many parts   four waves a row, a group a team of dim / 4 lanes (64 rows of 64 parts of 128: 7 us; 2 048 of 11: 12 us, the other form 7)
+//   many rows                  dim / 4 lanes a row, a wave takes 256 / dim heads of a token (10 000 rows of five parts of 64: 12 us)
+struct Joined { int b, n, len, first, form, splits, slots; };
 
 __device__ __forceinline__ Joined joined_of(const AttnArgs& a, int t) {
-    Joined j{0, 0, 0, 0, 0, 0};
+    Joined j{0, 0, 0, 0, 0, 0, 0};
     const int b = j.b = seq_of_token(a.cu_new, a.rows, t);
     if (b >= a.rows) return j;
     j.first = a.cu_new[b];
@@ -787,21 +861,31 @@ __device__ __forceinline__ Joined joined_of(const AttnArgs& a, int t) {
         const Cut cut = cut_of(j.n, j.len, a.group, a.kv_heads, a.window, a.dim <= 128, a.few, a.many, a.few_splits, a.many_splits);
         j.form = cut.form;
         j.splits = cut.splits;
+        j.slots = slots_of(cut.splits, cut.form == FEW ? a.few_fold : a.many_fold);
     }
     return j;
 }
 __device__ __forceinline__ long part_at(const AttnArgs& a, const Joined& j, int t, int h) {
     const int kv_head = h / a.group;
-    return part_at(a, j.form, j.splits, j.b, (t - j.first) * a.group + h - kv_head * a.group, kv_head, t, h);
+    return part_at(a, j.form, j.slots, j.b, (t - j.first) * a.group + h - kv_head * a.group, kv_head, t, h);
 }
+// the parts that a slot's group has in the workspace: 2^FOLD, or one, their sum
+__device__ __forceinline__ int group_of(const AttnArgs& a, const Joined& j) { return (j.form == FEW ? a.few_fold : a.many_fold) ? 1 : 1 << FOLD; }
 
-// the factor of a part of maximum m and sum l, `top` being the row's maximum; 0: a part that saw no key of the row, and left no numbers
-__device__ __forceinline__ float weight_of(float2 ml, float top) { return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : exp2_of(ml.x - top); }
-// (one rounding, written out: both forms of the join have to round alike)
-__device__ __forceinline__ float add_part(float sum, float w, float x) { return w != 0.f ? __builtin_fmaf(w, x, sum) : sum; }
+struct Sum {
+    float2 ml; f32x4 y;
+    __device__ __forceinline__ void add(bool first, float2 part, f32x4 x) {
+        if (first) { ml = part; y = x; return; }
+        const Fold f(ml, part);
+        y = f.add(y, x);
+        ml = float2{f.m, f.add(ml.y, part.y)};
+    }
+};
 
 template <typename T>
-__device__ __forceinline__ void put_joined(const AttnArgs& a, const Joined& j, int t, int h, int d, f32x4 y, float m, float l) {
+__device__ __forceinline__ void put_joined(const AttnArgs& a, const Joined& j, int t, int h, int d, const Sum& sum) {
+    const float m = sum.ml.x, l = sum.ml.y;
+    const f32x4 y = sum.y;
     const bool none = a.causal ? j.len - j.n + (t - j.first) < 0 : j.len <= 0;
     const float f = none ? 0.f : 1.f / l;
     Quad<T> r;
@@ -818,30 +902,24 @@ __device__ __forceinline__ void join_token(const AttnArgs& a, const Joined& j, i
     const int h = h0 + lane / quads, d = lane % quads * 4;
     if (lane / quads >= at_once || h >= a.q_heads) return;
     const long slot = part_at(a, j, t, h);
-    float m = -INFINITY, l[8];
-    f32x4 y[8];
-#pragma unroll
-    for (int g = 0; g < 8; ++g) { l[g] = 0.f; y[g] = f32x4{0, 0, 0, 0}; }
-    for (int s0 = 0; s0 < j.splits; s0 += 8)
-#pragma unroll
-        for (int g = 0; g < 8; ++g) if (s0 + g < j.splits) m = fmaxf(m, a.part_ml[slot + s0 + g].x);
-    for (int s0 = 0; s0 < j.splits; s0 += 8) {
-        float w[8];
+    const int group = group_of(a, j);
+    Sum all;
+    for (int s0 = 0; s0 < j.slots; s0 += group) {
+        float2 ml[8];
         f32x4 x[8];
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-            const float2 ml = s0 + g < j.splits ? a.part_ml[slot + s0 + g] : float2{-INFINITY, 0.f};
-            w[g] = weight_of(ml, m);
-            x[g] = s0 + g < j.splits ? *(const f32x4*)(a.part_o + (slot + s0 + g) * a.dim + d) : f32x4{0, 0, 0, 0};
-            l[g] = add_part(l[g], w[g], ml.y);
-        }
+        for (int i = 0; i < 8; ++i)
+            if (i < group && s0 + i < j.slots) {
+                ml[i] = a.part_ml[slot + s0 + i];
+                x[i] = *(const f32x4*)(a.part_o + (slot + s0 + i) * a.dim + d);
+            }
+        Sum sum;
 #pragma unroll
-        for (int g = 0; g < 8; ++g)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) y[g][i] = add_part(y[g][i], w[g], x[g][i]);
+        for (int i = 0; i < 8; ++i)
+            if (i < group && s0 + i < j.slots) sum.add(i == 0, ml[i], x[i]);
+        all.add(s0 == 0, sum.ml, sum.y);
     }
-    put_joined<T>(a, j, t, h, d, ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7])), m,
-                  ((l[0] + l[1]) + (l[2] + l[3])) + ((l[4] + l[5]) + (l[6] + l[7])));
+    put_joined<T>(a, j, t, h, d, all);
 }
 
 // A wave takes every so-manieth token and passes over all of a sequence whose keys are not split (2 048 tokens of one, nothing to join: 8 us less).
@@ -867,47 +945,70 @@ __global__ __launch_bounds__(256) void cache_attention_join_row_kernel(AttnArgs 
     const Joined j = joined_of(a, t);
     if (j.splits <= 1) return;
     const long slot = part_at(a, j, t, h);
-    const float2 ml = lane < j.splits ? a.part_ml[slot + lane] : float2{-INFINITY, 0.f};
-    float m = ml.x;
-#pragma unroll
-    for (int i = 32; i; i >>= 1) m = fmaxf(m, __shfl_xor(m, i));
-    const float w = weight_of(ml, m);
-    float l = 0.f;
-#pragma unroll
-    for (int s0 = 0; s0 < 64; s0 += 8) l = add_part(l, __shfl(w, s0 + (lane & 7)), __shfl(ml.y, s0 + (lane & 7)));
-    l += __shfl_xor(l, 1);
-    l += __shfl_xor(l, 2);
-    l += __shfl_xor(l, 4);
+    const int group = group_of(a, j);
+    // a team of dim / 4 lanes adds up a group's eight parts, whose loads go first
     const int quads = a.dim / 4, teams = 256 / quads < 8 ? 256 / quads : 8, team = threadIdx.x / quads, d = (threadIdx.x - team * quads) * 4;
-    for (int g0 = 0; g0 < 8; g0 += teams) {                        // (the weights are asked of all lanes: nobody leaves the loop early)
-        const int g = g0 + team;
-        f32x4 sum = f32x4{0, 0, 0, 0};
+    f32x4 x[8];
+    auto load = [&](int g) {
 #pragma unroll
-        for (int s0 = 0; s0 < 64; s0 += 8) {
-            const float ws = __shfl(w, (s0 + g) & 63);
-            if (team < teams && g < 8 && s0 + g < j.splits && ws != 0.f) {
-                const f32x4 x = *(const f32x4*)(a.part_o + (slot + s0 + g) * a.dim + d);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] = add_part(sum[i], ws, x[i]);
-            }
+        for (int i = 0; i < 8; ++i)
+            if (team < teams && i < group && g * group + i < j.slots) x[i] = *(const f32x4*)(a.part_o + (slot + g * group + i) * a.dim + d);
+    };
+    load(team);
+    const float2 ml = lane < j.slots ? a.part_ml[slot + lane] : float2{-INFINITY, 0.f};
+    // the factors: a lane follows the sums of its group, and keeps those of its own part; then all follow the groups'
+    const int place = group == 1 ? 0 : lane & 7;
+    float2 sum = float2{__shfl(ml.x, lane - place), __shfl(ml.y, lane - place)};
+    float of_sum = 0.f, of_part = 1.f;
+#pragma unroll 1
+    for (int i = 1; i < group && i < j.slots; ++i) {
+        const float2 part = float2{__shfl(ml.x, lane - place + i), __shfl(ml.y, lane - place + i)};
+        if (lane - place + i < j.slots) {
+            const Fold f(sum, part);
+            if (place == i) { of_sum = f.of_sum; of_part = f.of_part; }
+            sum = float2{f.m, f.add(sum.y, part.y)};
         }
-        if (team < teams && g < 8) *(f32x4*)&sums[g][d] = sum;
+    }
+    float2 all = float2{__shfl(sum.x, 0), __shfl(sum.y, 0)};
+    float of_all[8], of_group[8];
+#pragma unroll
+    for (int g = 1; g < 8; ++g) {
+        if (g * group < j.slots) {
+            const float2 part = float2{__shfl(sum.x, g * group), __shfl(sum.y, g * group)};
+            const Fold f(all, part);
+            of_all[g] = f.of_sum; of_group[g] = f.of_part;
+            all = float2{f.m, f.add(all.y, part.y)};
+        }
+    }
+    for (int g0 = 0; g0 < 8; g0 += teams) {                        // (the factors are asked of all lanes: nobody leaves the loop early)
+        const int g = g0 + team;
+        if (g0) load(g);
+        f32x4 y = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+            const int s = g * group + i;
+            const float fs = __shfl(of_sum, s & 63), fp = __shfl(of_part, s & 63);
+            if (i < group && s < j.slots) y = Fold::add(fs, y, fp, x[i]);
+        }
+        if (team < teams && g < 8 && g * group < j.slots) *(f32x4*)&sums[g][d] = y;
     }
     __syncthreads();
     if ((int)threadIdx.x >= quads) return;
-    f32x4 y[8];
+    f32x4 y = *(const f32x4*)&sums[0][d];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) y[g] = *(const f32x4*)&sums[g][threadIdx.x * 4];
-    put_joined<T>(a, j, t, h, threadIdx.x * 4, ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7])), m, l);
+    for (int g = 1; g < 8; ++g) if (g * group < j.slots) y = Fold::add(of_all[g], y, of_group[g], *(const f32x4*)&sums[g][d]);
+    put_joined<T>(a, j, t, h, d, Sum{all, y});
 }
 
 // ---- what the host decides ----------------------------------------------------------------------------------------------------------------------
 constexpr int FEW_LIMIT = 16, MANY_LIMIT = 1024;
+constexpr long ROOM = 256l << 20;
 
 struct Plan {
     bool few, many, large;             // which forms are launched
     int few_limit, many_limit;         // rows (INT_MAX: all)
     int few_splits, many_splits;       // a row's parts, at most
+    int few_fold, many_fold;
     bool few_by_sequence;
     int many_room;
     long few_parts, many_parts;        // in the workspace
@@ -941,14 +1042,21 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
                               : std::max(splits_of(MANY, 1, 1, keys, c.kv_heads, narrow), narrow && keys >= 16384 ? 2 : 1);
     }
     // Room for the parts: of every token's rows, or where that is less of every sequence's, which has at most FEW_LIMIT rows a key head there, and here, where
-    // its keys are split, at most 65 536 parts of rows (tiles * key heads * parts <= 512 of 128 rows, or 256 of 256) or two of each row of < 512 tiles
+    // its keys are split, at most 65 536 parts of rows (tiles * key heads * parts <= 512 of 128 rows, or 256 of 256) or two of each row of < 512 tiles.
+    // Where a form would take more than ROOM bytes, its workgroups compute whole groups of parts and keep one slot a group; there are sequences enough then
+    // to fill the GPU.  32 heads of 128 on 8, tables of 32 768, no bound on the lengths: 256 sequences of 17 tokens over 2 000 keys 633 us and 0.75 GB (a slot a
+    // part: 625 and 5.8), 1 000 single tokens over 1 024 1 024 us and 0.27 GB (929 and 2.1), 300 of 500 and one of 65 536 317 us (233).
     const long rows = (long)d.tokens * group, heads = (long)d.tokens * d.q_heads;
     p.few_by_sequence = p.few_limit == FEW_LIMIT && (long)c.rows * c.kv_heads * FEW_LIMIT < heads;
-    p.few_parts = p.few_splits > 1 ? (p.few_by_sequence ? (long)c.rows * c.kv_heads * FEW_LIMIT : heads) * p.few_splits : 0;
+    const long bytes = (long)c.dim * 4 + 8, few_rows = p.few_by_sequence ? (long)c.rows * c.kv_heads * FEW_LIMIT : heads;
+    p.few_fold = few_rows * p.few_splits * bytes > ROOM ? FOLD : 0;
+    p.few_parts = p.few_splits > 1 ? few_rows * slots_of(p.few_splits, p.few_fold) : 0;
     const long twice = 2 * c.kv_heads * (p.large ? MANY_LIMIT : rows);
     const int room = twice <= 65536 ? 65536 : (twice < 131072 ? (int)twice : 131072);
-    p.many_room = (long)c.rows * room < heads * p.many_splits ? room : 0;
-    p.many_parts = p.many_splits > 1 ? (p.many_room ? (long)c.rows * room : heads * p.many_splits) : 0;
+    p.many_fold = std::min((long)c.rows * room, heads * p.many_splits) * bytes > ROOM ? FOLD : 0;
+    const int many_slots = slots_of(p.many_splits, p.many_fold), many_room = p.many_fold ? 65536 : room;      // (two parts are one slot)
+    p.many_room = (long)c.rows * many_room < heads * many_slots ? many_room : 0;
+    p.many_parts = p.many_splits > 1 ? (p.many_room ? (long)c.rows * many_room : heads * many_slots) : 0;
     const long some = c.rows < d.tokens ? c.rows : d.tokens;
     p.few_units = (some + (p.few_limit == FEW_LIMIT ? 0 : rows / rows_of(FEW))) * p.few_splits * c.kv_heads;      // (at most FEW_LIMIT rows are one tile)
     p.many_units = (some + rows / rows_of(MANY)) * p.many_splits * c.kv_heads;
@@ -981,7 +1089,7 @@ int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
     }
     if (p.few_parts + p.many_parts > 0) {
         const long rows = (long)a.tokens * a.q_heads;
-        if ((p.few_splits > 8 || p.many_splits > 8) && rows <= 2048) cache_attention_join_row_kernel<T><<<(unsigned)rows, 256, 0, s>>>(a);
+        if ((p.few_splits > 16 || p.many_splits > 16) && rows <= 2048) cache_attention_join_row_kernel<T><<<(unsigned)rows, 256, 0, s>>>(a);
         else {
             const int waves_a_token = cdiv(a.q_heads, 256 / a.dim);
             const long most = cdiv(waves_a_token, 4) > 2048 ? cdiv(waves_a_token, 4) : 2048;      // (a wave for each part of a token at least)
@@ -1017,7 +1125,7 @@ int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc
     AttnArgs a{(const char*)q, (const char*)c.d_k, (const char*)c.d_v, (char*)out, lse, (float*)ws, (float2*)((char*)ws + parts * c.dim * 4),
                table, lens, cu_new, d.q_token * 2, d.q_head * 2, d.out_token * 2, d.out_head * 2, c.page_stride * 2, c.head_stride * 2, c.slot_stride * 2,
                d.tokens, d.q_heads, c.kv_heads, d.q_heads / c.kv_heads, c.dim, c.rows, c.table_width, c.pages, __builtin_ctz((unsigned)c.page_size), d.causal,
-               window, p.few_splits, p.many_splits, p.few_by_sequence, p.many_room, p.few_parts, p.few_limit, p.many_limit, fabsf(d.scale) * 1.4426950408889634f, d.scale < 0};
+               window, p.few_splits, p.many_splits, p.few_by_sequence, p.few_fold, p.many_fold, p.many_room, p.few_parts, p.few_limit, p.many_limit, fabsf(d.scale) * 1.4426950408889634f, d.scale < 0};
     if (a.c < 1e-37f) a.c = 1e-37f;                                // 0 * -inf is not the score of a key that is not seen
     return c.dtype == DISCO_F16 ? run_dims<f16>(a, p, s) : run_dims<bf16>(a, p, s);
 }

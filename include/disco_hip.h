@@ -499,7 +499,8 @@ typedef struct disco_attention_desc {
 } disco_attention_desc;
 /* out = softmax(scale q k^T) v of every new token over its sequence's cache; d_lse (tokens x q_heads fp32, may be NULL): the logarithm of the
  * softmax's sum.  A token that sees no key gets zeros and -inf; rows ahead of d_cu_new[0] and behind d_cu_new[rows] are left alone.  Keys that a query does not see cannot
- * reach it, whatever they hold.  d_out shares no memory with d_q.  A sequence's result does not depend on the others in the call, nor
+ * reach it, whatever they hold.  The workspace holds parts of rows in fp32, by what may be: tables and heads, the bounds of the descriptor where they are
+ * given (1 000 single tokens over tables of 32 768, 32 heads of 128 on 8: 0.3 GB); where it would be large, workgroups add parts up as they go.  d_out shares no memory with d_q.  A sequence's result does not depend on the others in the call, nor
  * on rows of none. */
 int disco_op_cache_attention_workspace_bytes(const disco_cache_desc *c, const disco_attention_desc *a, size_t *bytes);
 int disco_op_cache_attention(const disco_cache_desc *c, const disco_attention_desc *a, const void *d_q, const int32_t *d_page_table,

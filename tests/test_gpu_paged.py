@@ -444,6 +444,54 @@ def test_attention_workspace_stays_small():
     assert 0 < n.value < 1 << 29
 
 
+@pytest.mark.parametrize("rows,tokens,width", [(256, 4351, 2048), (64, 4159, 2048), (1000, 1000, 2048), (1000, 1000, 8192), (256, 16384, 8192)])
+def test_attention_workspace_of_many_sequences(rows, tokens, width):
+    """Steps of many sequences over tables of up to 131 072 tokens, nothing known of their lengths, 32 heads of 128 on 8: less than a gigabyte, and with a bound on
+    the lengths that single tokens and chunks have, less than half of one."""
+    import ctypes as C
+    n = C.c_size_t()
+    c = _ffi.CacheDesc(_ffi.BF16, 1, 90000, 8, 16, 128, rows, width, 0, 8 * 16 * 128, 16 * 128, 128, 1 << 20, 1 << 20)
+    for max_len, most in ((0, 3 << 30 if tokens > 5000 else 1 << 30), (4096, 1 << 29)):
+        a = _ffi.AttentionDesc(tokens, 32, 1, 0, 0, max_len, 0.1, 4096, 128, 4096, 128)
+        assert _ffi.lib().disco_op_cache_attention_workspace_bytes(C.byref(c), C.byref(a), C.byref(n)) == 0
+        assert 0 < n.value < most
+
+
+@pytest.mark.parametrize("kv_heads,group,dim,dtype", [(2, 4, 64, BF), (1, 8, 128, BF), (2, 4, 128, HF), (1, 3, 256, HF)])
+def test_groups_of_parts_have_the_bits_of_parts(kv_heads, group, dim, dtype):
+    """A call of so many sequences that its workgroups add up groups of parts themselves: every form, windows, values that are not finite, pages outside the
+    cache; bit for bit what each sequence has alone, where a join adds them up."""
+    rows, page, keys = 2200, 64, 30000
+    lens, new = [70] * rows, [1] * rows
+    for b, (n, m) in enumerate([(30000, 1), (9001, 2), (20000, 20), (700, 1), (29999, 60), (12345, 700 // group), (25000, 3000 // group), (26000, 5), (24000, 33), (17000, 400)]):
+        lens[3 * b], new[3 * b] = n, m
+    g = gen(dim)
+    pages = keys // page + 1
+    table = torch.stack([torch.randperm(pages, generator=g) for _ in range(40)]).int().repeat(rows // 40, 1)
+    k, v = (torch.randn(pages, kv_heads, page, dim, generator=g).to(dtype).to(DEV) for _ in range(2))
+    v[int(table[21, 300]), 0, 5, 3] = math.inf            # row 21 sees it whole, others somewhere
+    table[24, 200] = -7
+    table = table.contiguous().to(DEV)
+    cu = [0]
+    for m in new:
+        cu.append(cu[-1] + m)
+    q = torch.randn(cu[-1], kv_heads * group, dim, generator=g).to(dtype).to(DEV)
+    import ctypes as C
+    c, n = paged._cache(k, v, table), C.c_size_t()
+    a = _ffi.AttentionDesc(cu[-1], kv_heads * group, 1, 0, 0, 0, 0.1, kv_heads * group * dim, dim, kv_heads * group * dim, dim)
+    assert _ffi.lib().disco_op_cache_attention_workspace_bytes(C.byref(c), C.byref(a), C.byref(n)) == 0
+    assert n.value < kv_heads * group * cu[-1] * 64 * (dim * 4 + 8)        # (less than a slot for every part of a row)
+    for kw in (dict(), dict(window=11000)):
+        got, sums = paged.cache_attention(q, k, v, table, ints(lens), ints(cu), return_lse=True, **kw)
+        for b in (*range(0, 30, 3), 1, 2, rows - 1):
+            at, to = cu[b], cu[b + 1]
+            alone, alone_sums = paged.cache_attention(q[at:to], k, v, table[b:b + 1].contiguous(), ints(lens[b:b + 1]), ints([0, to - at]), return_lse=True, **kw)
+            for x, y in ((got[at:to], alone), (sums[at:to], alone_sums)):
+                assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x.nan_to_num(7, 8, 9), y.nan_to_num(7, 8, 9)), b
+        if not kw:
+            assert got[cu[24]:cu[25]].isnan().all() and not got[cu[27]:cu[28]].isnan().any()
+
+
 def test_attention_of_nothing():
     s = Served([50, 0, 20], [0, 0, 0], 2, 2, 64, 16, BF)
     assert paged.cache_attention(s.q, *s.args()).shape == (0, 4, 64)
