@@ -492,6 +492,125 @@ def test_groups_of_parts_have_the_bits_of_parts(kv_heads, group, dim, dtype):
             assert got[cu[24]:cu[25]].isnan().all() and not got[cu[27]:cu[28]].isnan().any()
 
 
+def close_heads(got, lse, s, pick, **kw):
+    """Some heads and tokens of a large call against the plain form: `pick` [(sequence, first new token, how many)]."""
+    kv_heads, group = s.k.shape[1], s.q.shape[1] // s.k.shape[1]
+    for b, i, n in pick:
+        at, length, new = int(s.cu[b]), int(s.lens[b]), int(s.cu[b + 1] - s.cu[b])
+        h = (b + i) % kv_heads
+        heads = slice(h * group, h * group + 1)
+        k, v = s.k[:, h:h + 1], s.v[:, h:h + 1]
+        end = torch.tensor([length - new + i + n], dtype=torch.int32) if kw.get("causal", True) else s.lens[b:b + 1]
+        rows = slice(at + i, at + i + n)
+        if not kw.get("causal", True):
+            assert i + n == new
+        close_attended(got[rows, heads], lse[rows, heads], s.q[rows, heads], k, v, s.table[b:b + 1], end, torch.tensor([0, n]), **kw)
+
+
+LARGE = [
+    # lens, new, kv heads, group, dim: rows of more than 1 024 in heads of 72 to 128
+    ([1300], [1300], 1, 1, 128), ([2600], [1100], 1, 2, 72), ([700, 900], [600, 513], 2, 2, 80), ([40000], [300], 1, 4, 96), ([5000, 30, 0, 300], [520, 30, 0, 1], 2, 4, 104),
+    ([1200], [1025], 8, 1, 120), ([3000, 3000], [1040, 1030], 4, 1, 128),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("case", LARGE)
+@pytest.mark.parametrize("kw", [dict(), dict(window=333), dict(causal=False), dict(scale=-0.1)])
+def test_the_form_of_256_rows(case, dtype, kw):
+    """Split and not, heads that do not fill their blocks, alone and beside the other forms, masks and types."""
+    lens, new, kv_heads, group, dim = case
+    s = Served(lens, new, kv_heads, group, dim, 16, dtype, seed=dim)
+    got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True, **kw)
+    pick = []
+    for b, n in enumerate(new):
+        if n:
+            m = min(n, 7)
+            pick += [(b, i, m) for i in ({0, n // 2, n - m} if kw.get("causal", True) else {n - m})]
+    close_heads(got, lse, s, pick, **kw)
+    if len(new) > 1:                                      # beside the others, and alone: the same bits
+        alone = paged.cache_attention(s.q[:new[0]], s.k, s.v, s.table[:1].contiguous(), s.lens[:1].contiguous(), ints([0, new[0]]), **kw)
+        assert torch.equal(alone, got[:new[0]])
+
+
+def test_every_form_in_one_call():
+    """Few, many and large rows of heads of 128, split and not, in one call and each alone: the same bits, and the plain form's values."""
+    lens, new = [9000, 1200, 20000, 0, 3000, 700, 6000, 50], [1, 600, 40, 0, 5, 300, 1100, 50]
+    s = Served(lens, new, 2, 4, 128, 16, BF, seed=7)
+    for kw in (dict(), dict(window=777), dict(max_new=1100, max_len=20000)):
+        got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True, **kw)
+        call = {n: kw[n] for n in kw if n == "window"}
+        close_heads(got, lse, s, [(b, i, min(n, 5)) for b, n in enumerate(new) if n for i in {0, min(n // 3, n - min(n, 5)), n - min(n, 5)}], **call)
+        for b, n in enumerate(new):
+            at = int(s.cu[b])
+            alone = paged.cache_attention(s.q[at:at + n], s.k, s.v, s.table[b:b + 1].contiguous(), s.lens[b:b + 1].contiguous(), ints([0, n]), **call)
+            assert torch.equal(alone, got[at:at + n])
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, BF), (80, HF)])
+@pytest.mark.parametrize("length", [1500, 20000])
+def test_256_rows_and_what_they_do_not_see(dim, dtype, length):
+    """Values and keys that are not finite, and pages outside the cache, reach only the rows that see them; split and not."""
+    new = 1100
+    s = Served([length], [new], 1, 1, dim, 16, dtype, seed=dim)
+    pos = torch.arange(length - new, length, device=DEV)
+    for kw, hit in ((dict(), length - 500), (dict(window=300), length - 700), (dict(window=300), length - new - 100)):
+        sees = (pos >= hit) & (pos < hit + kw.get("window", 1 << 30))
+        assert sees.any() and not sees.all()
+        clean = paged.cache_attention(s.q, *s.args(), **kw)
+        page, slot = int(s.table[0, hit // 16]), hit % 16
+        for value in (math.nan, math.inf, -math.inf):
+            keep = s.v[page, 0, slot].clone()
+            s.v[page, 0, slot, 3:11] = value
+            got = paged.cache_attention(s.q, *s.args(), **kw)
+            assert torch.equal(got[~sees], clean[~sees])
+            want = clean[sees].clone()
+            want[..., 3:11] = value
+            assert torch.equal(got[sees].nan_to_num(7, 8, 9), want.nan_to_num(7, 8, 9))
+            s.v[page, 0, slot] = keep
+        keep = s.k[page, 0, slot].clone()
+        s.k[page, 0, slot, 5] = math.nan
+        got = paged.cache_attention(s.q, *s.args(), **kw)
+        assert torch.equal(got[~sees], clean[~sees]) and got[sees].isnan().all()
+        s.k[page, 0, slot] = keep
+        number, first = int(s.table[0, hit // 16]), hit // 16 * 16
+        sees = (pos >= first) & (pos - kw.get("window", 1 << 30) < first + 15)
+        s.table[0, hit // 16] = 1 << 30
+        got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True, **kw)
+        assert torch.equal(got[~sees], clean[~sees]) and got[sees].isnan().all() and lse[sees].isnan().all()
+        s.table[0, hit // 16] = number
+
+
+@pytest.mark.parametrize("length", [50, 3000, 20000])
+@pytest.mark.parametrize("new,group,dim", [(2, 1, 64), (40, 1, 64), (40, 2, 256), (1100, 1, 128)])
+def test_rows_of_infinite_scores(new, group, dim, length):
+    """One score of +inf: NaN, as exp(inf - inf), in the rows that see it.  One of -inf: a key without weight.  All of them -inf: NaN, unlike a row without keys.  Whichever
+    part of a split row has them, and the other rows of their tiles are as they were."""
+    length = max(length, new + 10)
+    s = Served([length], [new], 1, group, dim, 16, BF, seed=dim)
+    s.k[..., 0] = 0                                       # (times 3e38: every score but the one that is set stays as it is)
+    s.q[..., 0] = 3e38
+    clean = paged.cache_attention(s.q, *s.args())
+    pos = torch.arange(length - new, length, device=DEV)
+    for hit in (3, length - new + new // 2):              # a key that all see, in the first part, and one that the later half sees, in the last
+        page, slot, sees = int(s.table[0, hit // 16]), hit % 16, pos >= hit
+        s.k[page, 0, slot, 0] = 3e38
+        got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True)
+        assert got[sees].isnan().all() and not lse[sees].isfinite().any()
+        assert torch.equal(got[~sees], clean[~sees]) and lse[~sees].isfinite().all()
+        s.k[page, 0, slot, 0] = -3e38
+        got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True)
+        keep = s.v[page, 0, slot].clone()
+        s.v[page, 0, slot] = 1000
+        other = paged.cache_attention(s.q, *s.args())
+        assert got.isfinite().all() and lse.isfinite().all() and torch.equal(got, other) and torch.equal(got[~sees], clean[~sees])
+        s.v[page, 0, slot] = keep
+        s.k[page, 0, slot, 0] = 0
+    s.k[..., 0] = -3e38
+    got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True)
+    assert got.isnan().all() and (lse == -math.inf).all()
+
+
 def test_attention_of_nothing():
     s = Served([50, 0, 20], [0, 0, 0], 2, 2, 64, 16, BF)
     assert paged.cache_attention(s.q, *s.args()).shape == (0, 4, 64)
