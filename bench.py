@@ -82,13 +82,18 @@ def cpu_baseline(sd, seconds_budget=30.0, all_cores=False):
 
 
 def source_hash():
-    """Hash of everything libdisco_hip.so is built from (build.SOURCES + HEADERS: every translation unit incl. the per-arithmetic
-    instantiation lists, the packers and the pooling kernels - round 3 hashed four files only)."""
+    """Hash of everything in libdisco_hip.so that the forward is built from: every translation unit incl. the per-arithmetic
+    instantiation lists, the packers and the pooling kernels (build.SOURCES + HEADERS), without the operators of paged caches, which share the library
+    and nothing else, and their section of the C header: the forward's counters and counts do not change with them."""
     from disentangledcolorization_amd import build as B
     h = hashlib.sha256()
-    for f in sorted(B.SOURCES) + sorted(B.HEADERS):
+    for f in sorted(set(B.SOURCES) - set(B.PAGED_SOURCES)) + sorted(set(B.HEADERS) - set(B.PAGED_HEADERS)):
         with open(os.path.join(B.CSRC, f), "rb") as fh:
-            h.update(fh.read())
+            data = fh.read()
+        if f.endswith("disco_hip.h"):
+            at = data.index(b"/* ---- token sequences served from a paged cache")
+            data = data[:at] + data[data.index(b"#ifdef __cplusplus\n}", at):]
+        h.update(data)
     return h.hexdigest()[:16]
 
 

@@ -13,8 +13,10 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdisco_hip.so")
-SOURCES = ["util.cpp", "api_load.cpp", "api_plan.cpp", "api_calib.cpp", "api_diag.cpp", "api_ops.cpp", "conv_pack.cpp", "conv_mx.hip", "conv_mx_ar0.hip", "conv_mx_ar1.hip", "conv_mx_ar2.hip", "conv_mx_ar3.hip", "conv_direct.hip", "color.hip", "spixel.hip", "pool.hip", "tokens.hip", "attention.hip", "kmeans.hip", "anchor_colors.hip", "attention_mfma.hip", "diag.hip",
-           "api_cache.cpp", "rotary.hip", "cache_pages.hip", "cache_attention.hip"]
+SOURCES = ["util.cpp", "api_load.cpp", "api_plan.cpp", "api_calib.cpp", "api_diag.cpp", "api_ops.cpp", "conv_pack.cpp", "conv_mx.hip", "conv_mx_ar0.hip", "conv_mx_ar1.hip", "conv_mx_ar2.hip", "conv_mx_ar3.hip", "conv_direct.hip", "color.hip", "spixel.hip", "pool.hip", "tokens.hip", "attention.hip", "kmeans.hip", "anchor_colors.hip", "attention_mfma.hip", "diag.hip"]
+# the operators of paged caches: in the same library, but no part of the forward (bench.source_hash)
+PAGED_SOURCES = ["api_cache.cpp", "rotary.hip", "cache_pages.hip", "cache_attention.hip"]
+SOURCES += PAGED_SOURCES
 # per-file extra flags
 # -fno-slp-vectorize: the SLP vectoriser forms v_pk_*_f32 with op_sel (the low result half takes the HIGH dword of a source), and on this part
 # that form returns a wrong low half while other waves of the CU issue MFMAs (tools/pk_fault_repro.hip, profiles/r03_pk_fma_op_sel_fault.txt;
@@ -23,9 +25,10 @@ SOURCES = ["util.cpp", "api_load.cpp", "api_plan.cpp", "api_calib.cpp", "api_dia
 EXTRA_FLAGS = {"pool.hip": ["-fno-slp-vectorize"], "spixel.hip": ["-fno-slp-vectorize"], "color.hip": ["-fno-slp-vectorize"],
                "attention_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 # the paged-cache kernels use no packed fp32 instruction of any form (hipcc's host pass says that it does not know the feature: harmless)
-EXTRA_FLAGS.update({f: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for f in ("rotary.hip", "cache_pages.hip", "cache_attention.hip")})
+EXTRA_FLAGS.update({f: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for f in PAGED_SOURCES if f.endswith(".hip")})
 EXTRA_FLAGS["cache_attention.hip"] += ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-HEADERS = ["common.h", "paged.h", "ctx.h", "plan.h", "conv_mx_kernel.h", os.path.join("..", "..", "include", "disco_hip.h")]
+PAGED_HEADERS = ["paged.h"]
+HEADERS = PAGED_HEADERS + ["common.h", "ctx.h", "plan.h", "conv_mx_kernel.h", os.path.join("..", "..", "include", "disco_hip.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-x", "hip", "-Wno-unused-result"]
 

@@ -13,8 +13,6 @@
  *   disco_workspace_bytes             (allocation the reference leaves to torch's caching allocator)
  *   disco_op_*                        the individual stock-PyTorch operators of SURVEY §2b
  *                                     (K1..K16), exposed so each kernel can be parity-tested
- *   disco_op_rotary*, disco_op_cache_*  (no counterpart in the reference) token sequences served from a
- *                                     paged cache: rotary positions, append, attention, pages
  *
  * Conventions
  *   - plain pointers and sizes only; no torch types.  `d_` arguments are DEVICE pointers on the
@@ -421,6 +419,8 @@ int disco_op_mark_color_hints(const float *d_gray, const float *d_target_ab, con
                               float *d_out, int n, int h, int w, int kernel_size, void *stream);
 
 /* ---- token sequences served from a paged cache ---------------------------------------------------------------------
+ * disco_op_rotary*, disco_op_cache_*: no counterpart in the reference (rotary positions, append, attention, pages).
+ *
  * The cache of one model: pages of `page_size` tokens, keys and values apart, bf16 or fp16.  Element (layer, page, head, slot, i) of the keys
  * lies at d_k + layer * layer_stride + page * page_stride + head * head_stride + slot * slot_stride + i (strides in elements, the values with
  * the same ones).  Row b of the page table (int32, rows x table_width, device) names the pages of sequence b, d_lens[b] says how many tokens

@@ -232,3 +232,33 @@ def test_structs_mirror_the_header():
         kinds = {"int32_t": C.c_int32, "int64_t": C.c_int64, "float": C.c_float, "double": C.c_double, "void": C.c_void_p}
         want = [(n.strip().lstrip("*"), kinds[d.split()[0]]) for d in map(str.strip, body.split(";")) if d for n in d.split(None, 1)[1].split(",")]
         assert want == list(py._fields_)
+
+
+def test_the_forwards_records_do_not_go_stale_with_the_paged_cache(tmp_path, monkeypatch):
+    """bench.source_hash keys counters of the forward: a change of these operators, or of their section of the header, leaves it; one of the forward's files does not."""
+    import shutil
+
+    import bench
+    from disentangledcolorization_amd import build as B
+    csrc = tmp_path / "pkg" / "csrc"
+    shutil.copytree(B.CSRC, csrc, ignore=shutil.ignore_patterns("build"))
+    shutil.copytree(os.path.join(REPO, "include"), tmp_path / "include")
+    was = bench.source_hash()
+    monkeypatch.setattr(B, "CSRC", str(csrc))
+    assert bench.source_hash() == was
+    for name in (*B.PAGED_SOURCES, *B.PAGED_HEADERS):
+        with open(csrc / name, "a") as f:
+            f.write("// more\n")
+    header = tmp_path / "include" / "disco_hip.h"
+    text = header.read_text()
+    header.write_text(text.replace("typedef struct disco_cache_desc {", "/* more */\ntypedef struct disco_cache_desc {"))
+    assert header.read_text() != text and bench.source_hash() == was
+    header.write_text(text.replace("#pragma once", "#pragma once\n\n", 1) if "#pragma once" in text else "\n" + text)
+    assert bench.source_hash() != was
+    header.write_text(text)
+    for name in ("conv_mx_kernel.h", "tokens.hip", "util.cpp"):
+        with open(csrc / name, "a") as f:
+            f.write("// more\n")
+        assert bench.source_hash() != was
+        shutil.copy(os.path.join(REPO, "disentangledcolorization_amd", "csrc", name), csrc / name)
+    assert bench.source_hash() == was
