@@ -156,6 +156,7 @@ SIGNATURES = {
     "disco_op_cache_append_reserved": (_I, [C.POINTER(CacheDesc), C.POINTER(AppendDesc), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "disco_op_cache_attention_workspace_bytes": (_I, [C.POINTER(CacheDesc), C.POINTER(AttentionDesc), C.POINTER(_SZ)]),
     "disco_op_cache_attention": (_I, [C.POINTER(CacheDesc), C.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "disco_op_cache_attention_precise": (_I, [C.POINTER(CacheDesc), C.POINTER(AttentionDesc), _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "disco_op_cache_reserve": (_I, [_I, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     "disco_op_cache_select": (_I, [C.POINTER(CacheDesc), _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "disco_op_cache_compact": (_I, [C.POINTER(CacheDesc), _P, _P, _P, _P, _P, _P, _SZ, _P]),

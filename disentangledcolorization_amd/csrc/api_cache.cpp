@@ -133,8 +133,8 @@ int disco_op_cache_attention_workspace_bytes(const disco_cache_desc* c, const di
     return DISCO_OK;
 }
 
-int disco_op_cache_attention(const disco_cache_desc* c, const disco_attention_desc* a, const void* d_q, const int32_t* d_page_table,
-                             const int32_t* d_lens, const int32_t* d_cu_new, void* d_out, float* d_lse, void* d_ws, size_t ws_bytes, void* stream) {
+static int attend(const disco_cache_desc* c, const disco_attention_desc* a, const void* d_q, const int32_t* d_page_table, const int32_t* d_lens,
+                  const int32_t* d_cu_new, void* d_out, float* d_lse, void* d_ws, size_t ws_bytes, bool precise, void* stream) {
     const char* op = "cache_attention";
     if (int rc = check_attention(op, c, a)) return rc;
     if (!a->tokens) return DISCO_OK;
@@ -143,7 +143,17 @@ int disco_op_cache_attention(const disco_cache_desc* c, const disco_attention_de
     const size_t need = cache_attention_ws_bytes(*c, *a);
     if (need && (!d_ws || ws_bytes < need || (uintptr_t)d_ws % 16)) { set_error("%s: workspace too small or not aligned (%zu < %zu)", op, ws_bytes, need); return DISCO_ENOMEM; }
     if (d_q == d_out) return bad_value(op, "out may not be q");
-    return launch_cache_attention(*c, *a, d_q, d_page_table, d_lens, d_cu_new, d_out, d_lse, d_ws, (hipStream_t)stream);
+    return launch_cache_attention(*c, *a, d_q, d_page_table, d_lens, d_cu_new, d_out, d_lse, d_ws, precise, (hipStream_t)stream);
+}
+
+int disco_op_cache_attention(const disco_cache_desc* c, const disco_attention_desc* a, const void* d_q, const int32_t* d_page_table,
+                             const int32_t* d_lens, const int32_t* d_cu_new, void* d_out, float* d_lse, void* d_ws, size_t ws_bytes, void* stream) {
+    return attend(c, a, d_q, d_page_table, d_lens, d_cu_new, d_out, d_lse, d_ws, ws_bytes, false, stream);
+}
+
+int disco_op_cache_attention_precise(const disco_cache_desc* c, const disco_attention_desc* a, const void* d_q, const int32_t* d_page_table,
+                                     const int32_t* d_lens, const int32_t* d_cu_new, void* d_out, float* d_lse, void* d_ws, size_t ws_bytes, void* stream) {
+    return attend(c, a, d_q, d_page_table, d_lens, d_cu_new, d_out, d_lse, d_ws, ws_bytes, true, stream);
 }
 
 int disco_op_cache_reserve(int rows, int table_width, int pages, int page_size, const int32_t* d_page_table, const int32_t* d_lens,

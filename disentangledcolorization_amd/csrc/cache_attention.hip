@@ -611,7 +611,12 @@ template <int DP> __device__ __forceinline__ int value_piece(int row, int piece)
 template <int DP> constexpr int tile_keys() { return DP <= 128 ? 64 : 32; }
 template <int DP> constexpr int many_lds() { return 4 * tile_keys<DP>() * DP * 2; }
 
-template <typename T, int DP, int FORM, bool ODD>
+// REST: what the rounding of the probabilities to the cache's type leaves is multiplied as well, as in the form of few rows.  There it costs nothing, here the
+// matrix cores have no time left: 2 048 tokens behind 16 384 keys (32 heads of 128 on 8) take 554 us without and 750 with it, chunks of up to 257 over 4 111
+// keys (12 heads of 64 on 4) 90 and 104, a window of 1 024 (8 heads of 256 on 2) 57 and 60.  Without it a result is off by half a step of the cache's type
+// at most (of the weighted |v|), which is what rounding the result takes anyway (bf16 chunk: 0.0023 instead of 0.0017 over all elements); so the caller
+// asks for it.
+template <typename T, int DP, int FORM, bool ODD, bool REST>
 __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds) {
     typedef typename Mat<T>::x8 x8;
     constexpr int ROWS = rows_of(FORM), KT = tile_keys<DP>(), SUB = KT / 32, KS = DP / 16, DB = DP / 32, ROW = DP * 2, BUF = KT * ROW, STEP = 32 * ROWS, NP = (BUF + STEP - 1) / STEP;
@@ -666,7 +671,7 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
     auto tile = [&](auto masked, int k0, const char* kb, const char* vb, unsigned long long bad) {
         constexpr bool MASKED = decltype(masked)::value;
         f32x16 s[SUB];
-        x8 p[SUB][2];
+        x8 p[SUB][2], rest[SUB][2];                                // (rest: only with REST)
         uint32_t seen[SUB] = {};
         auto scores = [&] {
 #pragma unroll
@@ -700,6 +705,7 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
                     const float e = exp2_of(fmaf(s[t][j], a->c, -base));
                     sum += e;
                     p[t][j >> 3][j & 7] = (T)e;
+                    if (REST) rest[t][j >> 3][j & 7] = (T)(e - (float)p[t][j >> 3][j & 7]);
                 }
             return sum;
         };
@@ -731,8 +737,9 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
         for (int x = 0; x < SUB * 2 * DB; ++x) {
             const int t = x / (2 * DB), m = x / DB % 2, i = x % DB;
             const x8 v = value(t, m, i);
-            if (ODD && MASKED) o[i] = multiply_seen<T, false>(v, p[t][m], p[t][m], seen[t] >> (8 * m), o[i]);
+            if (ODD && MASKED) o[i] = multiply_seen<T, REST>(v, p[t][m], rest[t][m], seen[t] >> (8 * m), o[i]);
             else o[i] = Mat<T>::mul(v, p[t][m], o[i]);
+            if (REST && !(ODD && MASKED)) o[i] = Mat<T>::mul(v, rest[t][m], o[i]);
         }
     };
     int pg = 0, pg_next = 0;
@@ -811,19 +818,19 @@ __device__ __forceinline__ uint32_t many_unit(ArgsAt a, const Unit& u, char* lds
     return odd;
 }
 
-template <typename T, int DP, int FORM>
+template <typename T, int DP, int FORM, bool REST>
 __device__ __noinline__ void many_unit_odd(uint64_t args, int want, uint32_t lds) {
     const ArgsAt a = args_at(args);
     Unit u;
     Cursor c{0, 0};
     if (!find_unit<FORM>(a, __builtin_amdgcn_readfirstlane(want), c, u)) return;
     for (; u.parts > 0; --u.parts, ++u.split, u.begin += u.cut.chunk) {
-        many_unit<T, DP, FORM, true>(a, u, lds_pointer(lds));
+        many_unit<T, DP, FORM, true, REST>(a, u, lds_pointer(lds));
         __syncthreads();
     }
 }
 
-template <typename T, int DP, int FORM>
+template <typename T, int DP, int FORM, bool REST>
 __global__ __launch_bounds__(2 * rows_of(FORM), DP <= 128 ? 2 : 1) void cache_attention_many_kernel(AttnArgs) {
     const ArgsAt a = (ArgsAt)__builtin_amdgcn_kernarg_segment_ptr();
     extern __shared__ __align__(16) char lds[];
@@ -836,8 +843,8 @@ __global__ __launch_bounds__(2 * rows_of(FORM), DP <= 128 ? 2 : 1) void cache_at
         Unit u;
         if (!find_unit<FORM>(fresh(a), want, c, u)) break;
         int odd = 0;
-        for (; u.parts > 0; --u.parts, ++u.split, u.begin += u.cut.chunk) odd |= __syncthreads_or(many_unit<T, DP, FORM, false>(fresh(a), u, lds) != 0);
-        if (odd) many_unit_odd<T, DP, FORM>(kernel_args(), want, lds_offset(lds));
+        for (; u.parts > 0; --u.parts, ++u.split, u.begin += u.cut.chunk) odd |= __syncthreads_or(many_unit<T, DP, FORM, false, REST>(fresh(a), u, lds) != 0);
+        if (odd) many_unit_odd<T, DP, FORM, REST>(kernel_args(), want, lds_offset(lds));
     }
 }
 
@@ -1069,20 +1076,20 @@ unsigned grid_for(long units, long most) { return (unsigned)(units < 1 ? 1 : (un
 // More workgroups than are resident at once: under a causal mask tiles differ in length, and the next one, the longest that is left, goes where one has
 // ended (8 192 tokens of 32 heads of 128 on 8: 657 us with 256 workgroups of the large form, 583 with 1 024, as with 2 048, of which more lie idle in
 // a call of short sequences: the bound on units is the host's).
-template <typename T, int DP, int FORM>
+template <typename T, int DP, int FORM, bool REST>
 int run_many(const AttnArgs& a, long units, hipStream_t s) {
     static_assert(many_lds<DP>() <= 65536, "more LDS has to be asked for");
-    cache_attention_many_kernel<T, DP, FORM><<<grid_for(units, 1024), 2 * rows_of(FORM), many_lds<DP>(), s>>>(a);
+    cache_attention_many_kernel<T, DP, FORM, REST><<<grid_for(units, 1024), 2 * rows_of(FORM), many_lds<DP>(), s>>>(a);
     DISCO_LAUNCH_CHECK("cache_attention_many_kernel");
     return DISCO_OK;
 }
 
 template <typename T, int DP>
-int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
+int run_forms(const AttnArgs& a, const Plan& p, bool precise, hipStream_t s) {
     if constexpr (DP > 64 && DP <= 128) {
-        if (p.large) if (int rc = run_many<T, DP, LARGE>(a, p.large_units, s)) return rc;
+        if (p.large) if (int rc = precise ? run_many<T, DP, LARGE, true>(a, p.large_units, s) : run_many<T, DP, LARGE, false>(a, p.large_units, s)) return rc;
     }
-    if (p.many) if (int rc = run_many<T, DP, MANY>(a, p.many_units, s)) return rc;
+    if (p.many) if (int rc = precise ? run_many<T, DP, MANY, true>(a, p.many_units, s) : run_many<T, DP, MANY, false>(a, p.many_units, s)) return rc;
     if (p.few) {
         cache_attention_few_kernel<T, DP><<<grid_for(p.few_units, 256 * few_waves(DP)), 256, 0, s>>>(a);
         DISCO_LAUNCH_CHECK("cache_attention_few_kernel");
@@ -1101,13 +1108,13 @@ int run_forms(const AttnArgs& a, const Plan& p, hipStream_t s) {
 }
 
 template <typename T>
-int run_dims(const AttnArgs& a, const Plan& p, hipStream_t s) {
-    if (a.dim <= 32) return run_forms<T, 32>(a, p, s);
-    if (a.dim <= 64) return run_forms<T, 64>(a, p, s);
-    if (a.dim <= 96) return run_forms<T, 96>(a, p, s);
-    if (a.dim <= 128) return run_forms<T, 128>(a, p, s);
-    if (a.dim <= 192) return run_forms<T, 192>(a, p, s);
-    return run_forms<T, 256>(a, p, s);
+int run_dims(const AttnArgs& a, const Plan& p, bool precise, hipStream_t s) {
+    if (a.dim <= 32) return run_forms<T, 32>(a, p, precise, s);
+    if (a.dim <= 64) return run_forms<T, 64>(a, p, precise, s);
+    if (a.dim <= 96) return run_forms<T, 96>(a, p, precise, s);
+    if (a.dim <= 128) return run_forms<T, 128>(a, p, precise, s);
+    if (a.dim <= 192) return run_forms<T, 192>(a, p, precise, s);
+    return run_forms<T, 256>(a, p, precise, s);
 }
 
 }  // namespace
@@ -1118,7 +1125,7 @@ size_t cache_attention_ws_bytes(const disco_cache_desc& c, const disco_attention
 }
 
 int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc& d, const void* q, const int* table, const int* lens,
-                           const int* cu_new, void* out, float* lse, void* ws, hipStream_t s) {
+                           const int* cu_new, void* out, float* lse, void* ws, bool precise, hipStream_t s) {
     const Plan p = plan_of(c, d);
     const size_t parts = (size_t)(p.few_parts + p.many_parts);
     const int window = d.window >= (long)c.table_width * c.page_size ? 0 : d.window;      // (no key is that far back)
@@ -1127,7 +1134,7 @@ int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc
                d.tokens, d.q_heads, c.kv_heads, d.q_heads / c.kv_heads, c.dim, c.rows, c.table_width, c.pages, __builtin_ctz((unsigned)c.page_size), d.causal,
                window, p.few_splits, p.many_splits, p.few_by_sequence, p.few_fold, p.many_fold, p.many_room, p.few_parts, p.few_limit, p.many_limit, fabsf(d.scale) * 1.4426950408889634f, d.scale < 0};
     if (a.c < 1e-37f) a.c = 1e-37f;                                // 0 * -inf is not the score of a key that is not seen
-    return c.dtype == DISCO_F16 ? run_dims<f16>(a, p, s) : run_dims<bf16>(a, p, s);
+    return c.dtype == DISCO_F16 ? run_dims<f16>(a, p, precise, s) : run_dims<bf16>(a, p, precise, s);
 }
 
 }  // namespace disco

@@ -33,7 +33,7 @@ int launch_cache_append(const disco_cache_desc& c, const disco_append_desc& a, c
 
 size_t cache_attention_ws_bytes(const disco_cache_desc& c, const disco_attention_desc& a);
 int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc& a, const void* q, const int* table, const int* lens,
-                           const int* cu_new, void* out, float* lse, void* ws, hipStream_t s);
+                           const int* cu_new, void* out, float* lse, void* ws, bool precise, hipStream_t s);
 
 int launch_cache_reserve(int rows, int width, int pages, int page_shift, const int* table, const int* lens, const int* refs, const int* cu_new,
                          int* table_out, int* lens_out, int* refs_out, int* info, hipStream_t s);

@@ -611,6 +611,57 @@ def test_rows_of_infinite_scores(new, group, dim, length):
     assert got.isnan().all() and (lse == -math.inf).all()
 
 
+PRECISE = [([300], [130], 2, 2, 128), ([129], [100], 1, 4, 256), ([333, 20], [77, 20], 1, 1, 192), ([200, 90], [64, 3], 2, 1, 96), ([31, 32, 33, 64, 65, 1], [5, 1, 33, 2, 65, 1], 2, 3, 64),
+           ([5000, 700], [40, 60], 1, 2, 32), ([1300], [1300], 1, 1, 128), ([20000, 90], [1100, 1], 1, 1, 80)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("case", PRECISE)
+@pytest.mark.parametrize("kw", [dict(), dict(window=100)])
+def test_precise_attention(case, dtype, kw):
+    """Weights of fp32 precision in every form.  What is left of them after two roundings is 2^-16 (bf16) and, as long as it stays above fp16's smallest step, 2^-22; the result
+    is rounded once.  A value of 2^-9 of the weighted |v| (half a step of bf16 weights) would not pass."""
+    lens, new, kv_heads, group, dim = case
+    s = Served(lens, new, kv_heads, group, dim, 16, dtype, seed=dim)
+    got, lse = paged.cache_attention(s.q, *s.args(), return_lse=True, precise=True, **kw)
+    plain, sums = paged.cache_attention(s.q, *s.args(), return_lse=True, **kw)
+    assert torch.equal(lse, sums)
+    for b, n in enumerate(new):
+        at = int(s.cu[b])
+        if n * group <= 16:
+            assert torch.equal(got[at:at + n], plain[at:at + n])
+        m = min(n, 6)
+        for i in {0, n - m}:
+            rows, length = slice(at + i, at + i + m), lens[b] - n + i + m
+            want, size, _, off = R.attended(s.q[rows], s.k, s.v, s.table[b:b + 1], torch.tensor([length]), torch.tensor([0, m]), **kw)
+            left = 2.0 ** -16 if dtype == BF else 2.0 ** -21
+            tiny = length * 2.0 ** -25 * 2.0 ** -6 * s.v.double().nan_to_num(0, 0, 0).abs().max().item() if dtype == HF else 0.0
+            tol = half(dtype) * want.abs() + (left + 2 * off[..., None] + 2.0 ** -20) * size + tiny + torch.finfo(dtype).smallest_normal
+            assert ((got[rows].double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("new,dim", [(40, 64), (1100, 128)])
+def test_precise_attention_and_what_is_not_seen(new, dim):
+    """Values that are not finite, and pages outside the cache, as without it."""
+    s = Served([1500], [new], 1, 1, dim, 16, BF, seed=dim)
+    pos, hit = torch.arange(1500 - new, 1500, device=DEV), 1500 - new // 2
+    sees = pos >= hit
+    clean = paged.cache_attention(s.q, *s.args(), precise=True)
+    page, slot = int(s.table[0, hit // 16]), hit % 16
+    for value in (math.nan, math.inf, -math.inf):
+        keep = s.v[page, 0, slot].clone()
+        s.v[page, 0, slot, 3:11] = value
+        got = paged.cache_attention(s.q, *s.args(), precise=True)
+        want = clean[sees].clone()
+        want[..., 3:11] = value
+        assert torch.equal(got[~sees], clean[~sees]) and torch.equal(got[sees].nan_to_num(7, 8, 9), want.nan_to_num(7, 8, 9))
+        s.v[page, 0, slot] = keep
+    s.table[0, hit // 16] = -1
+    got = paged.cache_attention(s.q, *s.args(), precise=True)
+    sees = pos >= hit // 16 * 16
+    assert torch.equal(got[~sees], clean[~sees]) and got[sees].isnan().all()
+
+
 def test_attention_of_nothing():
     s = Served([50, 0, 20], [0, 0, 0], 2, 2, 64, 16, BF)
     assert paged.cache_attention(s.q, *s.args()).shape == (0, 4, 64)

@@ -103,6 +103,15 @@ def test_bad_attention_is_refused(lib, kw):
     assert lib.disco_op_cache_attention_workspace_bytes(C.byref(c), C.byref(a), C.byref(n)) in (-1, -2)
 
 
+@pytest.mark.parametrize("kw", [dict(tokens=-1), dict(q_heads=3), dict(window=-1), dict(scale=math.nan), dict(q_token=4)])
+def test_bad_precise_attention_is_refused(lib, kw):
+    d = dict(tokens=4, q_heads=4, causal=1, window=0, max_new=0, max_len=0, scale=0.125, q_token=256, q_head=64, out_token=256, out_head=64)
+    d.update(kw)
+    a, c, p = _ffi.AttentionDesc(*[d[f] for f, _ in _ffi.AttentionDesc._fields_]), cache(), C.c_void_p(1 << 20)
+    assert lib.disco_op_cache_attention_precise(C.byref(c), C.byref(a), p, p, p, p, p, None, p, 1 << 40, None) in (-1, -2)
+    assert lib.disco_op_cache_attention_precise(None, C.byref(a), p, p, p, p, p, None, p, 1 << 40, None) == -1
+
+
 def test_more_heads_than_units_can_be_counted_for(lib):
     c, p, n = cache(kv_heads=1025), C.c_void_p(1 << 20), C.c_size_t()
     a = _ffi.AttentionDesc(4, 1025, 1, 0, 0, 0, 0.125, 1025 * 64, 64, 1025 * 64, 64)
