@@ -267,6 +267,16 @@ __global__ __launch_bounds__(PLAN) void cache_select_plan_kernel(PlanArgs a) {
     const Counts<LOCAL> counts{LOCAL ? keeper + a.rows : a.refs_out};
     if (tid == 0) bad = LOCAL ? 0 : *a.bad;
     for (int r = tid; r < a.rows; r += PLAN) keeper[r] = 1 << 30;
+    // what row r becomes: its parent, its length, how much of a last page that is not full, and that page (the thread's first row is looked up once)
+    struct Last { int parent, len, filled, page; };
+    auto last_of = [&](int r) {
+        Last x{r < a.rows ? parent_of(a, r) : -1, 0, 0, -1};
+        if (x.parent >= 0) x.len = clamp_len(a.lens[x.parent], capacity);
+        x.filled = x.len & ((1 << a.shift) - 1);
+        if (x.filled) x.page = a.table[(long)x.parent * a.width + (x.len >> a.shift)];
+        return x;
+    };
+    const Last first = last_of(tid);
     __syncthreads();
     if constexpr (LOCAL) count_here<true>(a, counts, &bad);
     for (int r = tid; r < a.rows; r += PLAN) {
@@ -278,30 +288,26 @@ __global__ __launch_bounds__(PLAN) void cache_select_plan_kernel(PlanArgs a) {
     // A page that is full for some row (whose neighbours have been cut back into it) has a count and stays that row's: all that end in it need copies.
     auto asked = [&](int r, int p) { return (p == r ? r : a.rows + r) - (1 << 30); };
     for (int r = tid; r < a.rows; r += PLAN) {
-        const int p = parent_of(a, r), len = p < 0 ? 0 : clamp_len(a.lens[p], capacity);
-        if (!(len & ((1 << a.shift) - 1))) continue;
-        const int page = a.table_out[(long)r * a.width + (len >> a.shift)];
-        if (page >= 0 && page < a.pages && counts.get(page) <= 0) counts.lower(page, asked(r, p));
+        const Last x = r == tid ? first : last_of(r);
+        if (x.filled && x.page >= 0 && x.page < a.pages && counts.get(x.page) <= 0) counts.lower(x.page, asked(r, x.parent));
     }
-    settle();
+    if (LOCAL) __syncthreads();
+    else settle();
     // the keeper's is in use, the others need copies, numbered by row
     int need = 0;
     for (int r0 = 0; r0 < a.rows; r0 += PLAN) {
-        const int r = r0 + tid, p = r < a.rows ? parent_of(a, r) : -1;
-        const int len = p < 0 ? 0 : clamp_len(a.lens[p], capacity), filled = len & ((1 << a.shift) - 1);
-        bool keeps = p >= 0 && keeper[p] == (p == r ? -1 : r);     // (of a page outside the cache)
-        int page = -1, all;
-        if (filled) {
-            page = a.table_out[(long)r * a.width + (len >> a.shift)];
-            if (page >= 0 && page < a.pages) {
-                keeps = counts.get(page) == asked(r, p);           // (who finds 1 there comes behind the keeper)
-                if (keeps) counts.set(page, 1);
-            }
+        const int r = r0 + tid;
+        const Last x = r0 ? last_of(r) : first;
+        bool keeps = x.parent >= 0 && keeper[x.parent] == (x.parent == r ? -1 : r);     // (of a page outside the cache)
+        if (x.filled && x.page >= 0 && x.page < a.pages) {
+            keeps = counts.get(x.page) == asked(r, x.parent);      // (who finds 1 there comes behind the keeper)
+            if (keeps) counts.set(x.page, 1);
         }
-        const bool asks = filled && !keeps;
+        int all;
+        const bool asks = x.filled && !keeps;
         const int rank = need + block_scan(asks, part, &all) - 1;
-        if (asks) a.copies[rank] = Copy{page, -1, filled, r};      // (a page outside the cache is left out by the copy)
-        if (r < a.rows) a.lens_out[r] = len;
+        if (asks) a.copies[rank] = Copy{x.page, -1, x.filled, r};  // (a page outside the cache is left out by the copy)
+        if (r < a.rows) a.lens_out[r] = x.len;
         need += all;
     }
     settle();
