@@ -8,7 +8,8 @@
 // but that between the lanes of a column, and the registers that hold the probabilities are in place the operand of O^T = V^T P^T (their key order
 // is the accumulator's; V^T is read in the same order by the transposing LDS read).
 //
-// Three forms, chosen by a sequence's own rows (new tokens * group), so that its result does not depend on what else is in the call:
+// Three forms, chosen by a sequence's own rows (new tokens * group), so that its result does not depend on what else is in the call (rows of no sequence
+// included, unless the caller has said that there are none):
 //   few (up to 16 rows)    cache_attention_few_kernel: 16 rows a workgroup, its four waves deal 32-key tiles; bound by reading the cache
 //   many                   cache_attention_many_kernel, 128 rows a workgroup, 32 a wave, keys and values staged in LDS for all of them; two workgroups
 //                          a CU, bound by what L2 delivers into LDS (7 TB/s over the chip) and, at short ranges, by latency
@@ -38,7 +39,7 @@ template <typename T> struct Mat;
 template <> struct Mat<f16> {
     typedef f16x8 x8;
     static constexpr uint32_t INF = 0x7c00, ONE = 0x3c00;
-    // probabilities below 2^-14 lose bits in fp16, so all of a row are 2^6 larger (at most 2^14: see the rescale)
+    // probabilities below 2^-14 lose bits in fp16, so all of a row are 2^6 larger (at most 2^15: Run::LIMIT)
     static constexpr float BIAS = 6.f;
     static __device__ __forceinline__ f32x16 mul(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x4 mul(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }

@@ -14,8 +14,8 @@ it holds, `refs` (pages,) int32 how many rows name a page (0: free).  The new to
     page_table, refs, info = cache_compact(page_table, lens, k_cache, v_cache)
 
 Serving only: nothing here is differentiable, and tensors that ask for a gradient are refused (`rotary(inverse=True)` is the transposed
-rotation).  No call synchronises; on the current stream of the tensors' device all of them may be captured into a graph.  No CPU fallback:
-CPU tensors raise DiscoError.
+rotation).  Only rotary_frequencies synchronises, as its table is made on the host: it comes once, ahead of the steps.  All others run on the current stream of
+the tensors' device and may be captured into a graph.  No CPU fallback: CPU tensors raise DiscoError.
 
 Whether there were pages enough only the GPU knows when a step is under way: info[1] tells, and cache_append, given info, leaves the cache of
 a step that found none as it was (what cache_attention then returns is not the new tokens').  The program looks at info when it suits it, frees pages and does

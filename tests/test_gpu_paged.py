@@ -376,6 +376,19 @@ def test_one_sequence_is_cut_by_its_own_rows(new, group, dim):
                 assert torch.equal(got[:new], want) and torch.equal(lse[:new], sums), (rows, kw)
 
 
+@pytest.mark.parametrize("group,dim", [(2, 64), (16, 128)])
+@pytest.mark.parametrize("new", [1, 5, 33])
+def test_one_sequence_of_fewer_tokens_than_promised(new, group, dim):
+    """max_new = tokens says that all rows are new tokens.  Where it is wrong the values are right all the same."""
+    s = Served([9000], [new], 1, group, dim, 16, BF, seed=new)
+    for rows in (40, 1500):
+        q = torch.cat((s.q, s.q.new_full((rows - new, *s.q.shape[1:]), math.nan)))
+        out = torch.full_like(q, 3.0)
+        got, lse = paged.cache_attention(q, *s.args(), out=out, return_lse=True, max_new=rows)
+        assert (got[new:] == 3).all()
+        close_attended(got, lse, s.q, *s.args())
+
+
 def test_a_mixed_call_with_long_prompts():
     """Every form in one call, keys split in each: long prompts, chunks, single tokens, idle rows, and parts kept by sequence and by token."""
     s = Served([3000, 5000, 0, 900, 2600, 40, 1200], [600, 1, 0, 70, 9, 3, 1100], 1, 2, 64, 16, BF, seed=3)
