@@ -1051,9 +1051,9 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     }
     // Room for the parts: of every token's rows, or where that is less of every sequence's, which has at most FEW_LIMIT rows a key head there, and here, where
     // its keys are split, at most 65 536 parts of rows (tiles * key heads * parts <= 512 of 128 rows, or 256 of 256) or two of each row of < 512 tiles.
-    // Where a form would take more than ROOM bytes, its workgroups compute whole groups of parts and keep one slot a group; there are sequences enough then
-    // to fill the GPU.  32 heads of 128 on 8, tables of 32 768, no bound on the lengths: 256 sequences of 17 tokens over 2 000 keys 633 us and 0.75 GB (a slot a
-    // part: 625 and 5.8), 1 000 single tokens over 1 024 1 024 us and 0.27 GB (929 and 2.1), 300 of 500 and one of 65 536 317 us (233).
+    // Where a form would take more than ROOM bytes, and less than half of that with one slot a group, its workgroups compute whole groups of parts; there are
+    // sequences enough then to fill the GPU.  32 heads of 128 on 8, tables of 32 768, no bound on the lengths: 256 sequences of 17 tokens over 2 000 keys 633 us
+    // and 0.7 GB (a slot a part: 625 and 5.8), 1 000 single tokens over 1 024 1 024 us and 0.27 GB (929 and 2.1), 300 of 500 and one of 65 536 317 us (233).
     const long rows = (long)d.tokens * group, heads = (long)d.tokens * d.q_heads;
     p.few_by_sequence = p.few_limit == FEW_LIMIT && (long)c.rows * c.kv_heads * FEW_LIMIT < heads;
     const long bytes = (long)c.dim * 4 + 8, few_rows = p.few_by_sequence ? (long)c.rows * c.kv_heads * FEW_LIMIT : heads;
@@ -1061,10 +1061,12 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     p.few_parts = p.few_splits > 1 ? few_rows * slots_of(p.few_splits, p.few_fold) : 0;
     const long twice = 2 * c.kv_heads * (p.large ? MANY_LIMIT : rows);
     const int room = twice <= 65536 ? 65536 : (twice < 131072 ? (int)twice : 131072);
-    p.many_fold = std::min((long)c.rows * room, heads * p.many_splits) * bytes > ROOM ? FOLD : 0;
-    const int many_slots = slots_of(p.many_splits, p.many_fold), many_room = p.many_fold ? 65536 : room;      // (two parts are one slot)
-    p.many_room = (long)c.rows * many_room < heads * many_slots ? many_room : 0;
-    p.many_parts = p.many_splits > 1 ? (p.many_room ? (long)c.rows * many_room : heads * many_slots) : 0;
+    const auto many = [&](int fold) {                              // (the two parts of a row of < 512 tiles are one slot)
+        return std::min((long)c.rows * (fold ? 65536 : room), heads * slots_of(p.many_splits, fold));
+    };
+    p.many_fold = many(0) * bytes > ROOM && 2 * many(FOLD) <= many(0) ? FOLD : 0;
+    p.many_parts = p.many_splits > 1 ? many(p.many_fold) : 0;
+    p.many_room = many(p.many_fold) < heads * slots_of(p.many_splits, p.many_fold) ? (p.many_fold ? 65536 : room) : 0;
     const long some = c.rows < d.tokens ? c.rows : d.tokens;
     p.few_units = (some + (p.few_limit == FEW_LIMIT ? 0 : rows / rows_of(FEW))) * p.few_splits * c.kv_heads;      // (at most FEW_LIMIT rows are one tile)
     p.many_units = (some + rows / rows_of(MANY)) * p.many_splits * c.kv_heads;

@@ -470,11 +470,11 @@ def test_attention_workspace_of_many_sequences(rows, tokens, width):
         assert 0 < n.value < most
 
 
-@pytest.mark.parametrize("kv_heads,group,dim,dtype", [(2, 4, 64, BF), (1, 8, 128, BF), (2, 4, 128, HF), (1, 3, 256, HF)])
-def test_groups_of_parts_have_the_bits_of_parts(kv_heads, group, dim, dtype):
+@pytest.mark.parametrize("rows,kv_heads,group,dim,dtype", [(2200, 2, 4, 64, BF), (2200, 1, 8, 128, BF), (2200, 2, 4, 128, HF), (2200, 1, 3, 256, HF), (13200, 64, 1, 8, HF)])
+def test_groups_of_parts_have_the_bits_of_parts(rows, kv_heads, group, dim, dtype):
     """A call of so many sequences that its workgroups add up groups of parts themselves: every form, windows, values that are not finite, pages outside the
     cache; bit for bit what each sequence has alone, where a join adds them up."""
-    rows, page, keys = 2200, 64, 30000
+    page, keys = 64, 30000
     lens, new = [70] * rows, [1] * rows
     for b, (n, m) in enumerate([(30000, 1), (9001, 2), (20000, 20), (700, 1), (29999, 60), (12345, 700 // group), (25000, 3000 // group), (26000, 5), (24000, 33), (17000, 400)]):
         lens[3 * b], new[3 * b] = n, m
