@@ -89,8 +89,8 @@ __device__ __forceinline__ int scan_pages(int pages, int* part, Look look, Then 
 
 // ---- reserve ------------------------------------------------------------------------------------------------------------------------
 // Block 0 plans: the rows' needs (scanned into LDS), the free pages in ascending order, each finding its row by bisection.  The other blocks copy the
-// entries that every row has already; who writes an entry depends on the input alone, so nothing waits.  Bound by latency: one launch of 4 us (64 rows
-// that take a token each) to 8 (five that take 80 pages each).
+// entries that every row has already; who writes an entry depends on the input alone, so nothing waits.  Bound by latency: one launch of 5 us (five rows
+// that take 80 pages each) to 8 (64 that take a token each, over tables of 4 096 tokens).
 struct ReserveArgs {
     const int *table, *lens, *refs, *cu_new;
     int *table_out, *lens_out, *refs_out, *info;
