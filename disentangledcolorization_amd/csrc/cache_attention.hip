@@ -1010,7 +1010,7 @@ __global__ __launch_bounds__(256) void cache_attention_join_row_kernel(AttnArgs 
 
 // ---- what the host decides ----------------------------------------------------------------------------------------------------------------------
 constexpr int FEW_LIMIT = 16, MANY_LIMIT = 1024;
-constexpr long ROOM = 256l << 20;
+constexpr long ROOM = 512l << 20;
 
 struct Plan {
     bool few, many, large;             // which forms are launched
@@ -1052,8 +1052,9 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     // Room for the parts: of every token's rows, or where that is less of every sequence's, which has at most FEW_LIMIT rows a key head there, and here, where
     // its keys are split, at most 65 536 parts of rows (tiles * key heads * parts <= 512 of 128 rows, or 256 of 256) or two of each row of < 512 tiles.
     // Where a form would take more than ROOM bytes, and less than half of that with one slot a group, its workgroups compute whole groups of parts; there are
-    // sequences enough then to fill the GPU.  32 heads of 128 on 8, tables of 32 768, no bound on the lengths: 256 sequences of 17 tokens over 2 000 keys 633 us
-    // and 0.7 GB (a slot a part: 625 and 5.8), 1 000 single tokens over 1 024 1 024 us and 0.27 GB (929 and 2.1), 300 of 500 and one of 65 536 317 us (233).
+    // sequences enough then to fill the GPU.  32 heads of 128 on 8, tables of 32 768, no bound on the lengths: 256 sequences of 17 tokens over 2 000 keys 649 us
+    // and 0.7 GB (a slot a part: 625 and 5.8), 1 000 single tokens over 1 024 983 us and 0.27 GB (929 and 2.1).  One long sequence among many pays most: 300 of
+    // 500 keys and one of 65 536, 0.3 GB, 200 us as it is, in groups 287; so ROOM is not smaller.
     const long rows = (long)d.tokens * group, heads = (long)d.tokens * d.q_heads;
     p.few_by_sequence = p.few_limit == FEW_LIMIT && (long)c.rows * c.kv_heads * FEW_LIMIT < heads;
     const long bytes = (long)c.dim * 4 + 8, few_rows = p.few_by_sequence ? (long)c.rows * c.kv_heads * FEW_LIMIT : heads;

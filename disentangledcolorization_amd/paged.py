@@ -218,7 +218,7 @@ def cache_attention(q, k_cache, v_cache, page_table, lens, cu_new, causal=True, 
     max_new, max_len: what the caller knows of the largest number of new tokens and the largest length; they size launches and
     workspace, a sequence beyond them still comes out right.  With one row in the table, max_new = tokens says that every row of q is a new token of
     its sequence: fewer launches (a padded call leaves max_new out, or gives less).  Steps of hundreds of sequences over
-    wide tables should give max_len: without it they take up to a gigabyte of workspace, and up to a third longer.  return_lse: also the logarithm of the softmax's sum, (tokens, q_heads)
+    wide tables should give max_len: without it they take up to a gigabyte of workspace, and up to a quarter longer.  return_lse: also the logarithm of the softmax's sum, (tokens, q_heads)
     fp32.  `out` shares no memory with q.  Rows of no sequence are left as they are in a given `out`, and undefined in lse and an `out` of its own."""
     device = _device((q, k_cache, v_cache), (page_table, lens, cu_new))
     c = _cache(k_cache, v_cache, page_table)

@@ -470,7 +470,7 @@ def test_attention_workspace_of_many_sequences(rows, tokens, width):
         assert 0 < n.value < most
 
 
-@pytest.mark.parametrize("rows,kv_heads,group,dim,dtype", [(2200, 2, 4, 64, BF), (2200, 1, 8, 128, BF), (2200, 2, 4, 128, HF), (2200, 1, 3, 256, HF), (13200, 64, 1, 8, HF)])
+@pytest.mark.parametrize("rows,kv_heads,group,dim,dtype", [(6000, 2, 4, 64, BF), (6000, 1, 8, 128, BF), (6000, 2, 4, 128, HF), (6000, 1, 3, 256, HF), (16000, 64, 1, 16, HF)])
 def test_groups_of_parts_have_the_bits_of_parts(rows, kv_heads, group, dim, dtype):
     """A call of so many sequences that its workgroups add up groups of parts themselves: every form, windows, values that are not finite, pages outside the
     cache; bit for bit what each sequence has alone, where a join adds them up."""
