@@ -1282,6 +1282,33 @@ def test_captured_page_calls_over_large_pools(rows, pages):
             assert torch.equal(x, y)
 
 
+def test_captured_groups_of_parts_and_two_streams():
+    """A call whose workgroups add parts up, replayed over lengths that change, with another such call on a second stream meanwhile."""
+    rows, pages, page, g = 6000, 400, 64, gen(3)
+    table = torch.stack([torch.randperm(pages, generator=g) for _ in range(40)]).int().repeat(rows // 40, 1).to(DEV)
+    k, v = (torch.randn(pages, 2, page, 64, generator=g).to(BF).to(DEV) for _ in range(2))
+    q, cu, lens = torch.randn(rows, 8, 64, generator=g).to(BF).to(DEV), ints(list(range(rows + 1))), ints([50] * rows)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        paged.cache_attention(q, k, v, table, lens, cu)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = paged.cache_attention(q, k, v, table, lens, cu)
+    other = ints([9000 if b % 1000 == 7 else 3 for b in range(rows)])
+    want_other = paged.cache_attention(q, k, v, table, other, cu)
+    for step in range(3):
+        lens.copy_(ints([25000 - 4000 * step if b % 999 == 1 else 10 + step for b in range(rows)]))
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(stream):
+            beside = paged.cache_attention(q, k, v, table, other, cu)
+        torch.cuda.synchronize()
+        now = got.clone()
+        assert torch.equal(beside, want_other) and torch.equal(now, paged.cache_attention(q, k, v, table, lens, cu))
+
+
 def test_other_streams_and_calls_at_once():
     """Each call runs on the current stream; calls on several streams at once have workspaces of their own."""
     s = [Served([3000 + 7 * i, 40], [1, 30], 2, 4, 64, 16, BF, seed=i) for i in range(4)]
