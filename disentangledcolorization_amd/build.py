@@ -15,7 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdisco_hip.so")
 SOURCES = ["util.cpp", "api_load.cpp", "api_plan.cpp", "api_calib.cpp", "api_diag.cpp", "api_ops.cpp", "conv_pack.cpp", "conv_mx.hip", "conv_mx_ar0.hip", "conv_mx_ar1.hip", "conv_mx_ar2.hip", "conv_mx_ar3.hip", "conv_direct.hip", "color.hip", "spixel.hip", "pool.hip", "tokens.hip", "attention.hip", "kmeans.hip", "anchor_colors.hip", "attention_mfma.hip", "diag.hip"]
 # the operators of paged caches: in the same library, but no part of the forward (bench.source_hash)
-PAGED_SOURCES = ["api_cache.cpp", "rotary.hip", "cache_pages.hip", "cache_attention.hip"]
+PAGED_SOURCES = ["api_cache.cpp", "rotary.hip", "cache_pages.hip", "cache_attention.hip", "cache_attention_precise.hip"]
 SOURCES += PAGED_SOURCES
 # per-file extra flags
 # -fno-slp-vectorize: the SLP vectoriser forms v_pk_*_f32 with op_sel (the low result half takes the HIGH dword of a source), and on this part
@@ -26,7 +26,9 @@ EXTRA_FLAGS = {"pool.hip": ["-fno-slp-vectorize"], "spixel.hip": ["-fno-slp-vect
                "attention_mfma.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 # the paged-cache kernels use no packed fp32 instruction of any form (hipcc's host pass says that it does not know the feature: harmless)
 EXTRA_FLAGS.update({f: ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] for f in PAGED_SOURCES if f.endswith(".hip")})
-EXTRA_FLAGS["cache_attention.hip"] += ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+for f in ("cache_attention.hip", "cache_attention_precise.hip"):
+    EXTRA_FLAGS[f] += ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+INCLUDED = {"cache_attention_precise.hip": ["cache_attention.hip"]}       # sources that a source includes
 PAGED_HEADERS = ["paged.h"]
 HEADERS = PAGED_HEADERS + ["common.h", "ctx.h", "plan.h", "conv_mx_kernel.h", os.path.join("..", "..", "include", "disco_hip.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -48,7 +50,7 @@ def build(force=False, verbose=True):
     for src in SOURCES:
         sp = os.path.join(CSRC, src)
         obj = os.path.join(objdir, os.path.splitext(src)[0] + ".o")
-        if force or _stale(obj, [sp, os.path.abspath(__file__)] + hdrs):        # (this file holds the flags)
+        if force or _stale(obj, [sp, os.path.abspath(__file__)] + hdrs + [os.path.join(CSRC, f) for f in INCLUDED.get(src, [])]):        # (this file holds the flags)
             jobs.append((sp, obj))
 
     def cc(job):

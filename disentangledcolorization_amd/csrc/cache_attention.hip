@@ -1008,6 +1008,46 @@ __global__ __launch_bounds__(256) void cache_attention_join_row_kernel(AttnArgs 
     put_joined<T>(a, j, t, h, d, Sum{all, y});
 }
 
+// More workgroups than are resident at once: under a causal mask tiles differ in length, and the next one, the longest that is left, goes where one has
+// ended (8 192 tokens of 32 heads of 128 on 8: 657 us with 256 workgroups of the large form, 583 with 1 024, as with 2 048, of which more lie idle in
+// a call of short sequences: the bound on units is the host's).
+unsigned grid_for(long units, long most) { return (unsigned)(units < 1 ? 1 : (units < most ? units : most)); }
+
+template <typename T, int DP, int FORM, bool REST>
+int run_many(const AttnArgs& a, long units, hipStream_t s) {
+    static_assert(many_lds<DP>() <= 65536, "more LDS has to be asked for");
+    cache_attention_many_kernel<T, DP, FORM, REST><<<grid_for(units, 1024), 2 * rows_of(FORM), many_lds<DP>(), s>>>(a);
+    DISCO_LAUNCH_CHECK("cache_attention_many_kernel");
+    return DISCO_OK;
+}
+// (units: 0 is no launch)
+template <typename T, int DP, bool REST>
+int run_many_forms(const AttnArgs& a, long many_units, long large_units, hipStream_t s) {
+    if constexpr (DP > 64 && DP <= 128) {
+        if (large_units) if (int rc = run_many<T, DP, LARGE, REST>(a, large_units, s)) return rc;
+    }
+    if (many_units) if (int rc = run_many<T, DP, MANY, REST>(a, many_units, s)) return rc;
+    return DISCO_OK;
+}
+
+#ifdef DISCO_CACHE_PRECISE
+template <typename T>
+int run_precise(const AttnArgs& a, long many_units, long large_units, hipStream_t s) {
+    if (a.dim <= 32) return run_many_forms<T, 32, true>(a, many_units, large_units, s);
+    if (a.dim <= 64) return run_many_forms<T, 64, true>(a, many_units, large_units, s);
+    if (a.dim <= 96) return run_many_forms<T, 96, true>(a, many_units, large_units, s);
+    if (a.dim <= 128) return run_many_forms<T, 128, true>(a, many_units, large_units, s);
+    if (a.dim <= 192) return run_many_forms<T, 192, true>(a, many_units, large_units, s);
+    return run_many_forms<T, 256, true>(a, many_units, large_units, s);
+}
+
+}  // namespace
+
+int launch_cache_attention_precise(const void* args, bool half, long many_units, long large_units, hipStream_t s) {
+    const AttnArgs& a = *(const AttnArgs*)args;
+    return half ? run_precise<f16>(a, many_units, large_units, s) : run_precise<bf16>(a, many_units, large_units, s);
+}
+#else
 // ---- what the host decides ----------------------------------------------------------------------------------------------------------------------
 constexpr int FEW_LIMIT = 16, MANY_LIMIT = 1024;
 constexpr long ROOM = 512l << 20;
@@ -1075,25 +1115,11 @@ Plan plan_of(const disco_cache_desc& c, const disco_attention_desc& d) {
     return p;
 }
 
-unsigned grid_for(long units, long most) { return (unsigned)(units < 1 ? 1 : (units < most ? units : most)); }
-
-// More workgroups than are resident at once: under a causal mask tiles differ in length, and the next one, the longest that is left, goes where one has
-// ended (8 192 tokens of 32 heads of 128 on 8: 657 us with 256 workgroups of the large form, 583 with 1 024, as with 2 048, of which more lie idle in
-// a call of short sequences: the bound on units is the host's).
-template <typename T, int DP, int FORM, bool REST>
-int run_many(const AttnArgs& a, long units, hipStream_t s) {
-    static_assert(many_lds<DP>() <= 65536, "more LDS has to be asked for");
-    cache_attention_many_kernel<T, DP, FORM, REST><<<grid_for(units, 1024), 2 * rows_of(FORM), many_lds<DP>(), s>>>(a);
-    DISCO_LAUNCH_CHECK("cache_attention_many_kernel");
-    return DISCO_OK;
-}
-
 template <typename T, int DP>
 int run_forms(const AttnArgs& a, const Plan& p, bool precise, hipStream_t s) {
-    if constexpr (DP > 64 && DP <= 128) {
-        if (p.large) if (int rc = precise ? run_many<T, DP, LARGE, true>(a, p.large_units, s) : run_many<T, DP, LARGE, false>(a, p.large_units, s)) return rc;
-    }
-    if (p.many) if (int rc = precise ? run_many<T, DP, MANY, true>(a, p.many_units, s) : run_many<T, DP, MANY, false>(a, p.many_units, s)) return rc;
+    const long many_units = p.many ? std::max(p.many_units, 1l) : 0, large_units = p.large ? std::max(p.large_units, 1l) : 0;
+    if (int rc = precise ? launch_cache_attention_precise(&a, std::is_same<T, f16>::value, many_units, large_units, s)
+                         : run_many_forms<T, DP, false>(a, many_units, large_units, s)) return rc;
     if (p.few) {
         cache_attention_few_kernel<T, DP><<<grid_for(p.few_units, 256 * few_waves(DP)), 256, 0, s>>>(a);
         DISCO_LAUNCH_CHECK("cache_attention_few_kernel");
@@ -1140,5 +1166,6 @@ int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc
     if (a.c < 1e-37f) a.c = 1e-37f;                                // 0 * -inf is not the score of a key that is not seen
     return c.dtype == DISCO_F16 ? run_dims<f16>(a, p, precise, s) : run_dims<bf16>(a, p, precise, s);
 }
+#endif
 
 }  // namespace disco

@@ -31,6 +31,8 @@ int launch_rotary(const disco_rotary_desc& d, const void* x, const void* positio
 int launch_cache_append(const disco_cache_desc& c, const disco_append_desc& a, const void* q, const void* k, const void* v, const int* table,
                         const int* lens, const int* cu_new, const void* positions, const double* inv_freq, void* q_out, const int* info, hipStream_t s);
 
+// args: an AttnArgs (cache_attention.hip)
+int launch_cache_attention_precise(const void* args, bool half, long many_units, long large_units, hipStream_t s);
 size_t cache_attention_ws_bytes(const disco_cache_desc& c, const disco_attention_desc& a);
 int launch_cache_attention(const disco_cache_desc& c, const disco_attention_desc& a, const void* q, const int* table, const int* lens,
                            const int* cu_new, void* out, float* lse, void* ws, bool precise, hipStream_t s);
